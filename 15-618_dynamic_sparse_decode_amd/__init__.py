@@ -26,6 +26,8 @@ LIB_PATH = BUILD_DIR / "libdsd_hip.so"
 OUTPUT_NONE, OUTPUT_OUTPUTS, OUTPUT_DEBUG = 0, 1, 2
 SCORE_CERTIFIED, SCORE_EXACT = 0, 1
 TIMING_NONE, TIMING_EVENTS = 0, 1
+KV8_E4M3, KV8_INT8 = 0, 1
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 
 class DsdError(Exception):
@@ -104,6 +106,19 @@ class AsyncStep(ctypes.Structure):
     def as_dict(self):
         return {n: (float(getattr(self, n)) if t is ctypes.c_double else int(getattr(self, n)))
                 for n, t in self._fields_}
+
+
+class Kv8Arrays(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "keys", "values", "key_scales", "value_scales", "summaries", "token_counts")]
+
+
+class Kv8BatchArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "batch", "tokens", "max_tokens", "max_pages", "total_pages", "list_stride")] + [
+        (n, ctypes.c_void_p) for n in (
+            "page_offsets", "page_counts", "page_ids", "token_offsets", "past_tokens",
+            "positions")]
 
 
 # name -> (restype, argtypes)
@@ -208,6 +223,27 @@ _SIGNATURES = {
     "dsd_dense_run_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, _c_float_p, _c_int_p,
                                            _c_int_p, _c_float_p, _c_double_p]),
     "dsd_dense_run_batch_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 5),
+    "dsd_kv8_create": (ctypes.c_int, [ctypes.c_int] * 5 + [ctypes.POINTER(Kv8Arrays),
+                                                           ctypes.POINTER(ctypes.c_void_p)]),
+    "dsd_kv8_destroy": (ctypes.c_int, [ctypes.c_void_p]),
+    "dsd_kv8_reset": (ctypes.c_int, [ctypes.c_void_p]),
+    "dsd_kv8_device_arrays": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8Arrays)]),
+    "dsd_kv8_set_rotation": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                            _c_double_p, ctypes.c_double]),
+    "dsd_kv8_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs), ctypes.c_int,
+                                      ctypes.c_int]
+                       + [ctypes.c_void_p, ctypes.c_int64] * 4 + [ctypes.c_void_p] * 2),
+    "dsd_kv8_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs), ctypes.c_int,
+                                      ctypes.c_int] + [ctypes.c_void_p, ctypes.c_int64] * 2
+                       + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
+                       + [ctypes.c_void_p] * 2),
+    "dsd_kv8_attend_prompt": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                             ctypes.c_int, ctypes.c_int]
+                              + [ctypes.c_void_p, ctypes.c_int64] * 2
+                              + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
+                              + [ctypes.c_void_p] * 2),
+    "dsd_kv8_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                               ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -843,6 +879,119 @@ def dense_run_batch_device(pool: DevicePagePool, batch, d_queries, d_cand_offset
     _check(load_library().dsd_dense_run_batch_device(pool.handle, batch, d_queries,
                                                      d_cand_offsets, d_cand_ids, d_outputs,
                                                      stream or None))
+
+
+class Kv8Batch:
+    """The requests of a call on a Kv8Cache (dsd_kv8_batch): sizes, and device
+    addresses of the page lists (page_offsets or list_stride with page_counts;
+    page_ids), the new tokens' rows (token_offsets), the tokens before them
+    (past_tokens) and, optionally, their positions."""
+
+    def __init__(self, batch: int, tokens: int = 0, max_tokens: int = 1, max_pages: int = 0,
+                 total_pages: int = 0, list_stride: int = 0, page_offsets: int = 0,
+                 page_counts: int = 0, page_ids: int = 0, token_offsets: int = 0,
+                 past_tokens: int = 0, positions: int = 0):
+        self.args = Kv8BatchArgs(batch, tokens, max_tokens, max_pages, total_pages, list_stride,
+                                 page_offsets or None, page_counts or None, page_ids or None,
+                                 token_offsets or None, past_tokens or None, positions or None)
+        self.pointer = ctypes.pointer(self.args)
+
+
+class Kv8Cache:
+    """An 8-bit paged KV cache (dsd_kv8_*): a scale per page and key head,
+    grouped query heads, float32 / bf16 / f16 rows.  arrays: device addresses
+    of the caller's memory by name (keys, values, key_scales, value_scales,
+    token_counts and, optionally, summaries); without, the cache allocates its
+    own.  Rows, batches and workspaces are device addresses; calls are
+    asynchronous on `stream`."""
+
+    def __init__(self, num_kv_heads: int, head_dim: int, page_size: int, capacity_pages: int,
+                 fmt: int = KV8_E4M3, arrays=None):
+        self._lib = load_library()
+        given = None
+        if arrays is not None:
+            given = Kv8Arrays(**{n: int(p) or None for n, p in arrays.items()})
+        handle = ctypes.c_void_p()
+        _check(self._lib.dsd_kv8_create(num_kv_heads, head_dim, page_size, capacity_pages, fmt,
+                                        given, ctypes.byref(handle)))
+        self.handle = handle
+        self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
+        self.capacity, self.format = capacity_pages, fmt
+
+    def close(self) -> None:
+        if self.handle:
+            _check(self._lib.dsd_kv8_destroy(self.handle))
+            self.handle = ctypes.c_void_p()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def reset(self) -> None:
+        _check(self._lib.dsd_kv8_reset(self.handle))
+
+    def device_arrays(self) -> dict:
+        arr = Kv8Arrays()
+        _check(self._lib.dsd_kv8_device_arrays(self.handle, ctypes.byref(arr)))
+        return {n: int(getattr(arr, n) or 0) for n, _ in arr._fields_}
+
+    def set_rotation(self, rotary_dim: int, inv_freq=(), interleaved: bool = False,
+                     magnitude: float = 1.0) -> None:
+        """Append turns dims [0, rotary_dim) of queries and keys, pair i by
+        position * inv_freq[i] radians (rotary_dim 0: not at all)."""
+        f = np.ascontiguousarray(inv_freq, dtype=np.float64)
+        if f.size != rotary_dim // 2:
+            raise InvalidArgument(1, "one inv_freq per pair of dims")
+        _check(self._lib.dsd_kv8_set_rotation(
+            self.handle, rotary_dim, int(bool(interleaved)),
+            _ptr(f, ctypes.c_double) if f.size else None, magnitude))
+
+    def append(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int, k: int,
+               k_stride: int, v: int, v_stride: int, q_out: int, q_out_stride: int, fail: int = 0,
+               stream: int = 0) -> None:
+        """Rotates and writes the batch's new tokens behind its past ones, and
+        rotates their queries into q_out (dsd_kv8_append)."""
+        status = self._lib.dsd_kv8_append(
+            self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, k, k_stride, v, v_stride,
+            q_out, q_out_stride, fail, stream)
+        if status:
+            _check(status)
+
+    def attend(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int,
+               out: int, out_stride: int, scale: float = 0.0, workspace: int = 0,
+               workspace_bytes: int = 0, fail: int = 0, stream: int = 0) -> None:
+        """Attention of one query token a request over its listed pages
+        (dsd_kv8_attend)."""
+        status = self._lib.dsd_kv8_attend(
+            self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, out, out_stride, scale,
+            workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def attend_prompt(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int,
+                      out: int, out_stride: int, scale: float = 0.0, workspace: int = 0,
+                      workspace_bytes: int = 0, fail: int = 0, stream: int = 0) -> None:
+        """Attention of a request's several query tokens, each over the tokens
+        up to its own (dsd_kv8_attend_prompt)."""
+        status = self._lib.dsd_kv8_attend_prompt(
+            self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, out, out_stride, scale,
+            workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def workspace_bytes(self, batch: Kv8Batch, num_q_heads: int) -> int:
+        out = ctypes.c_size_t()
+        _check(self._lib.dsd_kv8_workspace_bytes(self.handle, batch.pointer, num_q_heads,
+                                                 ctypes.byref(out)))
+        return out.value
 
 
 # ---------------------------------------------------------------------------

@@ -21,6 +21,7 @@
 #include "dsd_hip.h"
 #include "dsd_internal.h"
 #include "host_workers.h"
+#include "kv8.h"
 
 using dsdk::PoolView;
 
@@ -3104,6 +3105,311 @@ int dsd_dense_run_batch_device(dsd_pool* pool, int batch,
     a.scale = 1.0f / std::sqrt(static_cast<float>(pool->view.head_dim));
     a.outputs = d_outputs;
     LaunchDense(pool, &a, 0, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// 8-bit paged cache
+// ---------------------------------------------------------------------------
+struct dsd_kv8 {
+  dsdk::Kv8View view;
+  bool owned = false;  // the arrays are the handle's
+  int device = 0;
+  dsdk::Kv8Rotation rotation;
+  DeviceBuffer<double> turns;
+
+  ~dsd_kv8() {
+    if (!owned) return;
+    if (view.keys) (void)hipFree(view.keys);
+    if (view.values) (void)hipFree(view.values);
+    if (view.key_scales) (void)hipFree(view.key_scales);
+    if (view.value_scales) (void)hipFree(view.value_scales);
+    if (view.summaries) (void)hipFree(view.summaries);
+    if (view.token_counts) (void)hipFree(view.token_counts);
+  }
+
+  void RequireCurrent() const {
+    int now = 0;
+    DSD_HIP_CHECK(hipGetDevice(&now));
+    Require(now == device, "the cache's device must be the current one");
+  }
+};
+
+namespace {
+
+// A batch's sizes and pointers, as the calls need them (tokens: with new ones).
+void RequireKv8Batch(const dsd_kv8* cache, const dsd_kv8_batch* b, bool tokens) {
+  Require(cache != nullptr && b != nullptr, "cache and batch must be non-null");
+  cache->RequireCurrent();
+  Require(b->batch >= 0 && b->tokens >= 0 && b->max_tokens >= 0 && b->max_pages >= 0 &&
+              b->total_pages >= 0 && b->list_stride >= 0,
+          "sizes must be non-negative");
+  if (b->batch == 0) return;
+  Require(b->batch <= 65535, "at most 65535 requests per call");
+  if (b->list_stride > 0) {
+    Require(static_cast<int64_t>(b->batch) * b->list_stride <= 0x7fffffff,
+            "batch * list_stride must fit 31 bits");
+    Require(b->page_counts != nullptr, "page_counts must be non-null");
+  } else {
+    Require(b->page_offsets != nullptr, "page_offsets must be non-null");
+  }
+  Require(b->total_pages == 0 || b->page_ids != nullptr, "page_ids must be non-null");
+  // (the kernels read page 0 in place of none)
+  Require(b->total_pages == 0 || cache->view.capacity > 0, "the cache holds no page");
+  if (tokens) {
+    Require(b->token_offsets != nullptr && b->past_tokens != nullptr,
+            "token_offsets and past_tokens must be non-null");
+    Require(b->tokens == 0 || b->max_tokens > 0, "max_tokens must be positive");
+  }
+}
+
+size_t TypeSize(int type) {
+  Require(type == DSD_TYPE_F32 || type == DSD_TYPE_BF16 || type == DSD_TYPE_F16,
+          "type must be DSD_TYPE_F32, DSD_TYPE_BF16 or DSD_TYPE_F16");
+  return type == DSD_TYPE_F32 ? 4 : 2;
+}
+
+// Rows of `heads` heads at p, `stride` elements apart.
+void RequireRows(const dsd_kv8* cache, const void* p, int64_t stride, int heads, size_t size) {
+  Require(p != nullptr, "rows must be non-null");
+  Require(reinterpret_cast<uintptr_t>(p) % size == 0, "rows must be aligned to their type");
+  Require(stride >= static_cast<int64_t>(heads) * cache->view.dim,
+          "a row stride is at least the row");
+}
+
+void RequireHeads(const dsd_kv8* cache, int q_heads) {
+  Require(q_heads >= 0 && q_heads % cache->view.heads == 0,
+          "num_q_heads must be a multiple of num_kv_heads");
+  // (a launch's first dimension counts its heads)
+  Require(q_heads <= 65536, "at most 65536 query heads");
+}
+
+int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, bool causal, int type, int num_q_heads,
+              const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
+              void* workspace, size_t workspace_bytes, unsigned long long* d_fail, void* stream) {
+  return Guard([&] {
+    RequireKv8Batch(cache, batch, causal);
+    const size_t size = TypeSize(type);
+    RequireHeads(cache, num_q_heads);
+    Require(num_q_heads > 0, "num_q_heads must be positive");
+    if (batch->batch == 0 || (causal && batch->tokens == 0)) return;
+    RequireRows(cache, q, q_stride, num_q_heads, size);
+    RequireRows(cache, out, out_stride, num_q_heads, size);
+    Require(std::isfinite(scale), "scale must be finite");
+    Require(workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+            "the workspace must be 16-byte aligned");
+    dsdk::Kv8AttendArgs a;
+    a.c = cache->view;
+    a.b = *batch;
+    a.type = type;
+    a.q_heads = num_q_heads;
+    a.causal = causal;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->view.dim));
+    a.workspace = workspace;
+    a.workspace_bytes = workspace != nullptr ? workspace_bytes : 0;
+    a.fail.word = d_fail;
+    dsdk::LaunchKv8Attend(a, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_pages, int format,
+                   const dsd_kv8_arrays* arrays, dsd_kv8** out_cache) {
+  return Guard([&] {
+    Require(out_cache != nullptr, "out_cache must be non-null");
+    *out_cache = nullptr;
+    Require(capacity_pages >= 0, "capacity_pages must be non-negative");
+    Require(num_kv_heads > 0 && num_kv_heads <= 4096, "num_kv_heads must be in [1, 4096]");
+    Require(head_dim > 0 && head_dim <= 256 && head_dim % 16 == 0,
+            "head_dim must be a multiple of 16 up to 256");
+    Require(page_size > 0 && page_size <= 256 && page_size % 16 == 0,
+            "page_size must be a multiple of 16 up to 256");
+    // (a page's scales are indexed by 32 bits)
+    Require(static_cast<int64_t>(capacity_pages) * num_kv_heads <= 0x7fffffff,
+            "capacity_pages * num_kv_heads must fit 31 bits");
+    Require(format == DSD_KV8_E4M3 || format == DSD_KV8_INT8,
+            "format must be DSD_KV8_E4M3 or DSD_KV8_INT8");
+    if (arrays != nullptr && capacity_pages > 0) {
+      const void* all[] = {arrays->keys, arrays->values, arrays->key_scales, arrays->value_scales,
+                           arrays->token_counts};
+      for (const void* p : all) Require(p != nullptr, "cache arrays must be non-null");
+      for (const void* p : all) {
+        Require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "cache arrays must be 16-byte aligned");
+      }
+      Require(reinterpret_cast<uintptr_t>(arrays->summaries) % 16 == 0,
+              "cache arrays must be 16-byte aligned");
+    }
+    if (!dsd_gpu_available()) throw std::runtime_error("no visible gfx950 GPU");
+    auto cache = std::make_unique<dsd_kv8>();
+    DSD_HIP_CHECK(hipGetDevice(&cache->device));
+    dsdk::Kv8View& v = cache->view;
+    v.heads = num_kv_heads;
+    v.dim = head_dim;
+    v.page = page_size;
+    v.chunks = page_size / 16;
+    v.capacity = capacity_pages;
+    v.format = format;
+    if (arrays != nullptr) {
+      v.keys = arrays->keys;
+      v.values = arrays->values;
+      v.key_scales = arrays->key_scales;
+      v.value_scales = arrays->value_scales;
+      v.summaries = arrays->summaries;
+      v.token_counts = arrays->token_counts;
+    } else if (capacity_pages > 0) {
+      cache->owned = true;
+      const size_t page_heads = static_cast<size_t>(capacity_pages) * num_kv_heads;
+      const size_t codes = page_heads * page_size * head_dim;
+      auto make = [](auto** p, size_t bytes) {
+        DSD_HIP_CHECK(hipMalloc(reinterpret_cast<void**>(p), bytes));
+        DSD_HIP_CHECK(hipMemset(*p, 0, bytes));
+      };
+      make(&v.keys, codes);
+      make(&v.values, codes);
+      make(&v.key_scales, page_heads * sizeof(float));
+      make(&v.value_scales, page_heads * sizeof(float));
+      make(&v.summaries, page_heads * head_dim * sizeof(float));
+      make(&v.token_counts, static_cast<size_t>(capacity_pages) * sizeof(int));
+      DSD_HIP_CHECK(hipDeviceSynchronize());
+    }
+    dsdk::PreloadKv8Append(v);
+    dsdk::PreloadKv8Attend(v);
+    *out_cache = cache.release();
+  });
+}
+
+int dsd_kv8_destroy(dsd_kv8* cache) {
+  return Guard([&] {
+    if (cache == nullptr) return;
+    (void)hipDeviceSynchronize();
+    delete cache;
+  });
+}
+
+int dsd_kv8_reset(dsd_kv8* cache) {
+  return Guard([&] {
+    Require(cache != nullptr, "cache must be non-null");
+    cache->RequireCurrent();
+    DSD_HIP_CHECK(hipDeviceSynchronize());
+    if (cache->view.capacity > 0) {
+      DSD_HIP_CHECK(hipMemset(cache->view.token_counts, 0,
+                              sizeof(int) * static_cast<size_t>(cache->view.capacity)));
+      DSD_HIP_CHECK(hipDeviceSynchronize());
+    }
+  });
+}
+
+int dsd_kv8_device_arrays(const dsd_kv8* cache, dsd_kv8_arrays* out) {
+  return Guard([&] {
+    Require(cache != nullptr && out != nullptr, "cache and out must be non-null");
+    const dsdk::Kv8View& v = cache->view;
+    out->keys = v.keys;
+    out->values = v.values;
+    out->key_scales = v.key_scales;
+    out->value_scales = v.value_scales;
+    out->summaries = v.summaries;
+    out->token_counts = v.token_counts;
+  });
+}
+
+int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved, const double* inv_freq,
+                         double magnitude) {
+  return Guard([&] {
+    Require(cache != nullptr, "cache must be non-null");
+    cache->RequireCurrent();
+    Require(rotary_dim >= 0 && rotary_dim <= cache->view.dim && rotary_dim % 16 == 0,
+            "rotary_dim must be a multiple of 16 up to head_dim");
+    Require(rotary_dim == 0 || inv_freq != nullptr, "inv_freq must be non-null");
+    Require(interleaved == 0 || interleaved == 1, "interleaved must be 0 or 1");
+    Require(std::isfinite(magnitude), "magnitude must be finite");
+    const int pairs = rotary_dim / 2;
+    std::vector<double> turns(static_cast<size_t>(pairs));
+    for (int i = 0; i < pairs; ++i) {
+      Require(std::isfinite(inv_freq[i]), "inv_freq must be finite");
+      turns[i] = static_cast<double>(inv_freq[i] / 3.14159265358979323846264338327950288L);
+    }
+    DSD_HIP_CHECK(hipDeviceSynchronize());
+    if (pairs > 0) {
+      cache->turns.Reserve(static_cast<size_t>(pairs));
+      DSD_HIP_CHECK(hipMemcpy(cache->turns.ptr, turns.data(), sizeof(double) * turns.size(),
+                              hipMemcpyHostToDevice));
+    }
+    cache->rotation.turns = cache->turns.ptr;
+    cache->rotation.pairs = pairs;
+    cache->rotation.interleaved = interleaved;
+    cache->rotation.magnitude = magnitude;
+  });
+}
+
+int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num_q_heads,
+                   const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                   const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride,
+                   unsigned long long* d_fail, void* stream) {
+  return Guard([&] {
+    RequireKv8Batch(cache, batch, true);
+    const size_t size = TypeSize(type);
+    RequireHeads(cache, num_q_heads);
+    if (batch->batch == 0 || batch->tokens == 0) return;
+    Require(batch->total_pages > 0, "the requests' lists hold no page");
+    RequireRows(cache, k, k_stride, cache->view.heads, size);
+    RequireRows(cache, v, v_stride, cache->view.heads, size);
+    if (num_q_heads > 0) {
+      RequireRows(cache, q, q_stride, num_q_heads, size);
+      RequireRows(cache, q_out, q_out_stride, num_q_heads, size);
+    }
+    dsdk::Kv8AppendArgs a;
+    a.c = cache->view;
+    a.rot = cache->rotation;
+    a.b = *batch;
+    a.type = type;
+    a.q_heads = num_q_heads;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.out_stride = q_out_stride;
+    a.fail.word = d_fail;
+    dsdk::LaunchKv8Append(a, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int dsd_kv8_attend(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num_q_heads,
+                   const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
+                   void* workspace, size_t workspace_bytes, unsigned long long* d_fail,
+                   void* stream) {
+  return AttendKv8(cache, batch, false, type, num_q_heads, q, q_stride, out, out_stride, scale,
+                   workspace, workspace_bytes, d_fail, stream);
+}
+
+int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num_q_heads,
+                          const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                          float scale, void* workspace, size_t workspace_bytes,
+                          unsigned long long* d_fail, void* stream) {
+  return AttendKv8(cache, batch, true, type, num_q_heads, q, q_stride, out, out_stride, scale,
+                   workspace, workspace_bytes, d_fail, stream);
+}
+
+int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int num_q_heads,
+                            size_t* bytes) {
+  return Guard([&] {
+    Require(cache != nullptr && batch != nullptr && bytes != nullptr,
+            "cache, batch and bytes must be non-null");
+    Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0,
+            "sizes must be non-negative");
+    RequireHeads(cache, num_q_heads);
+    *bytes = num_q_heads > 0 ? dsdk::Kv8WorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
   });
 }
 

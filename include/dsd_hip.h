@@ -619,6 +619,146 @@ int dsd_dense_run_batch_device(dsd_pool* pool, int batch,
                                const int* d_cand_ids, float* d_outputs,
                                void* stream);
 
+/* ---- 8-bit paged cache -------------------------------------------------- */
+/* A second form of paged cache, for models whose projections are 16-bit and
+ * whose query heads share key heads: K and V are 8-bit codes with one float32
+ * scale for each page and key head (the stored value is code * scale), a
+ * quarter of dsd_pool's bytes.  No counterpart in the reference, whose cache
+ * is float32 with one key head per query head.
+ *
+ * Memory, owned by the handle or handed in by the caller (page p, key head h,
+ * token t of the page, dim d; P = page_size, K = num_kv_heads, D = head_dim):
+ *   keys          uint8[capacity][K][P][D]
+ *   values        uint8[capacity][K][P / 16][D][16]   (token t is t % 16 of
+ *                                                      group t / 16)
+ *   key_scales, value_scales   float[capacity][K]
+ *   summaries     float[capacity][K * D], mean of the page's stored keys
+ *   token_counts  int32[capacity]
+ * Codes are OCP e4m3 (DSD_KV8_E4M3) or two's complement in [-127, 127]
+ * (DSD_KV8_INT8).  A page's scale is the least that its largest finite number
+ * fits: of int8 codes that number / 127 (rounded to float), of e4m3 codes a
+ * power of two (its own exponent bits make up for it, and quotients by it are
+ * exact), never below 2^-126.
+ *
+ * The calls only enqueue work on `stream` (a hipStream_t; NULL = the default
+ * stream) of the cache's device, which must be the current one, and may be
+ * captured into a graph.  They allocate nothing and keep nothing between
+ * calls, so calls on several streams are independent as far as their memory
+ * is.  d_fail (may be NULL): memory the device writes
+ * a code to when it skips a request: 2 its offsets or lengths do not fit the
+ * batch's sizes, 3 a page id outside the cache; the caller clears it before
+ * and reads it after the call.  Nothing outside the arrays is touched then. */
+typedef struct dsd_kv8 dsd_kv8;
+
+enum { DSD_KV8_E4M3 = 0, DSD_KV8_INT8 = 1 };
+enum { DSD_TYPE_F32 = 0, DSD_TYPE_BF16 = 1, DSD_TYPE_F16 = 2 };
+
+typedef struct dsd_kv8_arrays {
+  unsigned char* keys;
+  unsigned char* values;
+  float* key_scales;
+  float* value_scales;
+  float* summaries; /* NULL: the cache keeps no page means */
+  int* token_counts;
+} dsd_kv8_arrays;
+
+/* head_dim a multiple of 16 up to 256, page_size a multiple of 16 up to 256.
+ * arrays NULL: the cache allocates its memory (with summaries), zeroed;
+ * otherwise device memory of the sizes above, 16-byte aligned, that the
+ * caller has filled or zeroed and that outlives the handle. */
+int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size,
+                   int capacity_pages, int format, const dsd_kv8_arrays* arrays,
+                   dsd_kv8** out_cache);
+int dsd_kv8_destroy(dsd_kv8* cache);
+/* Every token count zero (synchronous).  Codes and scales may stay: an append
+ * at a page's first token starts the page anew. */
+int dsd_kv8_reset(dsd_kv8* cache);
+int dsd_kv8_device_arrays(const dsd_kv8* cache, dsd_kv8_arrays* out);
+
+/* The rotation of dsd_kv8_append: dims [0, rotary_dim) of a head are turned in
+ * pairs, pair i by position * inv_freq[i] radians and times magnitude; the
+ * other dims pass.  rotary_dim a multiple of 16, 0 (no rotation, the state
+ * after creation) to head_dim; interleaved 0: pair i is dims (i, i +
+ * rotary_dim / 2), 1: (2 i, 2 i + 1).  inv_freq: rotary_dim / 2 host doubles.
+ * Angles and products are 64-bit, so positions of millions keep their
+ * angles.  Synchronous; not while a call on the cache runs. */
+int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved,
+                         const double* inv_freq, double magnitude);
+
+/* The requests of a call.  Pointers are device memory.  The sizes bound what
+ * the device data says; a request beyond them is skipped (d_fail). */
+typedef struct dsd_kv8_batch {
+  int batch;       /* requests */
+  int tokens;      /* rows of q, k, v and out */
+  int max_tokens;  /* most new (query) tokens of one request */
+  int max_pages;   /* most pages of one request's list: a hint that sizes the
+                      launch; longer lists are read whole all the same */
+  int total_pages; /* entries of page_ids */
+  int list_stride; /* 0: request r's list is page_ids[page_offsets[r] ..
+                      page_offsets[r + 1]); else page_counts[r] ids from
+                      r * list_stride on (dsd_sparse_run_batch_device's
+                      selected and selected_counts) */
+  const int* page_offsets;  /* [batch + 1] */
+  const int* page_counts;   /* [batch] */
+  const int* page_ids;
+  const int* token_offsets; /* [batch + 1]: request r's rows; unused by
+                               dsd_kv8_attend (row r) */
+  const int* past_tokens;   /* [batch]: tokens of the request before its new
+                               ones; unused by dsd_kv8_attend */
+  const int* positions;     /* [tokens] for the rotation; NULL: a token's index
+                               in its request */
+} dsd_kv8_batch;
+
+/* Writes each request's new tokens behind its past ones: token i of request r
+ * has index j = past_tokens[r] + i and goes to token j % P of page j / P of
+ * the request's list.  Keys are rotated, then both sides are quantised: a
+ * page's scale is the greater of the one it has (where the request already
+ * has tokens in the page) and the one its new tokens need; where it grows,
+ * the codes before are brought to it, each rounded once more.  Codes are the
+ * nearest to value / scale (halves to the even one); infinities become the
+ * largest code, NaN stays NaN in e4m3 and becomes 0 in int8.  token_counts of
+ * the page becomes its tokens up to the last one written, its summary their
+ * mean; tokens behind that stay as they were.  Writing a token again gives
+ * the same page.  A page takes tokens of one request per call.
+ * Queries: num_q_heads heads a token are rotated into q_out in their own type
+ * (q_out may be q with the same stride); num_q_heads 0: none.
+ * Rows: token i of q is num_q_heads * D elements from q + i * q_stride on
+ * (strides in elements, at least the row; any alignment of the element). */
+int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
+                   int num_q_heads, const void* q, int64_t q_stride,
+                   const void* k, int64_t k_stride, const void* v,
+                   int64_t v_stride, void* q_out, int64_t q_out_stride,
+                   unsigned long long* d_fail, void* stream);
+
+/* Attention of one query token a request over every token of its list's pages
+ * (token_counts each): out = softmax(scale * q K^T) V.  num_q_heads is a
+ * multiple of num_kv_heads; query head h reads key head h / (num_q_heads /
+ * num_kv_heads).  scale 0: 1 / sqrt(D).  A request without tokens gets zeros.
+ * Logits, sums and outputs before their one rounding are float32; out has q's
+ * type.  Row r of q and out is request r.
+ * workspace (16-byte aligned): dsd_kv8_workspace_bytes of device memory lets
+ * long lists spread over workgroups; calls that may overlap (streams, graphs)
+ * need one each.  NULL or smaller: the lists are not spread. */
+int dsd_kv8_attend(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
+                   int num_q_heads, const void* q, int64_t q_stride, void* out,
+                   int64_t out_stride, float scale, void* workspace,
+                   size_t workspace_bytes, unsigned long long* d_fail,
+                   void* stream);
+
+/* The same for several query tokens a request (a prompt, a chunk of one,
+ * drafted tokens): query token i of request r has index past_tokens[r] + i and
+ * attends to the request's tokens up to and with that index, which the cache
+ * holds already (token_counts is not read). */
+int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
+                          int num_q_heads, const void* q, int64_t q_stride,
+                          void* out, int64_t out_stride, float scale,
+                          void* workspace, size_t workspace_bytes,
+                          unsigned long long* d_fail, void* stream);
+/* Workspace of dsd_kv8_attend and dsd_kv8_attend_prompt for batches of at most
+ * these sizes (the pointers are not read). */
+int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                            int num_q_heads, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
