@@ -119,33 +119,29 @@ __device__ __forceinline__ bool FindSpan(const Kv8AttendArgs& a, const Plan& p, 
   return true;
 }
 
-// One 16-token chunk of a request's list.
-struct Chunk {
-  int64_t at = 0;    // its first token's key, as (page * heads + head) * page size + token
-  int scale = 0;     // index of its scales
-  int tokens = 0;    // its tokens in the cache
-  int begin = 0;     // its first token's index
+// One page of a request's list, staged in LDS.
+struct PageInfo {
+  int page;     // (0 for one that holds no token)
+  int tokens;   // in the cache
+  float key_scale;
+  float value_scale;
 };
+constexpr int kStage = 512;  // pages staged at a time
 
-__device__ __forceinline__ Chunk FindChunk(const Kv8AttendArgs& a, const Span& s, int head, int i) {
+__device__ __forceinline__ PageInfo ReadPage(const Kv8AttendArgs& a, const Span& s, int head,
+                                             int slot) {
   const Kv8View& c = a.c;
-  Chunk k;
-  const int slot = i / c.chunks, sub = i - slot * c.chunks;
-  int page = 0;
-  bool ok = i < s.chunks;
-  if (ok) {
-    page = a.b.page_ids[s.q.list + slot];
-    ok = InPool(page, c.capacity);
-    if (!ok) ReportFailure(a.fail, kFailPageId);
-  }
-  page = ok ? page : 0;
-  k.begin = i * 16;
-  if (ok) {
-    k.tokens = a.causal ? s.q.past + s.q.n - k.begin : c.token_counts[page] - sub * 16;
-    k.tokens = min(max(k.tokens, 0), 16);
-  }
-  k.scale = page * c.heads + head;
-  k.at = static_cast<int64_t>(k.scale) * c.page + sub * 16;
+  PageInfo k;
+  k.page = a.b.page_ids[s.q.list + slot];
+  const bool ok = InPool(k.page, c.capacity);
+  if (!ok) ReportFailure(a.fail, kFailPageId);
+  k.page = ok ? k.page : 0;
+  k.tokens = 0;
+  if (ok) k.tokens = a.causal ? s.q.past + s.q.n - slot * c.page : c.token_counts[k.page];
+  k.tokens = min(max(k.tokens, 0), c.page);
+  const int at = k.page * c.heads + head;
+  k.key_scale = k.tokens > 0 ? c.key_scales[at] : 1.0f;
+  k.value_scale = k.tokens > 0 ? fmaxf(c.value_scales[at], kKv8Tiny) : 1.0f;
   return k;
 }
 
@@ -162,11 +158,13 @@ constexpr int kWeightTerms = std::is_same<T, __bf16>::value ? 1 : 2;
 // operand of O^T = V^T P^T as they stand (the order of a product's inner index
 // is free), whose first operand, 16 tokens of one dim, is one load of the
 // values' layout.  No number crosses lanes but for the maxima.
-template <typename T, int FMT, int NU, int W>
+// kDim: head_dim where it is 64 * NU (no bounds tests), else 0.
+template <typename T, int FMT, int NU, int kDim, int W>
 __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Plan p) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>, NT = 4 * NU;
+  extern __shared__ __align__(16) float lds[];
   const Kv8View& c = a.c;
-  const int D = c.dim, tiles = D / 16;
+  const int D = kDim > 0 ? kDim : c.dim, tiles = kDim > 0 ? NT : D / 16;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int n = lane & 15, g = lane >> 4;
   const int r = blockIdx.y, head = blockIdx.x % c.heads;
@@ -184,7 +182,7 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
   const int token = there ? row / p.group : 0;
   const int q_head = head * p.group + (there ? row - token * p.group : 0);
   F16x8 q[NU][2][NQ];
-  float to_logit;  // what a product with codes lacks but the page's scale
+  float to_logit;  // what a product with codes lacks but the page's scale; >= 0
   {
     const T* qp = static_cast<const T*>(a.q) + (s.q.row0 + token) * a.q_stride +
                   static_cast<int64_t>(q_head) * D;
@@ -210,8 +208,9 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
     int e = 0;
     (void)frexpf(most, &e);
     e = most > 0.0f ? max(min(14 - e, 126), -126) : 0;
-    const float up = __uint_as_float(static_cast<unsigned>(e + 127) << 23);
-    to_logit = a.scale * kLog2e * __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+    const float up = copysignf(__uint_as_float(static_cast<unsigned>(e + 127) << 23), a.scale);
+    to_logit =
+        fabsf(a.scale) * kLog2e * __uint_as_float(static_cast<unsigned>(127 - e) << 23);
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
@@ -234,156 +233,213 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
   float m = -INFINITY, l = 0.0f;
   float mv = -INFINITY;  // of s + log2(value scale): acc is relative to it
   bool seen = false;
-  for (int grp = begin + wave; grp < end; grp += W) {
-    const Chunk kc = FindChunk(a, s, head, 4 * grp + (n >> 2));
-    const Chunk vc = FindChunk(a, s, head, 4 * grp + g);
-    uint4 kw[4][NU], vw[NT];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const int d = (g + 4 * u) * 16;
-        kw[t][u] = make_uint4(0, 0, 0, 0);
-        if (d < D) {
-          kw[t][u] = *reinterpret_cast<const uint4*>(c.keys + (kc.at + 4 * t + (n & 3)) * D + d);
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t < tiles) {
-        vw[t] = *reinterpret_cast<const uint4*>(c.values + vc.at * D + (16 * t + n) * 16);
-      }
-    }
-    const float key_scale = c.key_scales[vc.scale];
-    const float value_scale = vc.tokens > 0 ? fmaxf(c.value_scales[vc.scale], kKv8Tiny) : 1.0f;
 
-    F32x4 x[4];
+  // The list's pages are staged in LDS, so that a group's addresses are known
+  // before its turn: its keys are asked for as soon as the logits of the group
+  // before have taken their registers' contents, its values after the products.
+  PageInfo* info = reinterpret_cast<PageInfo*>(lds);
+  const int per_stage = max((kStage - 2) * c.chunks / 4, 1);  // groups
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
+  const int page_bytes = c.page * D;
+  uint4 kw[4][NU], vw[NT];
+  for (int g0 = begin; g0 < end; g0 += per_stage) {
+    const int g1 = min(end, g0 + per_stage);
+    const int slot0 = 4 * g0 / c.chunks;
+    const int slots = (min(4 * g1, s.chunks) - 1) / c.chunks + 1 - slot0;
+    if (g0 > begin) __syncthreads();
+    for (int i = threadIdx.x; i < slots; i += W * kWave) {
+      info[i] = ReadPage(a, s, head, slot0 + i);
+    }
+    __syncthreads();
+    // Chunk i of the list: its place among the staged ones, its part of the page.
+    auto place = [&](int i, int* sub) {
+      const int slot = c.chunks == 1 ? i : static_cast<int>(__umulhi(i, inverse));
+      *sub = i - slot * c.chunks;
+      return min(slot - slot0, slots - 1);
+    };
+    auto load_keys = [&](int grp) {
+      int sub;
+      const int page = info[place(4 * grp + (n >> 2), &sub)].page;
+      const uint8_t* kp = c.keys + static_cast<int64_t>(page * c.heads + head) * page_bytes +
+                          (sub * 16 + (n & 3)) * D + g * 16;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      x[t] = F32x4{0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const F16x8 k0 = Numbers8<FMT>(kw[t][u].x, kw[t][u].y);
-        const F16x8 k1 = Numbers8<FMT>(kw[t][u].z, kw[t][u].w);
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[u][0][i], x[t], 0, 0, 0);
-          x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[u][1][i], x[t], 0, 0, 0);
+        for (int u = 0; u < NU; ++u) {
+          if (kDim > 0 || (g + 4 * u) * 16 < D) {
+            kw[t][u] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + 64 * u);
+          } else {
+            kw[t][u] = make_uint4(0, 0, 0, 0);
+          }
         }
       }
-    }
-
-    // Row n's tokens of the chunk: those in the cache that it sees.
-    const int count = min(vc.tokens, sees - vc.begin);
-    const bool whole = __ballot(count < 16) == 0;
-    const float f = to_logit * key_scale;
-    float most = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[t][i] *= f;
-        if (!whole && 4 * t + i >= count) x[t][i] = -INFINITY;
-        most = fmaxf(most, x[t][i]);
-      }
-    }
-    seen = seen || count > 0;
-    const float m_new = fmaxf(m, Max4(most));
-    const float mv_new = fmaxf(mv, Max4(most + __builtin_amdgcn_logf(value_scale)));
-    const float base = m_new == -INFINITY ? 0.0f : m_new;
-    const float base_v = mv_new == -INFINITY ? 0.0f : mv_new;
-    const float shrink = Exp2(m - base);
-    const float shrink_acc = Exp2(mv - base_v);
-    const float to_half = value_scale * Exp2(base - base_v + kWeightBits);
-    m = m_new;
-    mv = mv_new;
-    l *= shrink;
-    F16x8 w[2][NP];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = Exp2(x[t][i] - base);
-        l += e;
-        const float y = e * to_half;
-        const _Float16 hi = static_cast<_Float16>(y);
-        w[t >> 1][0][4 * (t & 1) + i] = hi;
-        if constexpr (NP == 2) {
-          w[t >> 1][1][4 * (t & 1) + i] = static_cast<_Float16>(y - static_cast<float>(hi));
-        }
-      }
-    }
-    // Codes behind a request's tokens may be anything, and 0 * NaN is not 0.
-    if (!whole) {
+    };
+    PageInfo now;   // the values' page, and its tokens from the chunk's first on
+    auto load_values = [&](int grp) {
+      int sub;
+      now = info[place(4 * grp + g, &sub)];
+      now.tokens = 4 * grp + g < s.chunks ? now.tokens - sub * 16 : 0;
+      const uint8_t* vp = c.values +
+                          static_cast<int64_t>(now.page * c.heads + head) * page_bytes +
+                          (sub * D + n) * 16;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        unsigned* word = reinterpret_cast<unsigned*>(&vw[t]);
+        if (t < tiles) vw[t] = *reinterpret_cast<const uint4*>(vp + 256 * t);
+      }
+    };
+    int grp = g0 + wave;
+    if (grp < g1) {
+      load_keys(grp);
+      load_values(grp);
+    }
+    for (; grp < g1; grp += W) {
+      const bool more = grp + W < g1;
+      F32x4 x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int have = min(max(vc.tokens - 4 * i, 0), 4);
-          word[i] &= have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1u;
+      for (int t = 0; t < 4; ++t) {
+        x[t] = F32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const F16x8 k0 = Numbers8<FMT>(kw[t][u].x, kw[t][u].y);
+          const F16x8 k1 = Numbers8<FMT>(kw[t][u].z, kw[t][u].w);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[u][0][i], x[t], 0, 0, 0);
+            x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[u][1][i], x[t], 0, 0, 0);
+          }
         }
       }
-      // Nor may NaN codes of tokens that only later rows see reach the others:
-      // they are taken out, and the rows that see one get NaN.
-      if (FMT == DSD_KV8_E4M3 && a.causal) {
-        bool nan = false;
+      if (more) load_keys(grp + W);
+
+      // Row n's tokens of the chunk: those in the cache that it sees.
+      const int count = min(now.tokens, sees - (4 * grp + g) * 16);
+      const bool whole = __ballot(count < 16) == 0;
+      if (!whole) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (t < tiles) {
-            nan = nan || ((NanBytes(vw[t].x) | NanBytes(vw[t].y)) |
-                          (NanBytes(vw[t].z) | NanBytes(vw[t].w))) != 0u;
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (4 * t + i >= count) x[t][i] = -INFINITY;
           }
         }
-        if (__ballot(nan) != 0) {
-          F16x8 visible[2];
+      }
+      const float f = fmaxf(to_logit * now.key_scale, kKv8Tiny);
+      float most = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            visible[i >> 3][i & 7] = static_cast<_Float16>(i < count ? 1.0f : 0.0f);
+      for (int t = 0; t < 4; ++t) {
+        most = fmaxf(most, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+      }
+      most *= f;
+      seen = seen || count > 0;
+      const float m_new = fmaxf(m, Max4(most));
+      const float mv_new = fmaxf(mv, Max4(most + __builtin_amdgcn_logf(now.value_scale)));
+      const float base = m_new == -INFINITY ? 0.0f : m_new;
+      const float base_v = mv_new == -INFINITY ? 0.0f : mv_new;
+      if (__ballot(m_new > m || mv_new > mv) != 0) {
+        l *= Exp2(m - base);
+        const float shrink = Exp2(mv - base_v);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] *= shrink;
+        m = m_new;
+        mv = mv_new;
+      }
+      const float to_half = now.value_scale * Exp2(base - base_v + kWeightBits);
+      F16x8 w[2][NP];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = Exp2(fmaf(x[t][i], f, -base));
+          l += e;
+          y[i] = e * to_half;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const F32x2 pair = {y[i], y[i + 1]};
+          const F16x2 hi = __builtin_convertvector(pair, F16x2);
+          w[t >> 1][0][4 * (t & 1) + i] = hi[0];
+          w[t >> 1][0][4 * (t & 1) + i + 1] = hi[1];
+          if constexpr (NP == 2) {
+            const F32x2 rest = {y[i] - static_cast<float>(hi[0]),
+                                y[i + 1] - static_cast<float>(hi[1])};
+            const F16x2 lo = __builtin_convertvector(rest, F16x2);
+            w[t >> 1][1][4 * (t & 1) + i] = lo[0];
+            w[t >> 1][1][4 * (t & 1) + i + 1] = lo[1];
           }
+        }
+      }
+      if (!whole) {
+        // Codes behind a request's tokens may be anything, and 0 * NaN is not 0.
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          unsigned* word = reinterpret_cast<unsigned*>(&vw[t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int have = min(max(now.tokens - 4 * i, 0), 4);
+            word[i] &= have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1u;
+          }
+        }
+        // Nor may NaN codes of tokens that only later rows see reach the others:
+        // they are taken out, and the rows that see one get NaN.
+        if (FMT == DSD_KV8_E4M3 && a.causal) {
+          bool nan = false;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             if (t < tiles) {
-              unsigned* word = reinterpret_cast<unsigned*>(&vw[t]);
-              unsigned ones[4];
+              nan = nan || ((NanBytes(vw[t].x) | NanBytes(vw[t].y)) |
+                            (NanBytes(vw[t].z) | NanBytes(vw[t].w))) != 0u;
+            }
+          }
+          if (__ballot(nan) != 0) {
+            F16x8 visible[2];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const unsigned bytes = (NanBytes(word[i]) >> 7) * 0xffu;
-                ones[i] = bytes & 0x38383838u;  // 1.0
-                word[i] &= ~bytes;
-              }
-              F32x4 hits = {0, 0, 0, 0};
-              hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(Numbers8<FMT>(ones[0], ones[1]),
-                                                            visible[0], hits, 0, 0, 0);
-              hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(Numbers8<FMT>(ones[2], ones[3]),
-                                                            visible[1], hits, 0, 0, 0);
+            for (int i = 0; i < 16; ++i) {
+              visible[i >> 3][i & 7] = static_cast<_Float16>(i < count ? 1.0f : 0.0f);
+            }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (hits[i] > 0.0f) acc[t][i] = __builtin_nanf("");
+            for (int t = 0; t < NT; ++t) {
+              if (t < tiles) {
+                unsigned* word = reinterpret_cast<unsigned*>(&vw[t]);
+                unsigned ones[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const unsigned bytes = (NanBytes(word[i]) >> 7) * 0xffu;
+                  ones[i] = bytes & 0x38383838u;  // 1.0
+                  word[i] &= ~bytes;
+                }
+                F32x4 hits = {0, 0, 0, 0};
+                hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(Numbers8<FMT>(ones[0], ones[1]),
+                                                              visible[0], hits, 0, 0, 0);
+                hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(Numbers8<FMT>(ones[2], ones[3]),
+                                                              visible[1], hits, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if (hits[i] > 0.0f) acc[t][i] = __builtin_nanf("");
+                }
               }
             }
           }
         }
       }
-    }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t < tiles) {
-        acc[t] *= shrink_acc;
-        const F16x8 v0 = Numbers8<FMT>(vw[t].x, vw[t].y);
-        const F16x8 v1 = Numbers8<FMT>(vw[t].z, vw[t].w);
+      for (int t = 0; t < NT; ++t) {
+        if (t < tiles) {
+          const F16x8 v0 = Numbers8<FMT>(vw[t].x, vw[t].y);
+          const F16x8 v1 = Numbers8<FMT>(vw[t].z, vw[t].w);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[0][i], acc[t], 0, 0, 0);
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[1][i], acc[t], 0, 0, 0);
+          for (int i = 0; i < NP; ++i) {
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[0][i], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[1][i], acc[t], 0, 0, 0);
+          }
         }
       }
+      if (more) load_values(grp + W);
     }
   }
 
   // The waves' streams, through LDS: [W][16] m, l and mv, [W][16][D + 4] acc.
-  extern __shared__ __align__(16) float lds[];
+  __syncthreads();
   float* s_m = lds;
   float* s_l = lds + 16 * W;
   float* s_mv = lds + 32 * W;
@@ -443,44 +499,53 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
 }
 
 // The pieces' streams of a tile, in piece order.  Grid (key heads * row tiles,
-// batch).
+// batch).  Their factors first, in LDS, so that the sums' loads wait for nothing.
+constexpr int kMostPieces = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
+  __shared__ float factor[16][kMostPieces];
   const Kv8View& c = a.c;
   const int D = c.dim, quads = D / 4;
   const int r = blockIdx.y, head = blockIdx.x % c.heads, first = blockIdx.x / c.heads * 16;
   Span s;
   if (!FindSpan(a, p, r, first, &s) || s.pieces == 1) return;
   const int64_t slot0 = (static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces * p.rows;
-  for (int i = threadIdx.x; i < 16 * quads; i += blockDim.x) {
+  const int rows = min(16, s.rows - first);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  for (int k = wave; k < rows; k += 4) {
+    float2 st = make_float2(-INFINITY, -1.0f);
+    if (lane < s.pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows + k];
+    const bool some = !(st.y < 0.0f);
+    float peak = some ? st.x : -INFINITY;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+    const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
+    float sum = some ? st.y * e : 0.0f;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+    // (a request without tokens is one piece, so sum is 0 only for 0 / 0)
+    factor[k][lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * quads; i += 256) {
     const int k = i / quads, d = 4 * (i - k * quads), at = first + k;
-    if (at >= s.rows) break;
-    float m = -INFINITY, sum = 0.0f;
-    bool some = false;
+    const float* part = p.part + (slot0 + k) * D + d;
     F32x4 o = {0, 0, 0, 0};
+#pragma unroll 8
     for (int z = 0; z < s.pieces; ++z) {
-      const int64_t slot = slot0 + static_cast<int64_t>(z) * p.rows + k;
-      const float2 st = p.stats[slot];
-      if (st.y < 0.0f) continue;
-      some = true;
-      const float peak = fmaxf(m, st.x);
-      const float base = peak == -INFINITY ? 0.0f : peak;
-      const float e0 = Exp2(m - base), e1 = Exp2(st.x - base);
-      o = o * e0 + *reinterpret_cast<const F32x4*>(p.part + slot * D + d) * e1;
-      sum = sum * e0 + st.y * e1;
-      m = peak;
+      o += *reinterpret_cast<const F32x4*>(part + static_cast<int64_t>(z) * p.rows * D) *
+           factor[k][z];
     }
     const int tok = at / p.group;
     T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
              static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(some ? o[e] / sum : 0.0f);
+    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(o[e]);
   }
 }
 
 constexpr int kWaves = 4;
-constexpr int kTarget = 1024;  // workgroups worth spreading lists for
-constexpr int kMostPieces = 64;
+constexpr int kTarget = 768;  // workgroups worth spreading lists for
 
 // How a batch's lists are cut, by its sizes alone (the lengths themselves are
 // on the device).
@@ -505,11 +570,27 @@ size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
          (sizeof(float) * c.dim + sizeof(float2));
 }
 
-template <typename T, int FMT, int NU>
+size_t LdsBytes(int dim) {
+  return std::max(sizeof(float) * (48 * kWaves + kWaves * 16 * (dim + 4)),
+                  sizeof(PageInfo) * kStage);
+}
+
+// Calls f with the kernel of a head size.
+template <typename T, int FMT, typename F>
+void WithKernel(int dim, F&& f) {
+  if (dim == 64) return f(Kv8AttendKernel<T, FMT, 1, 64, kWaves>);
+  if (dim < 64) return f(Kv8AttendKernel<T, FMT, 1, 0, kWaves>);
+  if (dim == 128) return f(Kv8AttendKernel<T, FMT, 2, 128, kWaves>);
+  if (dim < 128) return f(Kv8AttendKernel<T, FMT, 2, 0, kWaves>);
+  return f(Kv8AttendKernel<T, FMT, 4, 0, kWaves>);
+}
+
+template <typename T, int FMT>
 void Launch(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid(a.c.heads * p.tiles, a.b.batch, p.pieces);
-  const size_t lds = sizeof(float) * (48 * kWaves + kWaves * 16 * (a.c.dim + 4));
-  Kv8AttendKernel<T, FMT, NU, kWaves><<<grid, kWaves * kWave, lds, stream>>>(a, p);
+  WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
+    kernel<<<grid, kWaves * kWave, LdsBytes(a.c.dim), stream>>>(a, p);
+  });
   DSD_HIP_CHECK(hipGetLastError());
   if (p.pieces > 1) {
     Kv8MergeKernel<T><<<dim3(grid.x, grid.y), 256, 0, stream>>>(a, p);
@@ -517,24 +598,15 @@ void Launch(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
   }
 }
 
-template <typename T, int FMT>
-void LaunchDim(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
-  if (a.c.dim <= 64) return Launch<T, FMT, 1>(a, p, stream);
-  if (a.c.dim <= 128) return Launch<T, FMT, 2>(a, p, stream);
-  return Launch<T, FMT, 4>(a, p, stream);
-}
-
 template <typename T>
 void LaunchType(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
-  a.c.format == DSD_KV8_INT8 ? LaunchDim<T, DSD_KV8_INT8>(a, p, stream)
-                             : LaunchDim<T, DSD_KV8_E4M3>(a, p, stream);
+  a.c.format == DSD_KV8_INT8 ? Launch<T, DSD_KV8_INT8>(a, p, stream)
+                             : Launch<T, DSD_KV8_E4M3>(a, p, stream);
 }
 
 template <typename T, int FMT>
 void PreloadDim(const Kv8View& c) {
-  if (c.dim <= 64) return PreloadKernel(Kv8AttendKernel<T, FMT, 1, kWaves>);
-  if (c.dim <= 128) return PreloadKernel(Kv8AttendKernel<T, FMT, 2, kWaves>);
-  return PreloadKernel(Kv8AttendKernel<T, FMT, 4, kWaves>);
+  WithKernel<T, FMT>(c.dim, [](auto kernel) { PreloadKernel(kernel); });
 }
 
 template <typename T>
