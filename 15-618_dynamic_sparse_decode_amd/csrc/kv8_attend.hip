@@ -160,7 +160,7 @@ constexpr int kWeightTerms = std::is_same<T, __bf16>::value ? 1 : 2;
 // values' layout.  No number crosses lanes but for the maxima.
 // kDim: head_dim where it is 64 * NU (no bounds tests), else 0.
 template <typename T, int FMT, int NU, int kDim, int W>
-__global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Plan p) {
+__global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8AttendArgs a, Plan p) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>, NT = 4 * NU;
   extern __shared__ __align__(16) float lds[];
   const Kv8View& c = a.c;
@@ -180,10 +180,10 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
   const int row = first + n;
   const bool there = row < s.rows;
   const int token = there ? row / p.group : 0;
-  const int q_head = head * p.group + (there ? row - token * p.group : 0);
   F16x8 q[NU][2][NQ];
-  float to_logit;  // what a product with codes lacks but the page's scale; >= 0
-  {
+  float to_logit = 0.0f;  // what a product with codes lacks but the page's scale; >= 0
+  auto load_query = [&] {
+    const int q_head = head * p.group + (there ? row - token * p.group : 0);
     const T* qp = static_cast<const T*>(a.q) + (s.q.row0 + token) * a.q_stride +
                   static_cast<int64_t>(q_head) * D;
     float x[NU][16];
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
         }
       }
     }
-  }
+  };
   const int sees = a.causal ? s.q.past + token + 1 : 0x7fffffff;  // row n's tokens
 
   F32x4 acc[NT];
@@ -292,6 +292,7 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
       load_keys(grp);
       load_values(grp);
     }
+    if (g0 == begin) load_query();  // (its latency beside the first group's)
     for (; grp < g1; grp += W) {
       const bool more = grp + W < g1;
       F32x4 x[4];
@@ -498,23 +499,29 @@ __global__ __launch_bounds__(W* kWave) void Kv8AttendKernel(Kv8AttendArgs a, Pla
   }
 }
 
-// The pieces' streams of a tile, in piece order.  Grid (key heads * row tiles,
-// batch).  Their factors first, in LDS, so that the sums' loads wait for nothing.
+// One row's pieces.  Grid (key heads * row tiles, batch, rows of a tile): the
+// pieces' factors first, in LDS, so that the sums' loads wait for nothing; the
+// threads beyond a row's quads take every 256 / quads-th piece, and their sums
+// are added in that order.
 constexpr int kMostPieces = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
-  __shared__ float factor[16][kMostPieces];
+  __shared__ float factor[kMostPieces];
+  __shared__ F32x4 part_sum[256];
   const Kv8View& c = a.c;
   const int D = c.dim, quads = D / 4;
   const int r = blockIdx.y, head = blockIdx.x % c.heads, first = blockIdx.x / c.heads * 16;
+  const int k = blockIdx.z, at = first + k;
   Span s;
-  if (!FindSpan(a, p, r, first, &s) || s.pieces == 1) return;
-  const int64_t slot0 = (static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces * p.rows;
-  const int rows = min(16, s.rows - first);
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  for (int k = wave; k < rows; k += 4) {
+  if (!FindSpan(a, p, r, first, &s) || s.pieces == 1 || at >= s.rows) return;
+  const int64_t slot0 =
+      (static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces * p.rows + k;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int shares = 256 / quads;  // threads per quad
+  const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
+  if (threadIdx.x < kWave) {
     float2 st = make_float2(-INFINITY, -1.0f);
-    if (lane < s.pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows + k];
+    if (lane < s.pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows];
     const bool some = !(st.y < 0.0f);
     float peak = some ? st.x : -INFINITY;
 #pragma unroll
@@ -523,25 +530,43 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
     float sum = some ? st.y * e : 0.0f;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-    // (a request without tokens is one piece, so sum is 0 only for 0 / 0)
-    factor[k][lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+    factor[lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+  }
+  // (loads that do not need the factors are on their way meanwhile)
+  constexpr int kAhead = 4;
+  const float* part = p.part + slot0 * D + d;
+  const int64_t step = static_cast<int64_t>(p.rows) * D;
+  F32x4 x[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int z = share + i * shares;
+    x[i] = F32x4{0, 0, 0, 0};
+    if (share < shares && z < s.pieces) {
+      x[i] = *reinterpret_cast<const F32x4*>(part + z * step);
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * quads; i += 256) {
-    const int k = i / quads, d = 4 * (i - k * quads), at = first + k;
-    const float* part = p.part + (slot0 + k) * D + d;
-    F32x4 o = {0, 0, 0, 0};
-#pragma unroll 8
-    for (int z = 0; z < s.pieces; ++z) {
-      o += *reinterpret_cast<const F32x4*>(part + static_cast<int64_t>(z) * p.rows * D) *
-           factor[k][z];
-    }
-    const int tok = at / p.group;
-    T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
-             static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
+  F32x4 o = {0, 0, 0, 0};
+  if (share < shares) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(o[e]);
+    for (int i = 0; i < kAhead; ++i) {
+      const int z = share + i * shares;
+      if (z < s.pieces) o += x[i] * factor[z];
+    }
+#pragma unroll 4
+    for (int z = share + kAhead * shares; z < s.pieces; z += shares) {
+      o += *reinterpret_cast<const F32x4*>(part + z * step) * factor[z];
+    }
   }
+  part_sum[threadIdx.x] = o;
+  __syncthreads();
+  if (share > 0) return;
+  for (int i = 1; i < shares; ++i) o += part_sum[i * quads + threadIdx.x];
+  const int tok = at / p.group;
+  T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
+           static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(o[e]);
 }
 
 constexpr int kWaves = 4;
@@ -593,7 +618,7 @@ void Launch(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
   });
   DSD_HIP_CHECK(hipGetLastError());
   if (p.pieces > 1) {
-    Kv8MergeKernel<T><<<dim3(grid.x, grid.y), 256, 0, stream>>>(a, p);
+    Kv8MergeKernel<T><<<dim3(grid.x, grid.y, p.rows), 256, 0, stream>>>(a, p);
     DSD_HIP_CHECK(hipGetLastError());
   }
 }
