@@ -3283,6 +3283,7 @@ int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_p
     }
     dsdk::PreloadKv8Append(v);
     dsdk::PreloadKv8Attend(v);
+    dsdk::PreloadKv8Prompt(v);
     *out_cache = cache.release();
   });
 }

@@ -1,5 +1,5 @@
 // kv8.h -- the 8-bit paged cache (dsd_kv8_*): launch interface of
-// kv8_append.hip and kv8_attend.hip.
+// kv8_append.hip, kv8_attend.hip and kv8_prompt.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -64,9 +64,12 @@ struct Kv8AttendArgs {
   FailReport fail;
 };
 void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream);
+// The form of it for many rows (kv8_prompt.hip).
+void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 // The kernels that calls on such a cache run.
 void PreloadKv8Append(const Kv8View& c);
 void PreloadKv8Attend(const Kv8View& c);
+void PreloadKv8Prompt(const Kv8View& c);
 
 }  // namespace dsdk

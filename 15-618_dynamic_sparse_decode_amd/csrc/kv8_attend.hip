@@ -12,63 +12,13 @@
 // log2 v, so at most 2^15 whatever the scales: half precision rounds them to
 // 2^-11, or 2^-22 as two terms where the output is finer than bf16.  All sums
 // are float32.
-#include "kv8_device.h"
+#include "kv8_attend.h"
 
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 namespace dsdk {
 namespace {
-
-constexpr float kWeightBits = 15.0f;  // weights reach 2^15 (half precision ends at 2^16)
-
-// The larger (sum) of the four lanes that share lane % 16.
-__device__ __forceinline__ float Max4(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float Sum4(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
-// Eight codes (two words) as half-precision numbers.
-template <int FMT>
-__device__ __forceinline__ F16x8 Numbers8(unsigned w0, unsigned w1) {
-  F16x2 x[4];
-  if constexpr (FMT == DSD_KV8_INT8) {
-    // 1024 + (code + 128) in the last bits of a half's fraction, less 1152
-    const F16x2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-    w0 ^= 0x80808080u;
-    w1 ^= 0x80808080u;
-    x[0] = __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) - bias;
-    x[1] = __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) - bias;
-    x[2] = __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) - bias;
-    x[3] = __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) - bias;
-  } else {
-    x[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
-    x[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
-    x[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
-    x[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
-  }
-  F16x8 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[2 * i] = x[i][0];
-    r[2 * i + 1] = x[i][1];
-  }
-  return r;
-}
-
-// The high bit of each byte that is an e4m3 NaN.
-__device__ __forceinline__ unsigned NanBytes(unsigned w) {
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-}
 
 // A launch as its kernels see it.
 struct Plan {
@@ -81,74 +31,11 @@ struct Plan {
   float2* stats = nullptr;  // [batch][heads * tiles][pieces][rows]: (m, l), l < 0: no token
 };
 
-// What a workgroup attends: rows [first, first + 16) of request r (row i:
-// token i / group, query head i % group of the key head), chunks of 16 tokens.
-struct Span {
-  Kv8Request q;
-  int rows = 0;    // of the request
-  int chunks = 0;  // that the tile's rows look at
-  int pieces = 1;  // that these are cut into
-};
-
-__device__ __forceinline__ bool FindSpan(const Kv8AttendArgs& a, const Plan& p, int r, int first,
-                                         Span* s) {
-  bool ok;
-  if (a.causal) {
-    ok = Kv8ReadTokens(a.b, r, a.c.page, &s->q);
-  } else {
-    ok = Kv8ReadList(a.b, r, &s->q);
-    s->q.row0 = r;
-    s->q.n = 1;
-  }
-  if (!ok || s->q.pages > 0x7fffff00 / a.c.page) {
-    if (threadIdx.x == 0) ReportFailure(a.fail, kFailShape);
-    // (a decode request still gets its zeros)
-    if (a.causal) return false;
-    s->q.pages = 0;
-  }
-  s->rows = s->q.n * p.group;
-  if (first >= s->rows) return false;
-  if (a.causal) {
-    const int last = (min(first + 16, s->rows) - 1) / p.group;
-    s->chunks = (s->q.past + last) / 16 + 1;
-  } else {
-    s->chunks = s->q.pages * a.c.chunks;
-  }
-  const int groups = (s->chunks + 3) / 4;
-  s->pieces = min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
-  return true;
+// The pieces that a span's list is cut into.
+__device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {
+  const int groups = (s.chunks + 3) / 4;
+  return min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
 }
-
-// One page of a request's list, staged in LDS.
-struct PageInfo {
-  int page;     // (0 for one that holds no token)
-  int tokens;   // in the cache
-  float key_scale;
-  float value_scale;
-};
-constexpr int kStage = 512;  // pages staged at a time
-
-__device__ __forceinline__ PageInfo ReadPage(const Kv8AttendArgs& a, const Span& s, int head,
-                                             int slot) {
-  const Kv8View& c = a.c;
-  PageInfo k;
-  k.page = a.b.page_ids[s.q.list + slot];
-  const bool ok = InPool(k.page, c.capacity);
-  if (!ok) ReportFailure(a.fail, kFailPageId);
-  k.page = ok ? k.page : 0;
-  k.tokens = 0;
-  if (ok) k.tokens = a.causal ? s.q.past + s.q.n - slot * c.page : c.token_counts[k.page];
-  k.tokens = min(max(k.tokens, 0), c.page);
-  const int at = k.page * c.heads + head;
-  k.key_scale = k.tokens > 0 ? c.key_scales[at] : 1.0f;
-  k.value_scale = k.tokens > 0 ? fmaxf(c.value_scales[at], kKv8Tiny) : 1.0f;
-  return k;
-}
-
-template <typename T>
-constexpr int kQueryTerms = sizeof(T) == 4 ? 2 : 1;
-template <typename T>
-constexpr int kWeightTerms = std::is_same<T, __bf16>::value ? 1 : 2;
 
 // Grid (key heads * row tiles, batch, pieces); W waves, each of which takes
 // every W-th group of 64 tokens of the piece for all of the tile's 16 rows.
@@ -170,11 +57,12 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
   const int r = blockIdx.y, head = blockIdx.x % c.heads;
   const int first = blockIdx.x / c.heads * 16;
   Span s;
-  if (!FindSpan(a, p, r, first, &s)) return;
-  if (static_cast<int>(blockIdx.z) >= s.pieces) return;
+  if (!FindSpan(a, p.group, r, first, 16, &s)) return;
+  const int pieces = Pieces(p, s);
+  if (static_cast<int>(blockIdx.z) >= pieces) return;
   const int groups = (s.chunks + 3) / 4;
   const int begin = blockIdx.z * p.piece;
-  const int end = static_cast<int>(blockIdx.z) == s.pieces - 1 ? groups : begin + p.piece;
+  const int end = static_cast<int>(blockIdx.z) == pieces - 1 ? groups : begin + p.piece;
 
   // Row n's query: units g + 4 u of 16 dims, eight at a time.
   const int row = first + n;
@@ -204,25 +92,12 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
         most = fmaxf(most, size < INFINITY ? size : 0.0f);
       }
     }
-    most = Max4(most);
-    int e = 0;
-    (void)frexpf(most, &e);
-    e = most > 0.0f ? max(min(14 - e, 126), -126) : 0;
-    const float up = copysignf(__uint_as_float(static_cast<unsigned>(e + 127) << 23), a.scale);
-    to_logit =
-        fabsf(a.scale) * kLog2e * __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+    const QueryScale scale = ScaleQuery(Max4(most), a.scale);
+    to_logit = scale.back;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float y = x[u][i] * up;
-        const _Float16 hi = static_cast<_Float16>(y);
-        q[u][i >> 3][0][i & 7] = hi;
-        if constexpr (NQ == 2) {
-          const float rest = y - static_cast<float>(hi);
-          q[u][i >> 3][1][i & 7] = static_cast<_Float16>(fabsf(y) < INFINITY ? rest : 0.0f);
-        }
-      }
+      for (int i = 0; i < 16; ++i) SplitQuery(x[u][i] * scale.up, q[u][i >> 3], i & 7);
     }
   };
   const int sees = a.causal ? s.q.past + token + 1 : 0x7fffffff;  // row n's tokens
@@ -348,26 +223,12 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
       F16x8 w[2][NP];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = Exp2(fmaf(x[t][i], f, -base));
-          l += e;
-          y[i] = e * to_half;
-        }
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const F32x2 pair = {y[i], y[i + 1]};
-          const F16x2 hi = __builtin_convertvector(pair, F16x2);
-          w[t >> 1][0][4 * (t & 1) + i] = hi[0];
-          w[t >> 1][0][4 * (t & 1) + i + 1] = hi[1];
-          if constexpr (NP == 2) {
-            const F32x2 rest = {y[i] - static_cast<float>(hi[0]),
-                                y[i + 1] - static_cast<float>(hi[1])};
-            const F16x2 lo = __builtin_convertvector(rest, F16x2);
-            w[t >> 1][1][4 * (t & 1) + i] = lo[0];
-            w[t >> 1][1][4 * (t & 1) + i + 1] = lo[1];
-          }
+          const float e0 = Exp2(fmaf(x[t][i], f, -base));
+          const float e1 = Exp2(fmaf(x[t][i + 1], f, -base));
+          l += e0 + e1;
+          SplitWeights(e0 * to_half, e1 * to_half, w[t >> 1], 4 * (t & 1) + i);
         }
       }
       if (!whole) {
@@ -484,7 +345,7 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
              Exp2(s_mv[w * 16 + k] - base - kWeightBits);
       }
     }
-    if (s.pieces == 1) {
+    if (pieces == 1) {
       const int tok = at / p.group;
       T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
                static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
@@ -513,7 +374,9 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   const int r = blockIdx.y, head = blockIdx.x % c.heads, first = blockIdx.x / c.heads * 16;
   const int k = blockIdx.z, at = first + k;
   Span s;
-  if (!FindSpan(a, p, r, first, &s) || s.pieces == 1 || at >= s.rows) return;
+  if (!FindSpan(a, p.group, r, first, 16, &s)) return;
+  const int pieces = Pieces(p, s);
+  if (pieces == 1 || at >= s.rows) return;
   const int64_t slot0 =
       (static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces * p.rows + k;
   const int lane = threadIdx.x & (kWave - 1);
@@ -521,7 +384,7 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
   if (threadIdx.x < kWave) {
     float2 st = make_float2(-INFINITY, -1.0f);
-    if (lane < s.pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows];
+    if (lane < pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows];
     const bool some = !(st.y < 0.0f);
     float peak = some ? st.x : -INFINITY;
 #pragma unroll
@@ -541,7 +404,7 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   for (int i = 0; i < kAhead; ++i) {
     const int z = share + i * shares;
     x[i] = F32x4{0, 0, 0, 0};
-    if (share < shares && z < s.pieces) {
+    if (share < shares && z < pieces) {
       x[i] = *reinterpret_cast<const F32x4*>(part + z * step);
     }
   }
@@ -551,10 +414,10 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int z = share + i * shares;
-      if (z < s.pieces) o += x[i] * factor[z];
+      if (z < pieces) o += x[i] * factor[z];
     }
 #pragma unroll 4
-    for (int z = share + kAhead * shares; z < s.pieces; z += shares) {
+    for (int z = share + kAhead * shares; z < pieces; z += shares) {
       o += *reinterpret_cast<const F32x4*>(part + z * step) * factor[z];
     }
   }
@@ -570,10 +433,12 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
 }
 
 constexpr int kWaves = 4;
-constexpr int kTarget = 768;  // workgroups worth spreading lists for
 
 // How a batch's lists are cut, by its sizes alone (the lengths themselves are
-// on the device).
+// on the device): two workgroups fit a CU (registers), 512 the chip, and lists
+// are cut until there are as many, each piece at least a group of 64 tokens a
+// wave.
+constexpr int kTarget = 512;
 Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal) {
   Plan p;
   p.group = q_heads / c.heads;
@@ -582,11 +447,16 @@ Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal
   p.rows = static_cast<int>(std::min<int64_t>(rows, 16));
   const int64_t groups = (static_cast<int64_t>(b.max_pages) * c.page + 63) / 64;
   const int64_t units = static_cast<int64_t>(c.heads) * p.tiles * b.batch;
-  int64_t want = (kTarget + units - 1) / std::max<int64_t>(units, 1);
-  want = std::min<int64_t>({want, (groups + kWaves - 1) / kWaves, kMostPieces});
+  const int64_t want = std::min<int64_t>(
+      {kTarget / std::max<int64_t>(units, 1), (groups + kWaves - 1) / kWaves, kMostPieces});
   p.pieces = static_cast<int>(std::max<int64_t>(want, 1));
   p.piece = static_cast<int>(std::max<int64_t>((groups + p.pieces - 1) / p.pieces, 1));
   return p;
+}
+
+// Whether a prompt call has rows enough for kv8_prompt.hip.
+bool ManyRows(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  return static_cast<int64_t>(b.max_tokens) * (q_heads / c.heads) > 64;
 }
 
 size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
@@ -644,8 +514,9 @@ void PreloadType(const Kv8View& c) {
 
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
   if (b.batch == 0) return 0;
-  return std::max(PlanBytes(c, b, MakePlan(c, b, q_heads, false)),
-                  PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
+  const size_t one = PlanBytes(c, b, MakePlan(c, b, q_heads, false));
+  if (ManyRows(c, b, q_heads)) return one;
+  return std::max(one, PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
 }
 
 void PreloadKv8Attend(const Kv8View& c) {
@@ -656,6 +527,7 @@ void PreloadKv8Attend(const Kv8View& c) {
 
 void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream) {
   if (a.b.batch == 0 || (a.causal && a.b.tokens == 0)) return;
+  if (a.causal && ManyRows(a.c, a.b, a.q_heads)) return LaunchKv8Prompt(a, stream);
   Plan p = MakePlan(a.c, a.b, a.q_heads, a.causal);
   if (p.pieces > 1) {
     if (a.workspace == nullptr || a.workspace_bytes < PlanBytes(a.c, a.b, p)) {
