@@ -3118,7 +3118,7 @@ struct dsd_kv8 {
   bool owned = false;  // the arrays are the handle's
   int device = 0;
   dsdk::Kv8Rotation rotation;
-  DeviceBuffer<double> turns;
+  DeviceBuffer<double2> table;
 
   ~dsd_kv8() {
     if (!owned) return;
@@ -3333,18 +3333,33 @@ int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved, const 
     Require(interleaved == 0 || interleaved == 1, "interleaved must be 0 or 1");
     Require(std::isfinite(magnitude), "magnitude must be finite");
     const int pairs = rotary_dim / 2;
-    std::vector<double> turns(static_cast<size_t>(pairs));
-    for (int i = 0; i < pairs; ++i) {
-      Require(std::isfinite(inv_freq[i]), "inv_freq must be finite");
-      turns[i] = static_cast<double>(inv_freq[i] / 3.14159265358979323846264338327950288L);
+    // Entry j of a level is the j-th power of its first, in extended precision:
+    // off by 256 * 2^-64 at most.
+    constexpr long double kTurn = 6.28318530717958647692528676655900576839L;
+    std::vector<double2> table(static_cast<size_t>(pairs) * 4 * 256);
+    for (int p = 0; p < pairs; ++p) {
+      Require(std::isfinite(inv_freq[p]), "inv_freq must be finite");
+      for (int level = 0; level < 4; ++level) {
+        long double turns = std::ldexp(static_cast<long double>(inv_freq[p]) / kTurn, 8 * level);
+        turns -= std::floor(turns);
+        const long double c = std::cos(turns * kTurn), s = std::sin(turns * kTurn);
+        long double x = 1.0L, y = 0.0L;
+        for (int j = 0; j < 256; ++j) {
+          table[(static_cast<size_t>(level) * 256 + j) * pairs + p] = {static_cast<double>(x),
+                                                                       static_cast<double>(y)};
+          const long double next = x * c - y * s;
+          y = x * s + y * c;
+          x = next;
+        }
+      }
     }
     DSD_HIP_CHECK(hipDeviceSynchronize());
     if (pairs > 0) {
-      cache->turns.Reserve(static_cast<size_t>(pairs));
-      DSD_HIP_CHECK(hipMemcpy(cache->turns.ptr, turns.data(), sizeof(double) * turns.size(),
+      cache->table.Reserve(table.size());
+      DSD_HIP_CHECK(hipMemcpy(cache->table.ptr, table.data(), sizeof(double2) * table.size(),
                               hipMemcpyHostToDevice));
     }
-    cache->rotation.turns = cache->turns.ptr;
+    cache->rotation.table = cache->table.ptr;
     cache->rotation.pairs = pairs;
     cache->rotation.interleaved = interleaved;
     cache->rotation.magnitude = magnitude;

@@ -28,7 +28,8 @@ struct Kv8View {
 };
 
 struct Kv8Rotation {
-  const double* turns = nullptr;  // [pairs]: inv_freq / pi
+  // [4][256][pairs]: (cos, sin) of pair p turned by j * 256^level positions
+  const double2* table = nullptr;
   int pairs = 0;
   int interleaved = 0;
   double magnitude = 1.0;

@@ -3,11 +3,12 @@
 // queries rotated.
 //
 // Mathematics.  Pair (x, y) of a head turns by a = position * inv_freq:
-// (x cos a - y sin a, y cos a + x sin a).  Angles are taken in half turns
-// (position * (inv_freq / pi), exact in 64 bits far beyond a million
-// positions, where 32 bits are off by whole hundredths of a radian) and the
-// products in 64 bits too: a key's code then falls on the right side of every
-// rounding border.  The codes of a page share one scale s >= largest / M (M =
+// (x cos a - y sin a, y cos a + x sin a).  A position is its four bytes, so
+// (cos a, sin a) is the product of four complex numbers out of a table of 4 x
+// 256 a pair, in 64 bits (32-bit angles are off by whole hundredths of a radian
+// at a million positions); the turns are 64-bit too: a key's code then falls on
+// the right side of every rounding border.  (Forming sines in place cost 25
+// registers, a quarter of the waves, and three times the instructions.)  The codes of a page share one scale s >= largest / M (M =
 // 448 or 127), so a token that needs a larger one takes the page's earlier
 // codes with it: code <- nearest(code * old / s).
 //
@@ -178,30 +179,30 @@ __device__ __forceinline__ int SineAt(int o, int i, int u, int turning) {
   return (o * 8 + i) * turning + u;
 }
 
-// x[0..8) at a, x[8..16) at b, turned into y; cs: the unit's first pair, the
-// others `step` apart.
-__device__ __forceinline__ void Turn(const float* x, const double2* cs, int step, const Unit& u,
-                                     int interleaved, double* y) {
-  if (!u.turns) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = static_cast<double>(x[i]);
-  } else if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double c = cs[i * step].x, s = cs[i * step].y;
-      const double p = static_cast<double>(x[2 * i]), q = static_cast<double>(x[2 * i + 1]);
-      y[2 * i] = p * c - q * s;
-      y[2 * i + 1] = q * c + p * s;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double c = cs[i * step].x, s = cs[i * step].y;
-      const double p = static_cast<double>(x[i]), q = static_cast<double>(x[8 + i]);
-      y[i] = p * c - q * s;
-      y[8 + i] = q * c + p * s;
-    }
+// Pair i of a unit whose elements are x[at..at + 8) at a, x[at + 8..at + 16) at
+// b: its place from `at` on and its numbers turned.  cs: the unit's first pair, the others `step` apart.
+// (The schedule is held to a pair at a time: left to interleave them the
+// compiler takes twice the registers, half the waves a CU.)
+struct Turned {
+  int i0, i1;
+  double y0, y1;
+};
+template <typename X>
+__device__ __forceinline__ Turned TurnPair(const X& x, int at, int i, const double2* cs, int step,
+                                           const Unit& u, bool interleaved) {
+  Turned t;
+  t.i0 = interleaved ? 2 * i : i;
+  t.i1 = interleaved ? 2 * i + 1 : 8 + i;
+  const double p = static_cast<double>(x[at + t.i0]);
+  const double q = static_cast<double>(x[at + t.i1]);
+  t.y0 = p;
+  t.y1 = q;
+  if (u.turns) {
+    const double2 w = cs[i * step];
+    t.y0 = p * w.x - q * w.y;
+    t.y1 = q * w.x + p * w.y;
   }
+  return t;
 }
 
 // One page's part of a call.
@@ -260,28 +261,55 @@ __device__ __forceinline__ bool FindTask(const Kv8AppendArgs& a, int u, Task* t)
 }
 
 // The sines and cosines of a chunk's tokens, offsets [lo, hi) of the 16 from
-// c0 on, [16][pairs].
+// c0 on (SineAt).
+__device__ __forceinline__ double2 Times(double2 a, double2 b) {
+  return {a.x * b.x - a.y * b.y, a.x * b.y + a.y * b.x};
+}
 __device__ __forceinline__ void FillSines(const Kv8AppendArgs& a, const Task& t, int c0, int lo,
                                           int hi, double2* cs) {
   const int pairs = a.rot.pairs;
   const int n = (hi - lo) * pairs;
+  const double2* table = a.rot.table;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int k = i / pairs, p = i - k * pairs;
     const int o = c0 + lo + k;
     const int at = a.b.positions != nullptr ? a.b.positions[t.row + o] : t.index + o;
-    double s, c;
-    sincospi(static_cast<double>(at) * a.rot.turns[p], &s, &c);
-    cs[SineAt(lo + k, p & 7, p >> 3, pairs / 8)] = {c * a.rot.magnitude, s * a.rot.magnitude};
+    const unsigned far = at < 0 ? 0u - static_cast<unsigned>(at) : static_cast<unsigned>(at);
+    const double2 w = Times(Times(table[(far & 255u) * pairs + p],
+                                  table[(256u + ((far >> 8) & 255u)) * pairs + p]),
+                            Times(table[(512u + ((far >> 16) & 255u)) * pairs + p],
+                                  table[(768u + (far >> 24)) * pairs + p]));
+    const double s = at < 0 ? -w.y : w.y;
+    cs[SineAt(lo + k, p & 7, p >> 3, pairs / 8)] = {w.x * a.rot.magnitude,
+                                                  s * a.rot.magnitude};
   }
 }
 
-// ---- keys ----------------------------------------------------------------------
-// Lane l has unit (l + 64 j) % units of token (l + 64 j) / units, j < NU =
-// ceil(dim / 64).
+// A chunk's new offsets within it.
+struct Part {
+  int c0 = 0, lo = 0, hi = 0;
+};
+__device__ __forceinline__ Part PartOf(const Task& t, int c) {
+  Part p;
+  p.c0 = 16 * c;
+  p.lo = min(max(t.first - p.c0, 0), 16);
+  p.hi = min(t.end - p.c0, 16);
+  return p;
+}
+
+// A side's new numbers of one chunk in a lane's registers.  Keys: lane l has unit
+// (l + 64 j) % units of token (l + 64 j) / units, j < NU = ceil(dim / 64), at
+// x[16 j ..].  Values: dims 2 l, 2 l + 1 of the m-th 128, all 16 tokens, at
+// x[32 m + 2 token ..].
+template <typename T, int NU>
+struct Numbers {
+  static constexpr int kPlanes = (NU + 1) / 2;
+  Packed<T, 32 * kPlanes> x;
+};
 
 template <typename T, int NU>
 __device__ __forceinline__ void LoadKeys(const Kv8AppendArgs& a, bool vec, const Task& t, int h,
-                                         int c0, int lo, int hi, float (&x)[NU][16]) {
+                                         const Part& p, Numbers<T, NU>* x) {
   const int lane = threadIdx.x & (kWave - 1);
   const int units = a.c.dim / 16;
   const T* k = static_cast<const T*>(a.k) + static_cast<int64_t>(h) * a.c.dim;
@@ -289,18 +317,18 @@ __device__ __forceinline__ void LoadKeys(const Kv8AppendArgs& a, bool vec, const
   for (int j = 0; j < NU; ++j) {
     const int i = lane + kWave * j;
     const int o = i / units, u = i - o * units;
-    if (o >= lo && o < hi) {
+    if (o >= p.lo && o < p.hi) {
       const Unit w = UnitOf(u, a.rot);
-      const T* p = k + (t.row + c0 + o) * a.k_stride;
-      Load8(p + w.a, vec, x[j]);
-      Load8(p + w.b, vec, x[j] + 8);
+      const T* from = k + (t.row + p.c0 + o) * a.k_stride;
+      x->x.Load8(16 * j, from + w.a, vec);
+      x->x.Load8(16 * j + 8, from + w.b, vec);
     }
   }
 }
 
-template <int NU>
-__device__ __forceinline__ float LargestKey(const Kv8AppendArgs& a, int lo, int hi,
-                                            const double2* cs, const float (&x)[NU][16]) {
+template <typename T, int NU, bool kInterleaved>
+__device__ __forceinline__ float LargestKey(const Kv8AppendArgs& a, const Part& p,
+                                            const double2* cs, const Numbers<T, NU>& x) {
   const int lane = threadIdx.x & (kWave - 1);
   const int units = a.c.dim / 16, turning = a.rot.pairs / 8;
   float most = 0.0f;
@@ -308,29 +336,33 @@ __device__ __forceinline__ float LargestKey(const Kv8AppendArgs& a, int lo, int 
   for (int j = 0; j < NU; ++j) {
     const int i = lane + kWave * j;
     const int o = i / units, u = i - o * units;
-    if (o >= lo && o < hi) {
-      double y[16];
-      Turn(x[j], cs + SineAt(o, 0, u, turning), turning, UnitOf(u, a.rot), a.rot.interleaved, y);
+    if (o >= p.lo && o < p.hi) {
+      const Unit w = UnitOf(u, a.rot);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = fmaxf(most, FiniteSize(static_cast<float>(y[e])));
+      for (int e = 0; e < 8; ++e) {
+        const Turned y = TurnPair(x.x, 16 * j, e, cs + SineAt(o, 0, u, turning), turning, w,
+                                  kInterleaved);
+        most = fmaxf(most, fmaxf(FiniteSize(static_cast<float>(y.y0)),
+                                 FiniteSize(static_cast<float>(y.y1))));
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   return most;
 }
 
 // One chunk's codes: offsets [lo, hi) new (x, turned again), those before them
-// as they are or brought from `had` to s.  tile:
-// 16 x dim bytes of LDS.  sums: the lane's dims 2 lane, 2 lane + 1 of each 128,
-// summed over offsets [0, hi).
-template <int FMT, int NU>
-__device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block, int lo, int hi,
+// as they are or brought from `had` to s.  tile: 16 x dim bytes of LDS.  sums:
+// the lane's dims 2 lane, 2 lane + 1 of each 128, summed over offsets [0, hi).
+template <int FMT, typename T, int NU, bool kInterleaved>
+__device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block, const Part& p,
                                           float had, bool grew, const Scale& s,
-                                          const float (&x)[NU][16], const double2* cs,
+                                          const Numbers<T, NU>& x, const double2* cs,
                                           uint8_t* tile, float (&sums)[(NU + 1) / 2][2]) {
   const int lane = threadIdx.x & (kWave - 1);
   const int D = a.c.dim;
-  const int units = D / 16;
-  const int turning = a.rot.pairs / 8;
+  const int units = D / 16, turning = a.rot.pairs / 8;
+  const int lo = p.lo, hi = p.hi;
   const int from = grew ? 0 : lo;  // offsets written
   if (lo > 0 && (grew || a.c.summaries != nullptr)) {
     for (int i = lane; i < lo * units; i += kWave) {
@@ -350,15 +382,29 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
     const int o = i / units, u = i - o * units;
     if (o >= lo && o < hi) {
       const Unit w = UnitOf(u, a.rot);
-      double y[16];
-      Turn(x[j], cs + SineAt(o, 0, u, turning), turning, w, a.rot.interleaved, y);
-      uint2 p, q;
-      p.x = Codes4<FMT>(y[0], y[1], y[2], y[3], s);
-      p.y = Codes4<FMT>(y[4], y[5], y[6], y[7], s);
-      q.x = Codes4<FMT>(y[8], y[9], y[10], y[11], s);
-      q.y = Codes4<FMT>(y[12], y[13], y[14], y[15], s);
-      *reinterpret_cast<uint2*>(tile + o * D + w.a) = p;
-      *reinterpret_cast<uint2*>(tile + o * D + w.b) = q;
+      // four pairs at a time: two words of codes
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        double y[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const Turned z = TurnPair(x.x, 16 * j, e + k, cs + SineAt(o, 0, u, turning), turning, w,
+                                    kInterleaved);
+          y[kInterleaved ? 2 * k : k] = z.y0;
+          y[kInterleaved ? 2 * k + 1 : 4 + k] = z.y1;
+        }
+        const unsigned c0 = Codes4<FMT>(y[0], y[1], y[2], y[3], s);
+        const unsigned c1 = Codes4<FMT>(y[4], y[5], y[6], y[7], s);
+        // interleaved: elements 2 e .. 2 e + 8; else e .. e + 4 of both parts
+        uint8_t* to = tile + o * D;
+        if constexpr (kInterleaved) {
+          *reinterpret_cast<uint2*>(to + (e == 0 ? w.a : w.b)) = make_uint2(c0, c1);
+        } else {
+          *reinterpret_cast<unsigned*>(to + w.a + e) = c0;
+          *reinterpret_cast<unsigned*>(to + w.b + e) = c1;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   WaveLdsFence();
@@ -371,10 +417,10 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
       const int d = 128 * m + 2 * lane;
       if (d < D) {
         for (int o = 0; o < hi; ++o) {
-          float x[4];
-          Numbers4<FMT>(*reinterpret_cast<const uint16_t*>(tile + o * D + d), x);
-          sums[m][0] += x[0];
-          sums[m][1] += x[1];
+          float v[4];
+          Numbers4<FMT>(*reinterpret_cast<const uint16_t*>(tile + o * D + d), v);
+          sums[m][0] += v[0];
+          sums[m][1] += v[1];
         }
       }
     }
@@ -382,37 +428,40 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
   WaveLdsFence();
 }
 
-// ---- values --------------------------------------------------------------------
-// Lane l has dims 2 l, 2 l + 1 of each 128 and the 16 tokens of a chunk.
-
-template <typename T>
+template <typename T, int NU>
 __device__ __forceinline__ void LoadValues(const Kv8AppendArgs& a, bool vec, const Task& t, int h,
-                                           int c0, int lo, int hi, int d, float (&x)[2][16]) {
-  const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(h) * a.c.dim + d;
-  typedef T T2 __attribute__((ext_vector_type(2)));
+                                           const Part& p, Numbers<T, NU>* x) {
+  const int lane = threadIdx.x & (kWave - 1);
+  constexpr int kWords = sizeof(T) / 2;  // of two elements
 #pragma unroll
-  for (int o = 0; o < 16; ++o) {
-    x[0][o] = 0.0f;
-    x[1][o] = 0.0f;
-    if (o >= lo && o < hi && d < a.c.dim) {
-      const T* p = v + (t.row + c0 + o) * a.v_stride;
-      if (vec) {
-        const T2 w = *reinterpret_cast<const T2*>(p);
-        x[0][o] = static_cast<float>(w[0]);
-        x[1][o] = static_cast<float>(w[1]);
-      } else {
-        x[0][o] = static_cast<float>(p[0]);
-        x[1][o] = static_cast<float>(p[1]);
+  for (int m = 0; m < Numbers<T, NU>::kPlanes; ++m) {
+    const int d = 128 * m + 2 * lane;
+    const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(h) * a.c.dim + d;
+#pragma unroll
+    for (int o = 0; o < 16; ++o) {
+      unsigned* to = x->x.w + (16 * m + o) * kWords;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) to[k] = 0u;
+      if (o >= p.lo && o < p.hi && d < a.c.dim) {
+        const T* from = v + (t.row + p.c0 + o) * a.v_stride;
+        if (vec || sizeof(T) == 4) {
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) to[k] = reinterpret_cast<const unsigned*>(from)[k];
+        } else {
+          const uint16_t* half = reinterpret_cast<const uint16_t*>(from);
+          to[0] = half[0] | static_cast<unsigned>(half[1]) << 16;
+        }
       }
     }
   }
 }
 
-__device__ __forceinline__ float LargestValue(const float (&x)[2][16]) {
+template <typename T, int NU>
+__device__ __forceinline__ float LargestValue(const Numbers<T, NU>& x) {
   float most = 0.0f;
 #pragma unroll
-  for (int o = 0; o < 16; ++o) {
-    most = fmaxf(most, fmaxf(FiniteSize(x[0][o]), FiniteSize(x[1][o])));
+  for (int i = 0; i < 32 * Numbers<T, NU>::kPlanes; ++i) {
+    most = fmaxf(most, FiniteSize(x.x[i]));
   }
   return most;
 }
@@ -425,14 +474,18 @@ __device__ __forceinline__ unsigned TokenMask(int i, int lo, int hi) {
   return below_h & ~below_l;
 }
 
-// column: the 16 codes of one dim.  Tokens outside [0, hi) stay as they are.
-template <int FMT>
+// column: the 16 codes of one dim, token t's number x[at + 2 t].  Tokens outside
+// [0, hi) stay as they are.
+template <int FMT, typename X>
 __device__ __forceinline__ void StoreValues(uint8_t* column, int lo, int hi, float had, bool grew,
-                                            const Scale& s, const float (&x)[16]) {
+                                            const Scale& s, const X& x, int at) {
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = lo < hi ? Codes4<FMT>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], s) : 0u;
+    w[i] = 0u;
+    if (lo < hi) {
+      w[i] = Codes4<FMT>(x[at + 8 * i], x[at + 8 * i + 2], x[at + 8 * i + 4], x[at + 8 * i + 6], s);
+    }
   }
   if (lo > 0 || hi < 16) {
     const uint4 old = *reinterpret_cast<const uint4*>(column);
@@ -455,170 +508,50 @@ __device__ __forceinline__ void StoreValues(uint8_t* column, int lo, int hi, flo
 // group's queries.  LDS: the sines of 16 tokens, then a 16 x dim tile per head.
 constexpr int kMostPer = 4;
 
-// Rotates the queries of offsets [c0 + lo, c0 + hi), heads [h0, h1).
-template <typename T>
+// Rotates the queries of a chunk's new tokens, heads [h0, h1).
+template <typename T, bool kInterleaved>
 __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const Task& t, int h0,
-                                        int h1, int c0, int lo, int hi, const double2* cs) {
+                                        int h1, const Part& p, const double2* cs) {
   const int units = a.c.dim / 16, row_heads = h1 - h0, turning = a.rot.pairs / 8;
   const int per_step = blockDim.x / units;
   const int mine = threadIdx.x / units, u = threadIdx.x - mine * units;
   if (mine >= per_step) return;
   const Unit w = UnitOf(u, a.rot);
-  for (int i = mine; i < (hi - lo) * row_heads; i += per_step) {
+  for (int i = mine; i < (p.hi - p.lo) * row_heads; i += per_step) {
     const int k = i / row_heads;
-    const int o = lo + k;
+    const int o = p.lo + k;
     const int64_t head = static_cast<int64_t>(h0 + i - k * row_heads) * a.c.dim;
-    const int64_t at = t.row + c0 + o;
-    const T* p = static_cast<const T*>(a.q) + at * a.q_stride + head;
+    const int64_t at = t.row + p.c0 + o;
+    const T* from = static_cast<const T*>(a.q) + at * a.q_stride + head;
     T* out = static_cast<T*>(a.q_out) + at * a.out_stride + head;
-    float x[16];
-    double y[16];
-    Load8(p + w.a, vec, x);
-    Load8(p + w.b, vec, x + 8);
-    Turn(x, cs + SineAt(o, 0, u, turning), turning, w, a.rot.interleaved, y);
+    Packed<T, 16> x;
+    x.Load8(0, from + w.a, vec);
+    x.Load8(8, from + w.b, vec);
+    // two pairs at a time: whole words of results
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = static_cast<float>(y[e]);
-    Store8(out + w.a, vec, x);
-    Store8(out + w.b, vec, x + 8);
-  }
-}
-
-// What a wave's side of a page starts from and ends with.
-struct Side {
-  uint8_t* codes = nullptr;  // the page's, of its head
-  float* scale = nullptr;
-  float had = 0.0f;
-};
-
-// A chunk's new offsets within it.
-struct Part {
-  int c0 = 0, lo = 0, hi = 0;
-};
-__device__ __forceinline__ Part PartOf(const Task& t, int c) {
-  Part p;
-  p.c0 = 16 * c;
-  p.lo = min(max(t.first - p.c0, 0), 16);
-  p.hi = min(t.end - p.c0, 16);
-  return p;
-}
-
-// The workgroup's barriers: both sides pass the same ones.  Before pass 1's
-// chunk c its sines replace the chunk's before; pass 2 forms them again unless
-// the new tokens lie in one chunk.
-__device__ __forceinline__ void NextSines(const Kv8AppendArgs& a, const Task& t, const Part& p,
-                                          double2* cs) {
-  __syncthreads();
-  FillSines(a, t, p.c0, p.lo, p.hi, cs);
-  __syncthreads();
-}
-
-// The largest new number first, then the codes.  New tokens of one chunk stay
-// in registers between the two; of several they are read again, from the cache.
-template <typename T, int FMT, int NU>
-__device__ __forceinline__ void KeySide(const Kv8AppendArgs& a, bool vec, const Task& t, int h0,
-                                        int h1, int h, const Side& side, double2* cs,
-                                        uint8_t* tile) {
-  constexpr int NV = (NU + 1) / 2;
-  const int group = a.q_heads / a.c.heads, lane = threadIdx.x & (kWave - 1);
-  const int chunk0 = t.first / 16, chunk1 = (t.end - 1) / 16;
-  const bool mine = h < h1;
-  float x[NU][16];
-  float most = 0.0f;
-  for (int c = chunk0; c <= chunk1; ++c) {
-    const Part p = PartOf(t, c);
-    if (mine) LoadKeys<T, NU>(a, vec, t, h, p.c0, p.lo, p.hi, x);
-    NextSines(a, t, p, cs);
-    if (mine) most = fmaxf(most, LargestKey<NU>(a, p.lo, p.hi, cs, x));
-    if (group > 0) Queries<T>(a, vec, t, h0 * group, h1 * group, p.c0, p.lo, p.hi, cs);
-  }
-  Scale s;
-  s.Set<FMT>(fmaxf(side.had, ScaleFor<FMT>(WaveMax(most))));
-  const bool grew = t.first > 0 && s.s > side.had;
-  const bool means = a.c.summaries != nullptr;
-  float sums[NV][2] = {};
-  for (int c = 0; c <= chunk1; ++c) {
-    const Part p = PartOf(t, c);
-    if (chunk0 != chunk1 && p.lo < p.hi) {
-      if (mine) LoadKeys<T, NU>(a, vec, t, h, p.c0, p.lo, p.hi, x);
-      NextSines(a, t, p, cs);
-    }
-    if (mine && (p.lo < p.hi || grew || means)) {
-      StoreKeys<FMT, NU>(a, side.codes + p.c0 * a.c.dim, p.lo, p.hi, side.had, grew, s, x, cs,
-                         tile, sums);
-    }
-  }
-  if (!mine) return;
-  if (lane == 0) {
-    *side.scale = s.s;
-    if (h == 0) a.c.token_counts[t.page] = t.end;
-  }
-  if (means) {
-    const double f = static_cast<double>(s.s);
-#pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      const int d = 128 * m + 2 * lane;
-      if (d < a.c.dim) {
-        float* out =
-            a.c.summaries + (static_cast<int64_t>(t.page) * a.c.heads + h) * a.c.dim + d;
-        out[0] = static_cast<float>(static_cast<double>(sums[m][0]) * f / t.end);
-        out[1] = static_cast<float>(static_cast<double>(sums[m][1]) * f / t.end);
+    for (int e = 0; e < 8; e += 2) {
+      const double2* at_cs = cs + SineAt(o, 0, u, turning);
+      const Turned y = TurnPair(x, 0, e, at_cs, turning, w, kInterleaved);
+      const Turned z = TurnPair(x, 0, e + 1, at_cs, turning, w, kInterleaved);
+      if constexpr (kInterleaved) {
+        x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(y.y1));
+        x.Set2(z.i0, static_cast<float>(z.y0), static_cast<float>(z.y1));
+      } else {
+        x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(z.y0));
+        x.Set2(y.i1, static_cast<float>(y.y1), static_cast<float>(z.y1));
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    x.Store8(0, out + w.a, vec);
+    x.Store8(8, out + w.b, vec);
   }
 }
 
-template <typename T, int FMT, int NU>
-__device__ __forceinline__ void ValueSide(const Kv8AppendArgs& a, bool vec, const Task& t, int h0,
-                                          int h1, int h, const Side& side, double2* cs) {
-  constexpr int NV = (NU + 1) / 2;
-  const int group = a.q_heads / a.c.heads, lane = threadIdx.x & (kWave - 1);
-  const int chunk0 = t.first / 16, chunk1 = (t.end - 1) / 16;
-  const bool mine = h < h1;
-  float x[NV][2][16];
-  float most = 0.0f;
-  for (int c = chunk0; c <= chunk1; ++c) {
-    const Part p = PartOf(t, c);
-    if (mine) {
-#pragma unroll
-      for (int m = 0; m < NV; ++m) {
-        LoadValues<T>(a, vec, t, h, p.c0, p.lo, p.hi, 128 * m + 2 * lane, x[m]);
-      }
-    }
-    NextSines(a, t, p, cs);
-#pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      if (mine) most = fmaxf(most, LargestValue(x[m]));
-    }
-    if (group > 0) Queries<T>(a, vec, t, h0 * group, h1 * group, p.c0, p.lo, p.hi, cs);
-  }
-  Scale s;
-  s.Set<FMT>(fmaxf(side.had, ScaleFor<FMT>(WaveMax(most))));
-  const bool grew = t.first > 0 && s.s > side.had;
-  for (int c = grew ? 0 : chunk0; c <= chunk1; ++c) {
-    const Part p = PartOf(t, c);
-    if (chunk0 != chunk1 && p.lo < p.hi) NextSines(a, t, p, cs);
-    if (!mine) continue;
-#pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      const int d = 128 * m + 2 * lane;
-      if (chunk0 != chunk1 && p.lo < p.hi) {
-        LoadValues<T>(a, vec, t, h, p.c0, p.lo, p.hi, d, x[m]);
-      }
-      if (d < a.c.dim) {
-        uint8_t* column = side.codes + p.c0 * a.c.dim + d * 16;
-        StoreValues<FMT>(column, p.lo, p.hi, side.had, grew, s, x[m][0]);
-        StoreValues<FMT>(column + 16, p.lo, p.hi, side.had, grew, s, x[m][1]);
-      }
-    }
-  }
-  if (mine && lane == 0) *side.scale = s.s;
-}
-
-template <typename T, int FMT, int NU>
+template <typename T, int FMT, int NU, bool kInterleaved>
 __global__ __launch_bounds__(2 * kMostPer * kWave) void Kv8AppendKernel(Kv8AppendArgs a, int per,
                                                                         bool vec) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int wave = threadIdx.x / kWave;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   if (a.b.max_tokens > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && wave == 0) {
     // (a malformed request may have no workgroup that looks at it)
     for (int r = threadIdx.x; r < a.b.batch; r += kWave) {
@@ -628,41 +561,105 @@ __global__ __launch_bounds__(2 * kMostPer * kWave) void Kv8AppendKernel(Kv8Appen
   }
   Task t;
   if (!FindTask(a, blockIdx.x, &t)) return;
-  const int heads = a.c.heads;
+  constexpr int NV = Numbers<T, NU>::kPlanes;
+  const int heads = a.c.heads, D = a.c.dim, group = a.q_heads / heads;
   const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
   const int h = h0 + wave / 2;
+  const bool mine = h < h1, keys = (wave & 1) == 0;
   double2* cs = reinterpret_cast<double2*>(smem);
-  const bool keys = (wave & 1) == 0;
+  uint8_t* tile = smem + sizeof(double2) * 16 * a.rot.pairs + wave / 2 * 16 * D;
   const int64_t page_head = static_cast<int64_t>(t.page) * heads + min(h, heads - 1);
-  Side side;
-  side.codes = (keys ? a.c.keys : a.c.values) + page_head * a.c.page * a.c.dim;
-  side.scale = (keys ? a.c.key_scales : a.c.value_scales) + page_head;
-  side.had = t.first > 0 ? *side.scale : 0.0f;
-  if (keys) {
-    uint8_t* tile = smem + sizeof(double2) * 16 * a.rot.pairs + wave / 2 * 16 * a.c.dim;
-    KeySide<T, FMT, NU>(a, vec, t, h0, h1, h, side, cs, tile);
-  } else {
-    ValueSide<T, FMT, NU>(a, vec, t, h0, h1, h, side, cs);
+  uint8_t* codes = (keys ? a.c.keys : a.c.values) + page_head * a.c.page * D;
+  float* scale = (keys ? a.c.key_scales : a.c.value_scales) + page_head;
+  const float had = t.first > 0 ? *scale : 0.0f;
+  const bool means = keys && a.c.summaries != nullptr;
+  const int chunk0 = t.first / 16, chunk1 = (t.end - 1) / 16;
+  const bool one = chunk0 == chunk1;
+
+  // First the largest new number, then the codes.  New tokens of one chunk stay
+  // in registers between the two; of several they are read again, from the
+  // cache, and their sines formed again.
+  Numbers<T, NU> x;
+  float most = 0.0f;
+  float sums[NV][2] = {};
+  Scale s;
+  bool grew = false;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      s.template Set<FMT>(fmaxf(had, ScaleFor<FMT>(WaveMax(most))));
+      grew = t.first > 0 && s.s > had;
+    }
+#pragma unroll 1
+    for (int c = pass == 1 && (grew || means) ? 0 : chunk0; c <= chunk1; ++c) {
+      const Part p = PartOf(t, c);
+      if (p.lo < p.hi && (pass == 0 || !one)) {
+        if (mine && keys) {
+          LoadKeys<T, NU>(a, vec, t, h, p, &x);
+        } else if (mine) {
+          LoadValues<T, NU>(a, vec, t, h, p, &x);
+        }
+        __syncthreads();
+        FillSines(a, t, p.c0, p.lo, p.hi, cs);
+        __syncthreads();
+      }
+      if (pass == 0) {
+        if (mine) {
+          most = fmaxf(most, keys ? LargestKey<T, NU, kInterleaved>(a, p, cs, x)
+                                  : LargestValue<T, NU>(x));
+        }
+        if (group > 0) {
+          Queries<T, kInterleaved>(a, vec, t, h0 * group, h1 * group, p, cs);
+        }
+      } else if (mine && keys) {
+        StoreKeys<FMT, T, NU, kInterleaved>(a, codes + p.c0 * D, p, had, grew, s, x, cs, tile,
+                                            sums);
+      } else if (mine) {
+#pragma unroll
+        for (int m = 0; m < NV; ++m) {
+          const int d = 128 * m + 2 * lane;
+          if (d < D) {
+            uint8_t* column = codes + p.c0 * D + d * 16;
+            StoreValues<FMT>(column, p.lo, p.hi, had, grew, s, x.x, 32 * m);
+            StoreValues<FMT>(column + 16, p.lo, p.hi, had, grew, s, x.x, 32 * m + 1);
+          }
+        }
+      }
+    }
+  }
+  if (!mine) return;
+  if (lane == 0) {
+    *scale = s.s;
+    if (h == 0 && keys) a.c.token_counts[t.page] = t.end;
+  }
+  if (means) {
+    const double f = static_cast<double>(s.s);
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const int d = 128 * m + 2 * lane;
+      if (d < D) {
+        float* out = a.c.summaries + page_head * D + d;
+        out[0] = static_cast<float>(static_cast<double>(sums[m][0]) * f / t.end);
+        out[1] = static_cast<float>(static_cast<double>(sums[m][1]) * f / t.end);
+      }
+    }
   }
 }
 
-template <typename T, int FMT, int NU>
-void Launch(const Kv8AppendArgs& a, bool vec, hipStream_t stream) {
-  const int per = std::min(2, a.c.heads);
-  const int64_t units = a.b.max_tokens > 1
-                            ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
-                            : a.b.batch;
-  const size_t lds = sizeof(double2) * 16 * a.rot.pairs + per * 16 * a.c.dim;
-  const dim3 grid(static_cast<unsigned>(units), (a.c.heads + per - 1) / per);
-  Kv8AppendKernel<T, FMT, NU><<<grid, 2 * per * kWave, lds, stream>>>(a, per, vec);
-  DSD_HIP_CHECK(hipGetLastError());
+// Calls f with the kernel of a head size.
+template <typename T, int FMT, bool kInterleaved, typename F>
+void WithDim(int dim, F&& f) {
+  if (dim <= 64) return f(Kv8AppendKernel<T, FMT, 1, kInterleaved>);
+  if (dim <= 128) return f(Kv8AppendKernel<T, FMT, 2, kInterleaved>);
+  return f(Kv8AppendKernel<T, FMT, 4, kInterleaved>);
 }
-
-template <typename T, int FMT>
-void LaunchDim(const Kv8AppendArgs& a, bool vec, hipStream_t stream) {
-  if (a.c.dim <= 64) return Launch<T, FMT, 1>(a, vec, stream);
-  if (a.c.dim <= 128) return Launch<T, FMT, 2>(a, vec, stream);
-  return Launch<T, FMT, 4>(a, vec, stream);
+template <typename T, typename F>
+void WithKernel(int format, int dim, bool interleaved, F&& f) {
+  if (format == DSD_KV8_INT8) {
+    interleaved ? WithDim<T, DSD_KV8_INT8, true>(dim, f) : WithDim<T, DSD_KV8_INT8, false>(dim, f);
+  } else {
+    interleaved ? WithDim<T, DSD_KV8_E4M3, true>(dim, f) : WithDim<T, DSD_KV8_E4M3, false>(dim, f);
+  }
 }
 
 template <typename T>
@@ -675,20 +672,23 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
   };
   const bool vec = even(a.k, a.k_stride) && even(a.v, a.v_stride) &&
                    (a.q_heads == 0 || (even(a.q, a.q_stride) && even(a.q_out, a.out_stride)));
-  a.c.format == DSD_KV8_INT8 ? LaunchDim<T, DSD_KV8_INT8>(a, vec, stream)
-                             : LaunchDim<T, DSD_KV8_E4M3>(a, vec, stream);
-}
-
-template <typename T, int FMT>
-void PreloadDim(const Kv8View& c) {
-  if (c.dim <= 64) return PreloadKernel(Kv8AppendKernel<T, FMT, 1>);
-  if (c.dim <= 128) return PreloadKernel(Kv8AppendKernel<T, FMT, 2>);
-  return PreloadKernel(Kv8AppendKernel<T, FMT, 4>);
+  const int per = std::min(2, a.c.heads);
+  const int64_t units = a.b.max_tokens > 1
+                            ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
+                            : a.b.batch;
+  const size_t lds = sizeof(double2) * 16 * a.rot.pairs + per * 16 * a.c.dim;
+  const dim3 grid(static_cast<unsigned>(units), (a.c.heads + per - 1) / per);
+  WithKernel<T>(a.c.format, a.c.dim, a.rot.interleaved != 0, [&](auto kernel) {
+    kernel<<<grid, 2 * per * kWave, lds, stream>>>(a, per, vec);
+  });
+  DSD_HIP_CHECK(hipGetLastError());
 }
 
 template <typename T>
 void PreloadType(const Kv8View& c) {
-  c.format == DSD_KV8_INT8 ? PreloadDim<T, DSD_KV8_INT8>(c) : PreloadDim<T, DSD_KV8_E4M3>(c);
+  for (bool interleaved : {false, true}) {
+    WithKernel<T>(c.format, c.dim, interleaved, [](auto kernel) { PreloadKernel(kernel); });
+  }
 }
 
 }  // namespace

@@ -1,6 +1,8 @@
 // kv8_device.h -- device helpers of the 8-bit paged cache's kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "kv8.h"
 #include "step_common.h"
 
@@ -59,43 +61,84 @@ __device__ __forceinline__ void WaveLdsFence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Eight consecutive elements as floats; vec: p is 16-byte aligned.
+// N consecutive elements as they lie in memory (16-bit ones two a word).
+template <typename T, int N>
+struct Packed {
+  unsigned w[N * sizeof(T) / 4];
+
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (std::is_same<T, float>::value) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __bf16>::value) {
+      return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    } else {
+      return static_cast<float>(
+          __builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)))));
+    }
+  }
+  // Elements i (even) and i + 1.
+  __device__ __forceinline__ void Set2(int i, float x, float y) {
+    if constexpr (std::is_same<T, float>::value) {
+      w[i] = __float_as_uint(x);
+      w[i + 1] = __float_as_uint(y);
+    } else {
+      typedef T T2 __attribute__((ext_vector_type(2)));
+      const F32x2 v = {x, y};
+      w[i >> 1] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, T2));
+    }
+  }
+  // Elements [at, at + 8) from p; vec: p is 16-byte aligned.
+  __device__ __forceinline__ void Load8(int at, const T* p, bool vec) {
+    unsigned* to = w + at * static_cast<int>(sizeof(T)) / 4;
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < static_cast<int>(sizeof(T)) * 2; k += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(p) + k);
+        to[k] = v.x;
+        to[k + 1] = v.y;
+        to[k + 2] = v.z;
+        to[k + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) to[k] = __float_as_uint(p[k]);
+    } else {
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        to[k] = from[2 * k] | static_cast<unsigned>(from[2 * k + 1]) << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void Store8(int at, T* p, bool vec) const {
+    const unsigned* from = w + at * static_cast<int>(sizeof(T)) / 4;
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < static_cast<int>(sizeof(T)) * 2; k += 4) {
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned*>(p) + k) =
+            make_uint4(from[k], from[k + 1], from[k + 2], from[k + 3]);
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] = __uint_as_float(from[k]);
+    } else {
+      uint16_t* to = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        to[2 * k] = static_cast<uint16_t>(from[k]);
+        to[2 * k + 1] = static_cast<uint16_t>(from[k] >> 16);
+      }
+    }
+  }
+};
+
+// Eight consecutive elements as floats.
 template <typename T>
 __device__ __forceinline__ void Load8(const T* p, bool vec, float* x) {
-  if (!vec) {
+  Packed<T, 8> raw;
+  raw.Load8(0, p, vec);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(p[i]);
-  } else if constexpr (sizeof(T) == 4) {
-    const F32x4 a = *reinterpret_cast<const F32x4*>(p);
-    const F32x4 b = *reinterpret_cast<const F32x4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
-    }
-  } else {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    const T8 a = *reinterpret_cast<const T8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a[i]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void Store8(T* p, bool vec, const float* x) {
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(x[i]);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<F32x4*>(p) = F32x4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<F32x4*>(p + 4) = F32x4{x[4], x[5], x[6], x[7]};
-  } else {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    T8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = static_cast<T>(x[i]);
-    *reinterpret_cast<T8*>(p) = a;
-  }
+  for (int i = 0; i < 8; ++i) x[i] = raw[i];
 }
 
 }  // namespace
