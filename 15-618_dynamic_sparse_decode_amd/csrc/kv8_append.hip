@@ -46,10 +46,8 @@ __device__ __forceinline__ float ScaleFor(float most) {
 __device__ __forceinline__ float ToOdd(double x) {
   const float y = static_cast<float>(x);
   const double back = static_cast<double>(y);
-  if (back == x || !(fabs(x) < 0x1p127)) return y;
-  unsigned bits = __float_as_uint(y);
-  if (fabs(back) > fabs(x)) --bits;
-  return __uint_as_float(bits | 1u);
+  const unsigned bits = __float_as_uint(y) - (fabs(back) > fabs(x) ? 1u : 0u);
+  return __uint_as_float(bits | (back != x && x == x ? 1u : 0u));
 }
 
 // A scale with its reciprocals.
@@ -113,6 +111,34 @@ __device__ __forceinline__ unsigned Codes4(X x0, X x1, X x2, X x3, const Scale& 
   }
 }
 
+// The same of finite numbers and a power of two, by the conversion's own scale.
+__device__ __forceinline__ unsigned PlainCodes4(float x0, float x1, float x2, float x3, float s) {
+  typedef short S2 __attribute__((ext_vector_type(2)));
+  S2 w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x0, x1, s, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x2, x3, s, true);
+  return __builtin_bit_cast(unsigned, w);
+}
+// Of four tokens' words of two 16-bit numbers each, their first or second ones.
+template <typename T>
+__device__ __forceinline__ unsigned PlainCodes4(unsigned w0, unsigned w1, unsigned w2, unsigned w3,
+                                                bool second, float s) {
+  typedef short S2 __attribute__((ext_vector_type(2)));
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  const unsigned take = second ? 0x07060302u : 0x05040100u;
+  const T2 a = __builtin_bit_cast(T2, __builtin_amdgcn_perm(w1, w0, take));
+  const T2 b = __builtin_bit_cast(T2, __builtin_amdgcn_perm(w3, w2, take));
+  S2 w = {0, 0};
+  if constexpr (std::is_same<T, __bf16>::value) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, a, s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, b, s, true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, a, s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, b, s, true);
+  }
+  return __builtin_bit_cast(unsigned, w);
+}
+
 // The four numbers that a word's codes stand for.
 template <int FMT>
 __device__ __forceinline__ void Numbers4(unsigned w, float* x) {
@@ -147,12 +173,6 @@ __device__ __forceinline__ float FiniteSize(float x) {
   return a < INFINITY ? a : 0.0f;
 }
 
-__device__ __forceinline__ float WaveMax(float x) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, kWave));
-  return x;
-}
-
 // Where a head's 16 elements of unit u lie: 8 from a on, 8 from b on, and
 // whether they turn with the sines of pairs [8 u, 8 u + 8).
 struct Unit {
@@ -180,28 +200,23 @@ __device__ __forceinline__ int SineAt(int o, int i, int u, int turning) {
 }
 
 // Pair i of a unit whose elements are x[at..at + 8) at a, x[at + 8..at + 16) at
-// b: its place from `at` on and its numbers turned.  cs: the unit's first pair, the others `step` apart.
-// (The schedule is held to a pair at a time: left to interleave them the
-// compiler takes twice the registers, half the waves a CU.)
+// b: its place from `at` on and its numbers turned.  cs: the unit's first pair,
+// the others `step` apart.
 struct Turned {
   int i0, i1;
   double y0, y1;
 };
 template <typename X>
 __device__ __forceinline__ Turned TurnPair(const X& x, int at, int i, const double2* cs, int step,
-                                           const Unit& u, bool interleaved) {
+                                           bool interleaved) {
   Turned t;
   t.i0 = interleaved ? 2 * i : i;
   t.i1 = interleaved ? 2 * i + 1 : 8 + i;
   const double p = static_cast<double>(x[at + t.i0]);
   const double q = static_cast<double>(x[at + t.i1]);
-  t.y0 = p;
-  t.y1 = q;
-  if (u.turns) {
-    const double2 w = cs[i * step];
-    t.y0 = p * w.x - q * w.y;
-    t.y1 = q * w.x + p * w.y;
-  }
+  const double2 w = cs[i * step];
+  t.y0 = fma(p, w.x, -(q * w.y));
+  t.y1 = fma(q, w.x, p * w.y);
   return t;
 }
 
@@ -248,11 +263,7 @@ __device__ __forceinline__ bool FindTask(const Kv8AppendArgs& a, int u, Task* t)
   const int slot0 = q.past / ps, last = (q.past + q.n - 1) / ps;
   const int slot = slot0 + within;
   if (slot > last) return false;
-  t->page = b.page_ids[q.list + slot];
-  if (!InPool(t->page, a.c.capacity)) {
-    if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
-    return false;
-  }
+  t->page = b.page_ids[q.list + slot];  // (checked where it is used)
   t->index = slot * ps;
   t->first = max(q.past - t->index, 0);
   t->end = min(q.past + q.n - t->index, ps);
@@ -260,28 +271,34 @@ __device__ __forceinline__ bool FindTask(const Kv8AppendArgs& a, int u, Task* t)
   return true;
 }
 
-// The sines and cosines of a chunk's tokens, offsets [lo, hi) of the 16 from
-// c0 on (SineAt).
+// The sines and cosines of the tokens at offsets [lo, hi) from c0 on (SineAt).
 __device__ __forceinline__ double2 Times(double2 a, double2 b) {
-  return {a.x * b.x - a.y * b.y, a.x * b.y + a.y * b.x};
+  return {fma(a.x, b.x, -(a.y * b.y)), fma(a.x, b.y, a.y * b.x)};
 }
 __device__ __forceinline__ void FillSines(const Kv8AppendArgs& a, const Task& t, int c0, int lo,
                                           int hi, double2* cs) {
   const int pairs = a.rot.pairs;
-  const int n = (hi - lo) * pairs;
-  const double2* table = a.rot.table;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int k = i / pairs, p = i - k * pairs;
-    const int o = c0 + lo + k;
-    const int at = a.b.positions != nullptr ? a.b.positions[t.row + o] : t.index + o;
+  if (pairs == 0) return;
+  // A thread has one pair of every `step`-th token.
+  const int step = max(static_cast<int>(blockDim.x) / pairs, 1);
+  const int k = threadIdx.x / pairs, p = threadIdx.x - k * pairs;
+  if (k >= step) return;
+  const double2* table = a.rot.table + p;
+  double2 high = {1.0, 0.0};
+  unsigned known = 0xffffffffu;  // whose upper bytes `high` is of
+  for (int o = lo + k; o < hi; o += step) {
+    const int at =
+        a.b.positions != nullptr ? a.b.positions[t.row + c0 + o] : t.index + c0 + o;
     const unsigned far = at < 0 ? 0u - static_cast<unsigned>(at) : static_cast<unsigned>(at);
-    const double2 w = Times(Times(table[(far & 255u) * pairs + p],
-                                  table[(256u + ((far >> 8) & 255u)) * pairs + p]),
-                            Times(table[(512u + ((far >> 16) & 255u)) * pairs + p],
-                                  table[(768u + (far >> 24)) * pairs + p]));
-    const double s = at < 0 ? -w.y : w.y;
-    cs[SineAt(lo + k, p & 7, p >> 3, pairs / 8)] = {w.x * a.rot.magnitude,
-                                                  s * a.rot.magnitude};
+    if (far >> 8 != known) {
+      known = far >> 8;
+      high = Times(Times(table[(256u + ((far >> 8) & 255u)) * pairs],
+                         table[(512u + ((far >> 16) & 255u)) * pairs]),
+                   table[(768u + (far >> 24)) * pairs]);
+      high = {high.x * a.rot.magnitude, high.y * a.rot.magnitude};
+    }
+    const double2 w = Times(table[(far & 255u) * pairs], high);
+    cs[SineAt(o, p & 7, p >> 3, pairs / 8)] = {w.x, at < 0 ? -w.y : w.y};
   }
 }
 
@@ -326,39 +343,77 @@ __device__ __forceinline__ void LoadKeys(const Kv8AppendArgs& a, bool vec, const
   }
 }
 
-template <typename T, int NU, bool kInterleaved>
-__device__ __forceinline__ float LargestKey(const Kv8AppendArgs& a, const Part& p,
-                                            const double2* cs, const Numbers<T, NU>& x) {
+constexpr unsigned kInfinity = 0x7f800000u;
+
+// The keys turned; returns the bits of the largest magnitude.  e4m3: into y, to
+// which they are rounded so that a code of y is the code of the key itself.
+// int8 keeps the numbers it was given and turns them again for their codes (and
+// leaves out what is not finite here).
+template <int FMT, typename T, int NU, bool kInterleaved>
+__device__ __forceinline__ unsigned TurnKeys(const Kv8AppendArgs& a, const Part& p,
+                                             const double2* cs, const Numbers<T, NU>& x,
+                                             float (&y)[16 * NU]) {
+  unsigned top = 0;
   const int lane = threadIdx.x & (kWave - 1);
   const int units = a.c.dim / 16, turning = a.rot.pairs / 8;
-  float most = 0.0f;
 #pragma unroll
   for (int j = 0; j < NU; ++j) {
     const int i = lane + kWave * j;
     const int o = i / units, u = i - o * units;
     if (o >= p.lo && o < p.hi) {
-      const Unit w = UnitOf(u, a.rot);
+      if (u < turning) {
+        const double2* at = cs + SineAt(o, 0, u, turning);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const Turned y = TurnPair(x.x, 16 * j, e, cs + SineAt(o, 0, u, turning), turning, w,
-                                  kInterleaved);
-        most = fmaxf(most, fmaxf(FiniteSize(static_cast<float>(y.y0)),
-                                 FiniteSize(static_cast<float>(y.y1))));
-        __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 8; ++e) {
+          const Turned z = TurnPair(x.x, 16 * j, e, at, turning, kInterleaved);
+          if constexpr (FMT == DSD_KV8_E4M3) {
+            y[16 * j + z.i0] = ToOdd(z.y0);
+            y[16 * j + z.i1] = ToOdd(z.y1);
+          } else {
+            top = max(top, max(__float_as_uint(FiniteSize(static_cast<float>(z.y0))),
+                               __float_as_uint(FiniteSize(static_cast<float>(z.y1)))));
+          }
+          // (two pairs at a time: all of them at once take twice the registers)
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          y[16 * j + e] = x.x[16 * j + e];
+          if (FMT != DSD_KV8_E4M3) top = max(top, __float_as_uint(FiniteSize(y[16 * j + e])));
+        }
       }
+    } else if (FMT == DSD_KV8_E4M3) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[16 * j + e] = 0.0f;
     }
   }
-  return most;
+  if constexpr (FMT == DSD_KV8_E4M3) {
+#pragma unroll
+    for (int e = 0; e < 16 * NU; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+  }
+  return top;
 }
 
-// One chunk's codes: offsets [lo, hi) new (x, turned again), those before them
-// as they are or brought from `had` to s.  tile: 16 x dim bytes of LDS.  sums:
-// the lane's dims 2 lane, 2 lane + 1 of each 128, summed over offsets [0, hi).
+// The bits of the largest finite magnitude.
+template <int N, typename X>
+__device__ __forceinline__ unsigned TopFinite(const X& x) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) most = fmaxf(most, FiniteSize(x[i]));
+  return __float_as_uint(most);
+}
+
+// One chunk's codes: offsets [lo, hi) new (y, or x turned again), those before
+// them as they are or brought from `had` to s.  plain: every new number is finite
+// and s a power of two.  tile: 16 x dim bytes of LDS.  sums: the lane's dims 2
+// lane, 2 lane + 1 of each 128, summed over offsets [0, hi).
 template <int FMT, typename T, int NU, bool kInterleaved>
 __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block, const Part& p,
-                                          float had, bool grew, const Scale& s,
-                                          const Numbers<T, NU>& x, const double2* cs,
-                                          uint8_t* tile, float (&sums)[(NU + 1) / 2][2]) {
+                                          float had, bool grew, const Scale& s, bool plain,
+                                          const Numbers<T, NU>& x, const float (&y)[16 * NU],
+                                          const double2* cs, uint8_t* tile,
+                                          float (&sums)[(NU + 1) / 2][2]) {
   const int lane = threadIdx.x & (kWave - 1);
   const int D = a.c.dim;
   const int units = D / 16, turning = a.rot.pairs / 8;
@@ -382,29 +437,41 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
     const int o = i / units, u = i - o * units;
     if (o >= lo && o < hi) {
       const Unit w = UnitOf(u, a.rot);
-      // four pairs at a time: two words of codes
+      uint8_t* to = tile + o * D;
+      unsigned c[4];
+      if constexpr (FMT == DSD_KV8_E4M3) {
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        double y[8];
+        for (int e = 0; e < 4; ++e) {
+          const int k = 16 * j + 4 * e;
+          c[e] = plain ? PlainCodes4(y[k], y[k + 1], y[k + 2], y[k + 3], s.s)
+                       : Codes4<FMT>(y[k], y[k + 1], y[k + 2], y[k + 3], s);
+        }
+      } else {
+        // four pairs at a time: two words of codes
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const Turned z = TurnPair(x.x, 16 * j, e + k, cs + SineAt(o, 0, u, turning), turning, w,
-                                    kInterleaved);
-          y[kInterleaved ? 2 * k : k] = z.y0;
-          y[kInterleaved ? 2 * k + 1 : 4 + k] = z.y1;
+        for (int e = 0; e < 8; e += 4) {
+          double z[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            Turned t;
+            if (u < turning) {
+              t = TurnPair(x.x, 16 * j, e + k, cs + SineAt(o, 0, u, turning), turning,
+                           kInterleaved);
+            } else {
+              t.y0 = static_cast<double>(x.x[16 * j + (kInterleaved ? 2 * (e + k) : e + k)]);
+              t.y1 = static_cast<double>(x.x[16 * j + (kInterleaved ? 2 * (e + k) + 1 : 8 + e + k)]);
+            }
+            z[kInterleaved ? 2 * k : k] = t.y0;
+            z[kInterleaved ? 2 * k + 1 : 4 + k] = t.y1;
+          }
+          // interleaved: elements 2 e .. 2 e + 8; else e .. e + 4 of both parts
+          c[kInterleaved ? e / 2 : e / 4] = Codes4<FMT>(z[0], z[1], z[2], z[3], s);
+          c[kInterleaved ? e / 2 + 1 : 2 + e / 4] = Codes4<FMT>(z[4], z[5], z[6], z[7], s);
+          __builtin_amdgcn_sched_barrier(0);  // (or all of it is live at once)
         }
-        const unsigned c0 = Codes4<FMT>(y[0], y[1], y[2], y[3], s);
-        const unsigned c1 = Codes4<FMT>(y[4], y[5], y[6], y[7], s);
-        // interleaved: elements 2 e .. 2 e + 8; else e .. e + 4 of both parts
-        uint8_t* to = tile + o * D;
-        if constexpr (kInterleaved) {
-          *reinterpret_cast<uint2*>(to + (e == 0 ? w.a : w.b)) = make_uint2(c0, c1);
-        } else {
-          *reinterpret_cast<unsigned*>(to + w.a + e) = c0;
-          *reinterpret_cast<unsigned*>(to + w.b + e) = c1;
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      *reinterpret_cast<uint2*>(to + w.a) = make_uint2(c[0], c[1]);
+      *reinterpret_cast<uint2*>(to + w.b) = make_uint2(c[2], c[3]);
     }
   }
   WaveLdsFence();
@@ -416,6 +483,7 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
     for (int m = 0; m < (NU + 1) / 2; ++m) {
       const int d = 128 * m + 2 * lane;
       if (d < D) {
+#pragma unroll 4
         for (int o = 0; o < hi; ++o) {
           float v[4];
           Numbers4<FMT>(*reinterpret_cast<const uint16_t*>(tile + o * D + d), v);
@@ -456,14 +524,26 @@ __device__ __forceinline__ void LoadValues(const Kv8AppendArgs& a, bool vec, con
   }
 }
 
+// The bits of the largest magnitude.
 template <typename T, int NU>
-__device__ __forceinline__ float LargestValue(const Numbers<T, NU>& x) {
-  float most = 0.0f;
+__device__ __forceinline__ unsigned TopValue(const Numbers<T, NU>& x) {
+  constexpr int kWords = 32 * Numbers<T, NU>::kPlanes * sizeof(T) / 4;
+  if constexpr (sizeof(T) == 4) {
+    unsigned top = 0;
 #pragma unroll
-  for (int i = 0; i < 32 * Numbers<T, NU>::kPlanes; ++i) {
-    most = fmaxf(most, FiniteSize(x.x[i]));
+    for (int i = 0; i < kWords; ++i) top = max(top, x.x.w[i] & 0x7fffffffu);
+    return top;
+  } else {
+    typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+    U2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(U2, x.x.w[i] & 0x7fff7fffu));
+    }
+    Packed<T, 2> most;
+    most.w[0] = max(top[0], top[1]);
+    return __float_as_uint(most[0]);
   }
-  return most;
 }
 
 // The byte mask of tokens [lo, hi) in word i (tokens 4 i ..) of a column.
@@ -476,15 +556,25 @@ __device__ __forceinline__ unsigned TokenMask(int i, int lo, int hi) {
 
 // column: the 16 codes of one dim, token t's number x[at + 2 t].  Tokens outside
 // [0, hi) stay as they are.
-template <int FMT, typename X>
+template <int FMT, typename T, typename X>
 __device__ __forceinline__ void StoreValues(uint8_t* column, int lo, int hi, float had, bool grew,
-                                            const Scale& s, const X& x, int at) {
+                                            const Scale& s, bool plain, const X& x, int at) {
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const int k = at + 8 * i;
     w[i] = 0u;
     if (lo < hi) {
-      w[i] = Codes4<FMT>(x[at + 8 * i], x[at + 8 * i + 2], x[at + 8 * i + 4], x[at + 8 * i + 6], s);
+      if (FMT == DSD_KV8_E4M3 && plain) {
+        if constexpr (std::is_same<T, float>::value) {
+          w[i] = PlainCodes4(x[k], x[k + 2], x[k + 4], x[k + 6], s.s);
+        } else {
+          const int b = k >> 1;
+          w[i] = PlainCodes4<T>(x.w[b], x.w[b + 1], x.w[b + 2], x.w[b + 3], (at & 1) != 0, s.s);
+        }
+      } else {
+        w[i] = Codes4<FMT>(x[k], x[k + 2], x[k + 4], x[k + 6], s);
+      }
     }
   }
   if (lo > 0 || hi < 16) {
@@ -502,13 +592,9 @@ __device__ __forceinline__ void StoreValues(uint8_t* column, int lo, int hi, flo
   *reinterpret_cast<uint4*>(column) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// ---- the kernel ----------------------------------------------------------------
-// Grid (pages' workgroups, groups of `per` key heads): 2 * per waves, wave w the
-// keys (w even) or values of key head w / 2 of the group; then all of them the
-// group's queries.  LDS: the sines of 16 tokens, then a 16 x dim tile per head.
-constexpr int kMostPer = 4;
+// ---- the kernels ---------------------------------------------------------------
 
-// Rotates the queries of a chunk's new tokens, heads [h0, h1).
+// Rotates the queries of the new tokens [p.lo, p.hi) from p.c0 on, heads [h0, h1).
 template <typename T, bool kInterleaved>
 __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const Task& t, int h0,
                                         int h1, const Part& p, const double2* cs) {
@@ -517,8 +603,9 @@ __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const 
   const int mine = threadIdx.x / units, u = threadIdx.x - mine * units;
   if (mine >= per_step) return;
   const Unit w = UnitOf(u, a.rot);
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(row_heads) + 1u;
   for (int i = mine; i < (p.hi - p.lo) * row_heads; i += per_step) {
-    const int k = i / row_heads;
+    const int k = row_heads == 1 ? i : static_cast<int>(__umulhi(i, inverse));
     const int o = p.lo + k;
     const int64_t head = static_cast<int64_t>(h0 + i - k * row_heads) * a.c.dim;
     const int64_t at = t.row + p.c0 + o;
@@ -528,40 +615,220 @@ __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const 
     x.Load8(0, from + w.a, vec);
     x.Load8(8, from + w.b, vec);
     // two pairs at a time: whole words of results
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    if (u < turning) {
       const double2* at_cs = cs + SineAt(o, 0, u, turning);
-      const Turned y = TurnPair(x, 0, e, at_cs, turning, w, kInterleaved);
-      const Turned z = TurnPair(x, 0, e + 1, at_cs, turning, w, kInterleaved);
-      if constexpr (kInterleaved) {
-        x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(y.y1));
-        x.Set2(z.i0, static_cast<float>(z.y0), static_cast<float>(z.y1));
-      } else {
-        x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(z.y0));
-        x.Set2(y.i1, static_cast<float>(y.y1), static_cast<float>(z.y1));
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const Turned y = TurnPair(x, 0, e, at_cs, turning, kInterleaved);
+        const Turned z = TurnPair(x, 0, e + 1, at_cs, turning, kInterleaved);
+        if constexpr (kInterleaved) {
+          x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(y.y1));
+          x.Set2(z.i0, static_cast<float>(z.y0), static_cast<float>(z.y1));
+        } else {
+          x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(z.y0));
+          x.Set2(y.i1, static_cast<float>(y.y1), static_cast<float>(z.y1));
+        }
+        if (e & 2) __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
     x.Store8(0, out + w.a, vec);
     x.Store8(8, out + w.b, vec);
   }
 }
 
-template <typename T, int FMT, int NU, bool kInterleaved>
-__global__ __launch_bounds__(2 * kMostPer * kWave) void Kv8AppendKernel(Kv8AppendArgs a, int per,
-                                                                        bool vec) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  if (a.b.max_tokens > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && wave == 0) {
-    // (a malformed request may have no workgroup that looks at it)
+// A malformed request may have no workgroup that looks at it: the last one does.
+__device__ __forceinline__ void CheckRequests(const Kv8AppendArgs& a) {
+  if (a.b.max_tokens > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 &&
+      threadIdx.x < kWave) {
     for (int r = threadIdx.x; r < a.b.batch; r += kWave) {
       Kv8Request q;
       if (!Kv8ReadTokens(a.b, r, a.c.page, &q)) ReportFailure(a.fail, kFailShape);
     }
   }
+}
+
+__device__ __forceinline__ unsigned WaveTop(unsigned x) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    x = max(x, static_cast<unsigned>(__shfl_xor(static_cast<int>(x), o, kWave)));
+  }
+  return x;
+}
+
+// What a wave does with its side of a head, a chunk at a time.
+template <typename T, int FMT, int NU, bool kInterleaved>
+struct Lane {
+  static constexpr int NV = Numbers<T, NU>::kPlanes;
+  Numbers<T, NU> x;
+  float y[16 * NU];      // keys turned (e4m3)
+  float sums[NV][2] = {};
+  float had = 0.0f;      // the page's scale so far (0: none)
+  Scale s;               // and from now on
+  bool grew = false;
+  bool plain = true;     // PlainCodes4 will do
+
+  __device__ __forceinline__ void Load(const Kv8AppendArgs& a, bool vec, const Task& t, bool keys,
+                                       int h, const Part& p) {
+    if (keys) {
+      LoadKeys<T, NU>(a, vec, t, h, p, &x);
+    } else {
+      LoadValues<T, NU>(a, vec, t, h, p, &x);
+    }
+  }
+  // The bits of the largest finite magnitude.
+  __device__ __forceinline__ unsigned Top(const Kv8AppendArgs& a, bool keys, const Part& p,
+                                          const double2* cs) {
+    unsigned top = keys ? TurnKeys<FMT, T, NU, kInterleaved>(a, p, cs, x, y) : TopValue<T, NU>(x);
+    if (__ballot(top >= kInfinity) != 0) {  // seldom
+      plain = false;
+      top = keys ? TopFinite<16 * NU>(y) : TopFinite<32 * NV>(x.x);
+    }
+    return top;
+  }
+  __device__ __forceinline__ void SetScale(const Task& t, unsigned top) {
+    s.template Set<FMT>(fmaxf(had, ScaleFor<FMT>(__uint_as_float(top))));
+    grew = t.first > 0 && s.s > had;
+    plain = plain && (__float_as_uint(s.s) & 0x007fffffu) == 0u;
+  }
+  __device__ __forceinline__ void Store(const Kv8AppendArgs& a, bool keys, uint8_t* chunk,
+                                        const Part& p, const double2* cs, uint8_t* tile) {
+    if (keys) {
+      StoreKeys<FMT, T, NU, kInterleaved>(a, chunk, p, had, grew, s, plain, x, y, cs, tile, sums);
+      return;
+    }
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const int d = 128 * m + 2 * static_cast<int>(threadIdx.x & (kWave - 1));
+      if (d < a.c.dim) {
+        StoreValues<FMT, T>(chunk + d * 16, p.lo, p.hi, had, grew, s, plain, x.x, 32 * m);
+        StoreValues<FMT, T>(chunk + d * 16 + 16, p.lo, p.hi, had, grew, s, plain, x.x, 32 * m + 1);
+      }
+    }
+  }
+  __device__ __forceinline__ void StoreMeans(const Kv8AppendArgs& a, const Task& t,
+                                             int64_t page_head) const {
+    const double f = static_cast<double>(s.s);
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const int d = 128 * m + 2 * static_cast<int>(threadIdx.x & (kWave - 1));
+      if (d < a.c.dim) {
+        float* out = a.c.summaries + page_head * a.c.dim + d;
+        out[0] = static_cast<float>(static_cast<double>(sums[m][0]) * f / t.end);
+        out[1] = static_cast<float>(static_cast<double>(sums[m][1]) * f / t.end);
+      }
+    }
+  }
+};
+
+// Pages of at most four chunks.  Grid (pages' workgroups, groups of `per` key
+// heads): 2 * per * chunks waves, wave w the keys (w even) or values of head
+// w / 2 % per of the group, chunk w / (2 * per); then all of them the group's
+// queries.  Every number is read once and stays in its lane until its code is
+// known.  LDS: the sines of a page's tokens, a 16 x dim tile and the sums of
+// each key wave, each wave's largest number.
+constexpr int kMostWaves = 8;
+template <typename T, int FMT, int NU, bool kInterleaved>
+__global__ __launch_bounds__(kMostWaves* kWave) void Kv8AppendKernel(Kv8AppendArgs a, int per,
+                                                                     bool vec) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  CheckRequests(a);
   Task t;
   if (!FindTask(a, blockIdx.x, &t)) return;
-  constexpr int NV = Numbers<T, NU>::kPlanes;
+  using L = Lane<T, FMT, NU, kInterleaved>;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int heads = a.c.heads, D = a.c.dim, chunks = a.c.chunks, group = a.q_heads / heads;
+  const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
+  const bool keys = (wave & 1) == 0;
+  const int within = wave / 2 % per, chunk = wave / (2 * per);
+  const int h = h0 + within;
+  const bool mine = h < h1;
+  double2* cs = reinterpret_cast<double2*>(smem);
+  const double2* my_cs = cs + SineAt(16 * chunk, 0, 0, a.rot.pairs / 8);
+  uint8_t* tiles = smem + sizeof(double2) * 16 * chunks * a.rot.pairs;
+  uint8_t* tile = tiles + wave / 2 * 16 * D;
+  float* all_sums = reinterpret_cast<float*>(tiles + per * chunks * 16 * D);
+  unsigned* all_tops = reinterpret_cast<unsigned*>(all_sums + per * chunks * D);
+
+  const Part p = PartOf(t, chunk);
+  const bool fresh = mine && p.lo < p.hi;
+  L w;
+  if (fresh) w.Load(a, vec, t, keys, h, p);
+  if (!InPool(t.page, a.c.capacity)) {  // (every wave's the same)
+    if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
+    return;
+  }
+  const int64_t page_head = static_cast<int64_t>(t.page) * heads + min(h, heads - 1);
+  float* scale = (keys ? a.c.key_scales : a.c.value_scales) + page_head;
+  w.had = t.first > 0 ? *scale : 0.0f;
+  FillSines(a, t, 0, t.first, t.end, cs);
+  __syncthreads();
+  unsigned top = fresh ? WaveTop(w.Top(a, keys, p, my_cs)) : 0u;
+  if (chunks > 1) {
+    if (lane == 0) all_tops[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < chunks; ++i) top = max(top, all_tops[(i * per + within) * 2 + (wave & 1)]);
+  }
+  w.SetScale(t, top);
+  const bool means = keys && a.c.summaries != nullptr;
+  if (mine && p.c0 < t.end && (fresh || w.grew || means)) {
+    uint8_t* codes = (keys ? a.c.keys : a.c.values) + (page_head * a.c.page + p.c0) * D;
+    w.Store(a, keys, codes, p, my_cs, tile);
+  }
+  if (mine && chunk == 0 && lane == 0) {
+    *scale = w.s.s;
+    if (h == 0 && keys) a.c.token_counts[t.page] = t.end;
+  }
+  if (a.c.summaries != nullptr) {
+    if (chunks > 1) {
+      if (mine && keys) {
+#pragma unroll
+        for (int m = 0; m < L::NV; ++m) {
+          const int d = 128 * m + 2 * lane;
+          if (d < D) {
+            *reinterpret_cast<float2*>(all_sums + wave / 2 * D + d) =
+                make_float2(w.sums[m][0], w.sums[m][1]);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (mine && keys && chunk == 0) {
+      for (int i = 1; i < chunks; ++i) {
+#pragma unroll
+        for (int m = 0; m < L::NV; ++m) {
+          const int d = 128 * m + 2 * lane;
+          if (d < D) {
+            w.sums[m][0] += all_sums[(i * per + within) * D + d];
+            w.sums[m][1] += all_sums[(i * per + within) * D + d + 1];
+          }
+        }
+      }
+      w.StoreMeans(a, t, page_head);
+    }
+  }
+  if (group > 0) {
+    Part all;
+    all.lo = t.first;
+    all.hi = t.end;
+    Queries<T, kInterleaved>(a, vec, t, h0 * group, h1 * group, all, cs);
+  }
+}
+
+// Larger pages: 2 * per waves, a wave all chunks of its side in turn, the largest
+// number of all of them first, then the codes; the second reading comes from the
+// cache, and the sines, of one chunk at a time, are formed again.
+template <typename T, int FMT, int NU, bool kInterleaved>
+__global__ __launch_bounds__(kMostWaves* kWave) void Kv8AppendPageKernel(Kv8AppendArgs a, int per,
+                                                                         bool vec) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  CheckRequests(a);
+  Task t;
+  if (!FindTask(a, blockIdx.x, &t)) return;
+  if (!InPool(t.page, a.c.capacity)) {
+    if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
+    return;
+  }
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int heads = a.c.heads, D = a.c.dim, group = a.q_heads / heads;
   const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
   const int h = h0 + wave / 2;
@@ -571,95 +838,70 @@ __global__ __launch_bounds__(2 * kMostPer * kWave) void Kv8AppendKernel(Kv8Appen
   const int64_t page_head = static_cast<int64_t>(t.page) * heads + min(h, heads - 1);
   uint8_t* codes = (keys ? a.c.keys : a.c.values) + page_head * a.c.page * D;
   float* scale = (keys ? a.c.key_scales : a.c.value_scales) + page_head;
-  const float had = t.first > 0 ? *scale : 0.0f;
   const bool means = keys && a.c.summaries != nullptr;
   const int chunk0 = t.first / 16, chunk1 = (t.end - 1) / 16;
-  const bool one = chunk0 == chunk1;
-
-  // First the largest new number, then the codes.  New tokens of one chunk stay
-  // in registers between the two; of several they are read again, from the
-  // cache, and their sines formed again.
-  Numbers<T, NU> x;
-  float most = 0.0f;
-  float sums[NV][2] = {};
-  Scale s;
-  bool grew = false;
+  Lane<T, FMT, NU, kInterleaved> w;
+  w.had = t.first > 0 ? *scale : 0.0f;
+  unsigned top = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    if (pass == 1) {
-      s.template Set<FMT>(fmaxf(had, ScaleFor<FMT>(WaveMax(most))));
-      grew = t.first > 0 && s.s > had;
-    }
+    if (pass == 1) w.SetScale(t, WaveTop(top));
 #pragma unroll 1
-    for (int c = pass == 1 && (grew || means) ? 0 : chunk0; c <= chunk1; ++c) {
+    for (int c = pass == 1 && (w.grew || means) ? 0 : chunk0; c <= chunk1; ++c) {
       const Part p = PartOf(t, c);
-      if (p.lo < p.hi && (pass == 0 || !one)) {
-        if (mine && keys) {
-          LoadKeys<T, NU>(a, vec, t, h, p, &x);
-        } else if (mine) {
-          LoadValues<T, NU>(a, vec, t, h, p, &x);
-        }
+      const bool fresh = p.lo < p.hi;
+      if (fresh) {
+        if (mine) w.Load(a, vec, t, keys, h, p);
         __syncthreads();
         FillSines(a, t, p.c0, p.lo, p.hi, cs);
         __syncthreads();
-      }
-      if (pass == 0) {
         if (mine) {
-          most = fmaxf(most, keys ? LargestKey<T, NU, kInterleaved>(a, p, cs, x)
-                                  : LargestValue<T, NU>(x));
+          const unsigned now = w.Top(a, keys, p, cs);
+          if (pass == 0) top = max(top, now);
         }
-        if (group > 0) {
-          Queries<T, kInterleaved>(a, vec, t, h0 * group, h1 * group, p, cs);
-        }
-      } else if (mine && keys) {
-        StoreKeys<FMT, T, NU, kInterleaved>(a, codes + p.c0 * D, p, had, grew, s, x, cs, tile,
-                                            sums);
-      } else if (mine) {
-#pragma unroll
-        for (int m = 0; m < NV; ++m) {
-          const int d = 128 * m + 2 * lane;
-          if (d < D) {
-            uint8_t* column = codes + p.c0 * D + d * 16;
-            StoreValues<FMT>(column, p.lo, p.hi, had, grew, s, x.x, 32 * m);
-            StoreValues<FMT>(column + 16, p.lo, p.hi, had, grew, s, x.x, 32 * m + 1);
-          }
-        }
+      }
+      if (pass == 1) {
+        if (mine) w.Store(a, keys, codes + p.c0 * D, p, cs, tile);
+      } else if (group > 0) {
+        Queries<T, kInterleaved>(a, vec, t, h0 * group, h1 * group, p, cs);
       }
     }
   }
   if (!mine) return;
   if (lane == 0) {
-    *scale = s.s;
+    *scale = w.s.s;
     if (h == 0 && keys) a.c.token_counts[t.page] = t.end;
   }
-  if (means) {
-    const double f = static_cast<double>(s.s);
-#pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      const int d = 128 * m + 2 * lane;
-      if (d < D) {
-        float* out = a.c.summaries + page_head * D + d;
-        out[0] = static_cast<float>(static_cast<double>(sums[m][0]) * f / t.end);
-        out[1] = static_cast<float>(static_cast<double>(sums[m][1]) * f / t.end);
-      }
-    }
-  }
+  if (means) w.StoreMeans(a, t, page_head);
 }
 
 // Calls f with the kernel of a head size.
+constexpr int kMostChunks = 4;
 template <typename T, int FMT, bool kInterleaved, typename F>
-void WithDim(int dim, F&& f) {
-  if (dim <= 64) return f(Kv8AppendKernel<T, FMT, 1, kInterleaved>);
-  if (dim <= 128) return f(Kv8AppendKernel<T, FMT, 2, kInterleaved>);
+void WithDim(const Kv8View& c, F&& f) {
+  if (c.chunks > kMostChunks) {
+    if (c.dim <= 64) return f(Kv8AppendPageKernel<T, FMT, 1, kInterleaved>);
+    if (c.dim <= 128) return f(Kv8AppendPageKernel<T, FMT, 2, kInterleaved>);
+    return f(Kv8AppendPageKernel<T, FMT, 4, kInterleaved>);
+  }
+  if (c.dim <= 64) return f(Kv8AppendKernel<T, FMT, 1, kInterleaved>);
+  if (c.dim <= 128) return f(Kv8AppendKernel<T, FMT, 2, kInterleaved>);
   return f(Kv8AppendKernel<T, FMT, 4, kInterleaved>);
 }
 template <typename T, typename F>
-void WithKernel(int format, int dim, bool interleaved, F&& f) {
-  if (format == DSD_KV8_INT8) {
-    interleaved ? WithDim<T, DSD_KV8_INT8, true>(dim, f) : WithDim<T, DSD_KV8_INT8, false>(dim, f);
+void WithKernel(const Kv8View& c, bool interleaved, F&& f) {
+  if (c.format == DSD_KV8_INT8) {
+    interleaved ? WithDim<T, DSD_KV8_INT8, true>(c, f) : WithDim<T, DSD_KV8_INT8, false>(c, f);
   } else {
-    interleaved ? WithDim<T, DSD_KV8_E4M3, true>(dim, f) : WithDim<T, DSD_KV8_E4M3, false>(dim, f);
+    interleaved ? WithDim<T, DSD_KV8_E4M3, true>(c, f) : WithDim<T, DSD_KV8_E4M3, false>(c, f);
   }
+}
+// Waves of a head, and LDS.
+int Across(const Kv8View& c) { return c.chunks > kMostChunks ? 1 : c.chunks; }
+size_t LdsBytes(const Kv8View& c, int pairs, int per) {
+  const int across = Across(c);
+  return sizeof(double2) * 16 * across * pairs + per * across * (16 + sizeof(float)) * c.dim +
+         sizeof(unsigned) * kMostWaves;
 }
 
 template <typename T>
@@ -672,14 +914,14 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
   };
   const bool vec = even(a.k, a.k_stride) && even(a.v, a.v_stride) &&
                    (a.q_heads == 0 || (even(a.q, a.q_stride) && even(a.q_out, a.out_stride)));
-  const int per = std::min(2, a.c.heads);
+  const int per = std::min(Across(a.c) == 1 ? 2 : 1, a.c.heads);
   const int64_t units = a.b.max_tokens > 1
                             ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
                             : a.b.batch;
-  const size_t lds = sizeof(double2) * 16 * a.rot.pairs + per * 16 * a.c.dim;
   const dim3 grid(static_cast<unsigned>(units), (a.c.heads + per - 1) / per);
-  WithKernel<T>(a.c.format, a.c.dim, a.rot.interleaved != 0, [&](auto kernel) {
-    kernel<<<grid, 2 * per * kWave, lds, stream>>>(a, per, vec);
+  WithKernel<T>(a.c, a.rot.interleaved != 0, [&](auto kernel) {
+    kernel<<<grid, 2 * per * Across(a.c) * kWave, LdsBytes(a.c, a.rot.pairs, per), stream>>>(
+        a, per, vec);
   });
   DSD_HIP_CHECK(hipGetLastError());
 }
@@ -687,7 +929,12 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
 template <typename T>
 void PreloadType(const Kv8View& c) {
   for (bool interleaved : {false, true}) {
-    WithKernel<T>(c.format, c.dim, interleaved, [](auto kernel) { PreloadKernel(kernel); });
+    WithKernel<T>(c, interleaved, [&](auto kernel) {
+      PreloadKernel(kernel);
+      DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(LdsBytes(c, c.dim / 2, 2))));
+    });
   }
 }
 
