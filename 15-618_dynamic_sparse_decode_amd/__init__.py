@@ -242,6 +242,13 @@ _SIGNATURES = {
                               + [ctypes.c_void_p, ctypes.c_int64] * 2
                               + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
                               + [ctypes.c_void_p] * 2),
+    "dsd_kv8_sparse_create": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int] * 4
+                              + [ctypes.POINTER(ctypes.c_void_p)]),
+    "dsd_kv8_sparse_destroy": (ctypes.c_int, [ctypes.c_void_p]),
+    "dsd_kv8_sparse_run": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int] * 4
+                           + [ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 3
+                           + [ctypes.c_int64] + [ctypes.c_void_p] * 3),
+    "dsd_kv8_sparse_status": (ctypes.c_int, [ctypes.c_void_p]),
     "dsd_kv8_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
                                                ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
 }
@@ -992,6 +999,52 @@ class Kv8Cache:
         _check(self._lib.dsd_kv8_workspace_bytes(self.handle, batch.pointer, num_q_heads,
                                                  ctypes.byref(out)))
         return out.value
+
+
+class Kv8SparseStep:
+    """The sparse step over a Kv8Cache (dsd_kv8_sparse_*): page scores through
+    the cache's summaries, the top_k pages of each request, attention over
+    them.  Addresses are device memory, the step is asynchronous."""
+
+    def __init__(self, cache: Kv8Cache, num_q_heads: int, top_k: int, max_batch: int,
+                 max_total_candidates: int):
+        self._lib = load_library()
+        self.cache = cache
+        handle = ctypes.c_void_p()
+        _check(self._lib.dsd_kv8_sparse_create(cache.handle, num_q_heads, top_k, max_batch,
+                                               max_total_candidates, ctypes.byref(handle)))
+        self.handle = handle
+        self.num_q_heads, self.top_k = num_q_heads, top_k
+
+    def close(self) -> None:
+        if self.handle:
+            _check(self._lib.dsd_kv8_sparse_destroy(self.handle))
+            self.handle = ctypes.c_void_p()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def run(self, batch: int, total_candidates: int, max_candidates: int, dtype: int, q: int,
+            q_stride: int, cand_offsets: int, cand_ids: int, out: int, out_stride: int,
+            selected: int = 0, selected_counts: int = 0, stream: int = 0) -> None:
+        status = self._lib.dsd_kv8_sparse_run(
+            self.handle, batch, total_candidates, max_candidates, dtype, q, q_stride, cand_offsets,
+            cand_ids, out, out_stride, selected or None, selected_counts or None, stream)
+        if status:
+            _check(status)
+
+    def status(self) -> None:
+        """Synchronize; raise what a step found wrong with its lists."""
+        _check(self._lib.dsd_kv8_sparse_status(self.handle))
 
 
 # ---------------------------------------------------------------------------

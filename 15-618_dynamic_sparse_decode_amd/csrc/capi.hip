@@ -3430,3 +3430,166 @@ int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, in
 }
 
 }  // extern "C"
+
+// The sparse step over an 8-bit cache: the score and select stages of a context
+// whose pool is the cache's summaries and token counts (no keys or values; the
+// stages read none), then the 8-bit attention over what they select.
+struct dsd_kv8_sparse {
+  dsd_kv8* cache = nullptr;
+  int q_heads = 0;
+  dsd_pool* pool = nullptr;
+  dsd_sparse_ctx* ctx = nullptr;
+  DeviceBuffer<unsigned char> workspace;
+  bool used = false;
+  hipStream_t last = nullptr;  // of the last step (the default one: null)
+
+  // Steps share the scratch: one on another stream follows the last one.
+  void OrderOn(hipStream_t s) {
+    if (used && last != s) {
+      DSD_HIP_CHECK(hipEventRecord(ctx->ev_switch, last));
+      DSD_HIP_CHECK(hipStreamWaitEvent(s, ctx->ev_switch, 0));
+    }
+    used = true;
+    last = s;
+  }
+
+  ~dsd_kv8_sparse() {
+    delete ctx;
+    if (pool != nullptr) {
+      pool->view = PoolView{};  // (the cache's memory)
+      delete pool;
+    }
+  }
+};
+
+extern "C" {
+
+int dsd_kv8_sparse_create(dsd_kv8* cache, int num_q_heads, int top_k, int max_batch,
+                          int max_total_candidates, dsd_kv8_sparse** out) {
+  return Guard([&] {
+    Require(out != nullptr, "out must be non-null");
+    *out = nullptr;
+    Require(cache != nullptr, "cache must be non-null");
+    cache->RequireCurrent();
+    RequireHeads(cache, num_q_heads);
+    Require(num_q_heads > 0, "num_q_heads must be positive");
+    Require(cache->view.summaries != nullptr, "the cache keeps no summaries");
+    Require(top_k >= 0 && max_batch >= 0 && max_total_candidates >= 0,
+            "sizes must be non-negative");
+    Require(max_batch <= 65535, "at most 65535 requests per call");
+    Require(static_cast<int64_t>(max_batch) * std::max(1, top_k) <= 0x7fffffff,
+            "max_batch * top_k must fit 31 bits");
+    auto step = std::make_unique<dsd_kv8_sparse>();
+    step->cache = cache;
+    step->q_heads = num_q_heads;
+    const dsdk::Kv8View& c = cache->view;
+    step->pool = new dsd_pool;
+    PoolView& v = step->pool->view;
+    v.summaries = c.summaries;
+    v.token_counts = c.token_counts;
+    v.num_heads = c.heads;
+    v.head_dim = c.dim;
+    v.page_size = c.page;
+    v.elements = c.heads * c.dim;
+    v.capacity = c.capacity;
+    v.page_elems = static_cast<int64_t>(c.page) * v.elements;
+    DSD_HIP_CHECK(hipStreamCreateWithFlags(&step->pool->stream, hipStreamNonBlocking));
+    const int status =
+        dsd_sparse_create(step->pool, top_k, max_batch, max_total_candidates, 0, &step->ctx);
+    if (status == DSD_ERR_INVALID_ARGUMENT) throw std::invalid_argument(g_last_error);
+    if (status != DSD_OK) throw dsdk::HipError(g_last_error);
+    dsd_kv8_batch b = {};
+    b.batch = max_batch;
+    b.max_pages = std::max(1, top_k);
+    // (fewer requests may be cut into more pieces: the most any batch takes)
+    size_t most = 0;
+    for (int n = 1; n <= max_batch; ++n) {
+      b.batch = n;
+      most = std::max(most, dsdk::Kv8WorkspaceBytes(c, b, num_q_heads));
+    }
+    if (most > 0) step->workspace.Reserve(most);
+    *out = step.release();
+  });
+}
+
+int dsd_kv8_sparse_destroy(dsd_kv8_sparse* step) {
+  return Guard([&] {
+    if (step == nullptr) return;
+    (void)hipDeviceSynchronize();
+    delete step;
+  });
+}
+
+int dsd_kv8_sparse_run(dsd_kv8_sparse* step, int batch, int total_candidates, int max_candidates,
+                       int type, const void* q, int64_t q_stride, const int* d_cand_offsets,
+                       const int* d_cand_ids, void* out, int64_t out_stride, int* d_selected,
+                       int* d_selected_counts, void* stream) {
+  return Guard([&] {
+    Require(step != nullptr, "step must be non-null");
+    dsd_kv8* cache = step->cache;
+    dsd_sparse_ctx* ctx = step->ctx;
+    cache->RequireCurrent();
+    const size_t size = TypeSize(type);
+    Require(batch >= 0 && total_candidates >= 0 && max_candidates >= 0,
+            "sizes must be non-negative");
+    if (batch == 0) return;
+    Require(batch <= ctx->max_batch, "request batch exceeds the step's capacity");
+    Require(total_candidates <= ctx->max_cand, "candidate page count exceeds the step's capacity");
+    RequireRows(cache, q, q_stride, step->q_heads, size);
+    RequireRows(cache, out, out_stride, step->q_heads, size);
+    Require(d_cand_offsets != nullptr, "cand_offsets must be non-null");
+    if (total_candidates > 0) {
+      Require(d_cand_ids != nullptr, "cand_ids must be non-null");
+      Require(cache->view.capacity > 0, "the cache holds no page");
+    }
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    StepLaunch L = ctx->Plan(batch, total_candidates, max_candidates, false);
+    L.fused = L.wide = L.wide_shape = false;
+    L.queries = ctx->d_queries.ptr;
+    L.offsets = d_cand_offsets;
+    L.ids = d_cand_ids;
+    if (d_selected != nullptr) L.selected = d_selected;
+    if (d_selected_counts != nullptr) L.counts = d_selected_counts;
+    if (s != nullptr && StreamCapturing(s)) {
+      L.epoch_src = ctx->d_epoch.ptr;  // (the select's helpers stay out of a graph)
+      step->used = false;
+    } else {
+      step->OrderOn(s);
+    }
+    ctx->Fresh(&L);
+    dsdk::LaunchKv8GroupQueries(cache->view, batch, type, step->q_heads, q, q_stride,
+                                ctx->d_queries.ptr, s);
+    EnqueueScoreStage(ctx->pool->view, L, s);
+    EnqueueSelectStage(ctx->pool->view, L, s);
+    dsdk::Kv8AttendArgs a;
+    a.c = cache->view;
+    a.b.batch = batch;
+    a.b.max_tokens = 1;
+    a.b.max_pages = std::max(1, ctx->top_k);
+    a.b.list_stride = std::max(1, ctx->top_k);
+    a.b.total_pages = batch * a.b.list_stride;
+    a.b.page_ids = L.selected;
+    a.b.page_counts = L.counts;
+    a.type = type;
+    a.q_heads = step->q_heads;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.scale = 1.0f / std::sqrt(static_cast<float>(cache->view.dim));
+    a.workspace = step->workspace.ptr;
+    a.workspace_bytes = step->workspace.count;
+    a.fail = L.Fail();
+    dsdk::LaunchKv8Attend(a, s);
+  });
+}
+
+int dsd_kv8_sparse_status(dsd_kv8_sparse* step) {
+  return Guard([&] {
+    Require(step != nullptr, "step must be non-null");
+    DSD_HIP_CHECK(hipDeviceSynchronize());
+    step->ctx->CheckFailure(0);
+  });
+}
+
+}  // extern "C"

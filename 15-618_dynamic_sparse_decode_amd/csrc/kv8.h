@@ -38,7 +38,7 @@ struct Kv8Rotation {
 struct Kv8AppendArgs {
   Kv8View c;
   Kv8Rotation rot;
-  dsd_kv8_batch b;
+  dsd_kv8_batch b = {};
   int type = 0;  // DSD_TYPE_*
   int q_heads = 0;
   const void* q = nullptr;
@@ -52,7 +52,7 @@ void LaunchKv8Append(const Kv8AppendArgs& a, hipStream_t stream);
 
 struct Kv8AttendArgs {
   Kv8View c;
-  dsd_kv8_batch b;
+  dsd_kv8_batch b = {};
   int type = 0;
   int q_heads = 0;
   bool causal = false;  // several query tokens a request, each over what precedes it
@@ -68,6 +68,9 @@ void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream);
 // The form of it for many rows (kv8_prompt.hip).
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
+// Each key head's queries summed, in order, in float32: sums[batch][heads * dim].
+void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, const void* q,
+                           int64_t q_stride, float* sums, hipStream_t stream);
 // The kernels that calls on such a cache run.
 void PreloadKv8Append(const Kv8View& c);
 void PreloadKv8Attend(const Kv8View& c);

@@ -432,6 +432,20 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(o[e]);
 }
 
+// Grid (256 numbers of a row each, batch).
+template <typename T>
+__global__ __launch_bounds__(256) void Kv8GroupQueriesKernel(const T* q, int64_t q_stride,
+                                                             int group, int dim, int elements,
+                                                             float* sums) {
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= elements) return;
+  const int head = e / dim, d = e - head * dim;
+  const T* p = q + blockIdx.y * q_stride + static_cast<int64_t>(head) * group * dim + d;
+  float sum = static_cast<float>(p[0]);
+  for (int g = 1; g < group; ++g) sum += static_cast<float>(p[g * dim]);
+  sums[static_cast<int64_t>(blockIdx.y) * elements + e] = sum;
+}
+
 constexpr int kWaves = 4;
 
 // How a batch's lists are cut, by its sizes alone (the lengths themselves are
@@ -508,6 +522,7 @@ template <typename T>
 void PreloadType(const Kv8View& c) {
   c.format == DSD_KV8_INT8 ? PreloadDim<T, DSD_KV8_INT8>(c) : PreloadDim<T, DSD_KV8_E4M3>(c);
   PreloadKernel(Kv8MergeKernel<T>);
+  PreloadKernel(Kv8GroupQueriesKernel<T>);
 }
 
 }  // namespace
@@ -517,6 +532,23 @@ size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) 
   const size_t one = PlanBytes(c, b, MakePlan(c, b, q_heads, false));
   if (ManyRows(c, b, q_heads)) return one;
   return std::max(one, PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
+}
+
+void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, const void* q,
+                           int64_t q_stride, float* sums, hipStream_t stream) {
+  const int elements = c.heads * c.dim;
+  const dim3 grid((elements + 255) / 256, batch);
+  auto launch = [&](auto* rows) {
+    using T = std::remove_cv_t<std::remove_pointer_t<decltype(rows)>>;
+    Kv8GroupQueriesKernel<T><<<grid, 256, 0, stream>>>(rows, q_stride, q_heads / c.heads, c.dim,
+                                                       elements, sums);
+  };
+  switch (type) {
+    case DSD_TYPE_F32: launch(static_cast<const float*>(q)); break;
+    case DSD_TYPE_BF16: launch(static_cast<const __bf16*>(q)); break;
+    default: launch(static_cast<const _Float16*>(q));
+  }
+  DSD_HIP_CHECK(hipGetLastError());
 }
 
 void PreloadKv8Attend(const Kv8View& c) {

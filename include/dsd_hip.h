@@ -645,9 +645,11 @@ int dsd_dense_run_batch_device(dsd_pool* pool, int batch,
  * captured into a graph.  They allocate nothing and keep nothing between
  * calls, so calls on several streams are independent as far as their memory
  * is.  d_fail (may be NULL): memory the device writes
- * a code to when it skips a request: 2 its offsets or lengths do not fit the
- * batch's sizes, 3 a page id outside the cache; the caller clears it before
- * and reads it after the call.  Nothing outside the arrays is touched then. */
+ * a code to when it cannot use an input: 2 a request's offsets or lengths do
+ * not fit the batch's sizes (the request is skipped; dsd_kv8_attend gives it
+ * zeros), 3 a page id outside the cache (the page holds no token, takes none);
+ * the caller clears it before and reads it after the call.  Nothing outside the
+ * arrays is touched then. */
 typedef struct dsd_kv8 dsd_kv8;
 
 enum { DSD_KV8_E4M3 = 0, DSD_KV8_INT8 = 1 };
@@ -758,6 +760,36 @@ int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
  * these sizes (the pointers are not read). */
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                             int num_q_heads, size_t* bytes);
+
+/* The sparse step (dsd_sparse_run_batch_device) over an 8-bit cache that keeps
+ * summaries: every candidate page scored through its summary, the top_k pages
+ * of each request kept, attention over those.  A page's score is the sum over
+ * key heads of (the sum of the head's queries) . (the page's mean key), times
+ * 1 / sqrt(D), each sum a sequential float32 one: with one query head per key
+ * head the score of dsd_sparse_*; selection equals that order's bit for bit,
+ * the lower id first among equals.  head_dim up to 128.
+ * The handle holds the scratch for max_batch requests of max_total_candidates
+ * pages in all; the cache must outlive it.  Steps on one handle share the
+ * scratch: a step on a stream other than the last step's first waits for that
+ * stream, which must still be valid.  On a capturing stream the step is
+ * recorded into the graph, and the caller orders replays and other steps. */
+typedef struct dsd_kv8_sparse dsd_kv8_sparse;
+int dsd_kv8_sparse_create(dsd_kv8* cache, int num_q_heads, int top_k,
+                          int max_batch, int max_total_candidates,
+                          dsd_kv8_sparse** out);
+int dsd_kv8_sparse_destroy(dsd_kv8_sparse* step);
+/* Device pointers; enqueued on `stream` (NULL: the default stream).  Sizes and
+ * candidate lists as dsd_sparse_run_batch_device's, rows as dsd_kv8_attend's.
+ * d_selected ([batch][top_k], unused slots untouched) and d_selected_counts may
+ * be NULL. */
+int dsd_kv8_sparse_run(dsd_kv8_sparse* step, int batch, int total_candidates,
+                       int max_candidates, int type, const void* q,
+                       int64_t q_stride, const int* d_cand_offsets,
+                       const int* d_cand_ids, void* out, int64_t out_stride,
+                       int* d_selected, int* d_selected_counts, void* stream);
+/* As dsd_sparse_device_status: waits for the device and reports what the steps
+ * found wrong with their lists. */
+int dsd_kv8_sparse_status(dsd_kv8_sparse* step);
 
 #ifdef __cplusplus
 }

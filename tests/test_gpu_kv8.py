@@ -795,3 +795,112 @@ def test_streams_and_graph(gpu):
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
+
+
+# ---- the sparse step ----------------------------------------------------------------
+
+def group_sums(q, kv):
+    """Each key head's queries added in order in float32, as rows [batch][kv * dim]."""
+    q = q.float().cpu().numpy()
+    B, H, D = q.shape
+    q = q.reshape(B, kv, H // kv, D)
+    total = q[:, :, 0].copy()
+    for g in range(1, H // kv):
+        total = (total + q[:, :, g]).astype(np.float32)
+    return total.reshape(B, kv * D)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,kind,fmt,k,lengths", [
+    (8, 2, 64, 16, "bf16", kv8.E4M3, 4, [300, 16, 1, 900]),
+    (4, 4, 128, 32, "f32", kv8.INT8, 8, [2000, 77]),
+    (32, 8, 128, 16, "f16", kv8.E4M3, 8, [700, 512, 2048]),
+    (6, 2, 80, 64, "f32", kv8.E4M3, 3, [1000, 64]),
+    (8, 2, 64, 16, "bf16", kv8.E4M3, 40, [9000, 8000]),  # beyond the certified helper's 256
+])
+def test_sparse_step(gpu, heads, kv, dim, page, kind, fmt, k, lengths):
+    """Prompts appended, then the step: the selection is the sequential float32
+    order's over the cache's own summaries, the output that of attention over
+    the selected pages."""
+    import torch
+    import _oracle as orc
+    rng = np.random.default_rng(dim + k)
+    need = [-(-n // page) for n in lengths]
+    pair = Pair(gpu, kv, dim, page, sum(need), fmt)
+    pair.cache.set_rotation(dim, inv_freq(dim))
+    lists = lists_for(rng, lengths, page, sum(need))
+    prompt = Batch(gpu, lists, [0] * len(lengths), lengths)
+    key, value = (rows(rng, kind, sum(lengths), kv, dim) for _ in range(2))
+    append(pair, prompt, kind, None, key, value, None)
+    # the model takes the cache as it is (the append has tests of its own)
+    stored = pair.stored()
+    pair.model.codes = [np.nan_to_num(x) for x in stored]
+    pair.model.scales = [pair.key_scales.cpu().numpy(), pair.value_scales.cpu().numpy()]
+    pair.model.counts = pair.counts.cpu().numpy()
+    q = rows(rng, kind, len(lengths), heads, dim)
+    out = torch.full_like(q, 9.0)
+    cand = Batch(gpu, lists)
+    offsets = np.concatenate([[0], np.cumsum(need)]).astype(np.int32)
+    ids = np.concatenate(lists).astype(np.int32)
+    selected = torch.full((len(lengths), k), -1, dtype=torch.int32, device="cuda")
+    counts = torch.zeros(len(lengths), dtype=torch.int32, device="cuda")
+    with gpu.Kv8SparseStep(pair.cache, heads, k, len(lengths), len(ids)) as step:
+        args = (len(lengths), len(ids), max(need), TYPES[kind], q.data_ptr(), q.stride(0),
+                cand.keep["page_offsets"].data_ptr(), cand.keep["page_ids"].data_ptr(),
+                out.data_ptr(), out.stride(0))
+        step.run(*args, selected=selected.data_ptr(), selected_counts=counts.data_ptr())
+        step.status()
+        summaries = pair.summaries.cpu().numpy()
+        E = kv * dim
+        zeros = np.zeros((sum(need), page, E), np.float32)
+        _, want, _ = orc.sparse_batch(group_sums(q, kv), zeros, zeros, summaries, pair.model.counts,
+                                      offsets, ids, kv, dim, page, k)
+        for r in range(len(lengths)):
+            n = int(counts[r])
+            assert selected[r, :n].tolist() == list(want[r]), r
+        kept = Batch(gpu, [list(w) for w in want])
+        check_attention(pair, kept, kind, q, out)
+        # without the caller's id buffers, on another stream, and as a graph
+        want_out = out.clone()
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for stream in (side.cuda_stream, 0, side.cuda_stream):
+            out.fill_(9.0)
+            torch.cuda.synchronize()
+            step.run(*args, stream=stream)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want_out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step.run(*args, stream=torch.cuda.current_stream().cuda_stream)
+        for _ in range(3):
+            out.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want_out)
+
+
+def test_sparse_step_refuses(gpu):
+    import torch
+    pair = Pair(gpu, 2, 64, 16, 4, rubbish=False)
+    q = torch.zeros(2, 4, 64, device="cuda")
+    with pytest.raises(gpu.InvalidArgument, match="summaries"):
+        gpu.Kv8SparseStep(Pair(gpu, 2, 64, 16, 4, summaries=False).cache, 4, 2, 2, 4)
+    with pytest.raises(gpu.InvalidArgument, match="head_dim"):
+        gpu.Kv8SparseStep(Pair(gpu, 2, 256, 16, 4).cache, 4, 2, 2, 4)
+    for args in ((3, 2, 2, 4), (4, -1, 2, 4), (4, 2, -1, 4), (4, 2, 70000, 4)):
+        with pytest.raises(gpu.InvalidArgument):
+            gpu.Kv8SparseStep(pair.cache, *args)
+    lists = Batch(gpu, [[0, 9], [1]])
+    with gpu.Kv8SparseStep(pair.cache, 4, 2, 2, 4) as step:
+        good = [2, 3, 2, 0, q.data_ptr(), 256, lists.keep["page_offsets"].data_ptr(),
+                lists.keep["page_ids"].data_ptr(), q.data_ptr(), 256]
+        for i, bad in ((0, 3), (1, 5), (3, 7), (4, 0), (5, 3), (6, 0), (7, 0), (8, 0)):
+            args = list(good)
+            args[i] = bad
+            with pytest.raises(gpu.InvalidArgument):
+                step.run(*args)
+        step.run(*good)  # page 9 is outside the cache
+        with pytest.raises(gpu.OutOfRange):
+            step.status()
+        step.status()
+        assert not bool(q.any())

@@ -56,6 +56,13 @@ def test_null_handles_are_refused(dsd):
     assert lib.dsd_kv8_attend_prompt(None, batch.pointer, 0, 1, None, 0, None, 0, 0.0, None, 0,
                                      None, None) == 1
     assert lib.dsd_kv8_workspace_bytes(None, batch.pointer, 1, None) == 1
+    out = ctypes.c_void_p()
+    assert lib.dsd_kv8_sparse_create(None, 1, 1, 1, 1, ctypes.byref(out)) == 1
+    assert lib.dsd_kv8_sparse_create(None, 1, 1, 1, 1, None) == 1
+    assert lib.dsd_kv8_sparse_destroy(None) == 0
+    assert lib.dsd_kv8_sparse_status(None) == 1
+    assert lib.dsd_kv8_sparse_run(None, 1, 1, 1, 0, None, 0, None, None, None, 0, None, None,
+                                  None) == 1
 
 
 def test_no_gpu_is_an_error(dsd):
