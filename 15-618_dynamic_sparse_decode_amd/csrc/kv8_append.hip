@@ -898,8 +898,9 @@ void WithKernel(const Kv8View& c, bool interleaved, F&& f) {
 }
 // Waves of a head, and LDS.
 int Across(const Kv8View& c) { return c.chunks > kMostChunks ? 1 : c.chunks; }
-size_t LdsBytes(const Kv8View& c, int pairs, int per) {
-  const int across = Across(c);
+int HeadsPerGroup(const Kv8View& c) { return std::min(Across(c) == 1 ? 2 : 1, c.heads); }
+size_t LdsBytes(const Kv8View& c, int pairs) {
+  const int across = Across(c), per = HeadsPerGroup(c);
   return sizeof(double2) * 16 * across * pairs + per * across * (16 + sizeof(float)) * c.dim +
          sizeof(unsigned) * kMostWaves;
 }
@@ -914,13 +915,13 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
   };
   const bool vec = even(a.k, a.k_stride) && even(a.v, a.v_stride) &&
                    (a.q_heads == 0 || (even(a.q, a.q_stride) && even(a.q_out, a.out_stride)));
-  const int per = std::min(Across(a.c) == 1 ? 2 : 1, a.c.heads);
+  const int per = HeadsPerGroup(a.c);
   const int64_t units = a.b.max_tokens > 1
                             ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
                             : a.b.batch;
   const dim3 grid(static_cast<unsigned>(units), (a.c.heads + per - 1) / per);
   WithKernel<T>(a.c, a.rot.interleaved != 0, [&](auto kernel) {
-    kernel<<<grid, 2 * per * Across(a.c) * kWave, LdsBytes(a.c, a.rot.pairs, per), stream>>>(
+    kernel<<<grid, 2 * per * Across(a.c) * kWave, LdsBytes(a.c, a.rot.pairs), stream>>>(
         a, per, vec);
   });
   DSD_HIP_CHECK(hipGetLastError());
@@ -933,7 +934,7 @@ void PreloadType(const Kv8View& c) {
       PreloadKernel(kernel);
       DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                         hipFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(LdsBytes(c, c.dim / 2, 2))));
+                                        static_cast<int>(LdsBytes(c, c.dim / 2))));
     });
   }
 }

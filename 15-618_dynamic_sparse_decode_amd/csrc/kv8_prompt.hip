@@ -63,6 +63,9 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
                                                                            int group, int blocks) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>;
   constexpr int KS = 4 * NU, NT = 2 * NU;
+  // (the scheduler's groups: vector, matrix, LDS reads)
+  constexpr int kValu = 0x002, kMfma = 0x008, kDsRead = 0x100;
+  constexpr int kAhead = 6, kHalfValu = 16 * (NP == 2 ? 8 : 5);
   extern __shared__ __align__(16) _Float16 smem[];
   const Kv8View& c = a.c;
   const int D = kDim > 0 ? kDim : c.dim, units = D / 16;
@@ -100,32 +103,22 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
     return k;
   };
 
-  // A group's codes on their way to LDS: thread i has 16 bytes i + 256 j of the
-  // keys and of the values.
+  // A group's codes on their way to LDS: a chunk's keys and its values are dim
+  // units of 16 bytes each, at the same offset of both arrays, and thread i has
+  // units i + 256 j of the group's four chunks.
   uint4 kw[NU], vw[NU];
   auto fetch = [&](int grp) {
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int i = threadIdx.x + kThreads * j;
       if (kDim > 0 || i < 4 * D) {
-        const int t = i / units, u = i - t * units;
-        int sub;
-        const int page = place(4 * grp + (t >> 4), &sub).page;
-        kw[j] = *reinterpret_cast<const uint4*>(
-            c.keys + static_cast<int64_t>(page * c.heads + head) * page_bytes +
-            (sub * 16 + (t & 15)) * D + u * 16);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NU; ++j) {
-      const int i = threadIdx.x + kThreads * j;
-      if (kDim > 0 || i < 4 * D) {
-        const int k = i / D, d = i - k * D;
+        const int k = i / D;
         int sub;
         const int page = place(4 * grp + k, &sub).page;
-        vw[j] = *reinterpret_cast<const uint4*>(
-            c.values + static_cast<int64_t>(page * c.heads + head) * page_bytes +
-            (sub * D + d) * 16);
+        const int64_t at = static_cast<int64_t>(page * c.heads + head) * page_bytes +
+                           (sub * D + i - k * D) * 16;
+        kw[j] = *reinterpret_cast<const uint4*>(c.keys + at);
+        vw[j] = *reinterpret_cast<const uint4*>(c.values + at);
       }
     }
   };
@@ -143,17 +136,12 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
     for (int j = 0; j < NU; ++j) {
       const int i = threadIdx.x + kThreads * j;
       if (kDim > 0 || i < 4 * D) {
+        // as keys: 16 dims of token t; as values: 16 tokens of dim d
         const int t = i / units, u = i - t * units;
+        const int k = i / D, d = i - k * D;
         _Float16* to = keys + t * (D + 8) + u * 16;
         *reinterpret_cast<F16x8*>(to) = Numbers8<FMT>(kw[j].x, kw[j].y);
         *reinterpret_cast<F16x8*>(to + 8) = Numbers8<FMT>(kw[j].z, kw[j].w);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NU; ++j) {
-      const int i = threadIdx.x + kThreads * j;
-      if (kDim > 0 || i < 4 * D) {
-        const int k = i / D, d = i - k * D;
         unsigned w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
         if (tail) {
           // Codes behind the request's tokens may be anything, and 0 * NaN is not 0.
@@ -171,12 +159,14 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
 #pragma unroll
             for (int e = 3; e >= 0; --e) {
               const unsigned is = NanBytes(w[e]);
-              if (is != 0u) atomicMin(&nan_from[d], grp * kGroup + 16 * k + 4 * e + (__ffs(is) >> 3) - 1);
+              if (is != 0u) {
+                atomicMin(&nan_from[d], grp * kGroup + 16 * k + 4 * e + (__ffs(is) >> 3) - 1);
+              }
               w[e] &= ~((is >> 7) * 0xffu);
             }
           }
         }
-        _Float16* to = values + d * kValueStride + 16 * k;
+        to = values + d * kValueStride + 16 * k;
         *reinterpret_cast<F16x8*>(to) = Numbers8<FMT>(w[0], w[1]);
         *reinterpret_cast<F16x8*>(to + 8) = Numbers8<FMT>(w[2], w[3]);
       }
@@ -266,6 +256,16 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
           }
         }
       }
+      if constexpr (kDim > 0) {
+        // Six operands on their way before the first product, then one a product.
+        __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS - kAhead; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, NQ, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead * NQ, 0);
+      }
       ChunkInfo ci[2];
       float f[2];
 #pragma unroll
@@ -318,10 +318,10 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
         }
       }
 #pragma unroll
-      for (int d = 0; d < NT; ++d) {
-        if (kDim > 0 || 32 * d < D) {
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+        for (int d = 0; d < NT; ++d) {
+          if (kDim > 0 || 32 * d < D) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const F16x8 v = *reinterpret_cast<const F16x8*>(values + 32 * d * kValueStride +
@@ -333,6 +333,23 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
             }
           }
         }
+      }
+      if constexpr (kDim > 0) {
+        // The first half's products beside the second half's exponentials.
+        __builtin_amdgcn_sched_group_barrier(kValu, kHalfValu, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, NP, 0);
+          __builtin_amdgcn_sched_group_barrier(kValu, kHalfValu / (2 * NT), 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NT - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, NP, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4 * NP, 0);
       }
     }
     if (grp + 1 < groups) put(grp + 1, buf ^ 1);
