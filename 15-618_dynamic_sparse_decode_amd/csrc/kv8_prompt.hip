@@ -20,6 +20,10 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRows = 32 * kWaves;
 constexpr int kGroup = 64;             // tokens
+// The running maxima follow a row's once it is 2^4 ahead of them (following it at
+// once, 64 products an update, cost 6%): weights reach 2^(11 + 4).
+constexpr float kSlack = 4.0f;
+constexpr float kPromptBits = 11.0f;
 constexpr int kValueStride = kGroup + 8;  // halves of a dim's row in LDS (16 bytes off the banks)
 
 // The larger (sum) of the two lanes that share lane % 32.
@@ -63,9 +67,8 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
                                                                            int group, int blocks) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>;
   constexpr int KS = 4 * NU, NT = 2 * NU;
-  // (the scheduler's groups: vector, matrix, LDS reads)
-  constexpr int kValu = 0x002, kMfma = 0x008, kDsRead = 0x100;
-  constexpr int kAhead = 6, kHalfValu = 16 * (NP == 2 ? 8 : 5);
+  constexpr int kMfma = 0x008, kDsRead = 0x100;  // (the scheduler's groups)
+  constexpr int kAhead = 4;
   extern __shared__ __align__(16) _Float16 smem[];
   const Kv8View& c = a.c;
   const int D = kDim > 0 ? kDim : c.dim, units = D / 16;
@@ -221,6 +224,7 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   }
   float m = -INFINITY, l = 0.0f;
   float mv = -INFINITY;  // of s + log2(value scale): acc is relative to it
+  // (m and mv follow within kSlack)
 
   __syncthreads();
   fetch(0);
@@ -241,6 +245,7 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
       const _Float16* values =
           value_tiles + buf * ValueHalves(D) + n * kValueStride + 16 * h;
       F32x16 x[2];
+      float to_half[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
         }
       }
       if constexpr (kDim > 0) {
-        // Six operands on their way before the first product, then one a product.
+        // kAhead operands on their way before the first product, then one a product.
         __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
         for (int i = 0; i < 2 * KS - kAhead; ++i) {
@@ -295,61 +300,62 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
       const float m_new = fmaxf(m, Max2(fmaxf(most[0], most[1])));
       const float mv_new = fmaxf(
           mv, Max2(fmaxf(most[0] + ci[0].log_value_scale, most[1] + ci[1].log_value_scale)));
-      const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float base_v = mv_new == -INFINITY ? 0.0f : mv_new;
-      if (__ballot(m_new > m || mv_new > mv) != 0) {
-        l *= Exp2(m - base);
-        const float shrink = Exp2(mv - base_v);
+      if (__ballot(m_new > m + kSlack || mv_new > mv + kSlack) != 0) {
+        const float from = m_new == -INFINITY ? 0.0f : m_new;
+        const float from_v = mv_new == -INFINITY ? 0.0f : mv_new;
+        l *= Exp2(m - from);
+        const float shrink = Exp2(mv - from_v);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] *= shrink;
         m = m_new;
         mv = mv_new;
       }
-      F16x8 w[2][2][NP];
+      const float base = m == -INFINITY ? 0.0f : m;
+      const float base_v = mv == -INFINITY ? 0.0f : mv;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const float to_half = ci[t].value_scale * Exp2(base - base_v + kWeightBits);
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float e0 = Exp2(fmaf(x[t][i], f[t], -base));
-          const float e1 = Exp2(fmaf(x[t][i + 1], f[t], -base));
-          l += e0 + e1;
-          SplitWeights(e0 * to_half, e1 * to_half, w[t][i >> 3], i & 7);
-        }
+        to_half[t] = ci[t].value_scale * Exp2(base - base_v + kPromptBits);
       }
+      // The weights of the first 32 tokens; then their products with the weights
+      // of the others in between, as the two units take turns; then the others'.
+      // Operands are asked for kAhead products before theirs.
+      F16x8 w[2][2][NP];
+      auto weights = [&](int t, int i) {  // elements i, i + 1
+        const float e0 = Exp2(fmaf(x[t][i], f[t], -base));
+        const float e1 = Exp2(fmaf(x[t][i + 1], f[t], -base));
+        l += e0 + e1;
+        SplitWeights(e0 * to_half[t], e1 * to_half[t], w[t][i >> 3], i & 7);
+      };
+      constexpr int kSteps = 2 * NT;
+      F16x8 v[2 * kSteps];
+      auto operand = [&](int step) {
+        const int t = step / kSteps, d = step % kSteps / 2, k = step % 2;
+        if (kDim > 0 || 32 * d < D) {
+          v[step] = *reinterpret_cast<const F16x8*>(values + 32 * d * kValueStride + 32 * t + 8 * k);
+        }
+      };
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int i = 0; i < kAhead; ++i) operand(i);
 #pragma unroll
-        for (int d = 0; d < NT; ++d) {
-          if (kDim > 0 || 32 * d < D) {
+      for (int i = 0; i < 16; i += 2) weights(0, i);
+      if (kDim > 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const F16x8 v = *reinterpret_cast<const F16x8*>(values + 32 * d * kValueStride +
-                                                              32 * t + 8 * k);
+      for (int step = 0; step < 2 * kSteps; ++step) {
+        const int t = step / kSteps, d = step % kSteps / 2, k = step % 2;
+        if (step + kAhead < 2 * kSteps) operand(step + kAhead);
+        if (kDim > 0 || 32 * d < D) {
 #pragma unroll
-              for (int i = 0; i < NP; ++i) {
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[t][k][i], acc[d], 0, 0, 0);
-              }
-            }
+          for (int i = 0; i < NP; ++i) {
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[step], w[t][k][i], acc[d], 0, 0, 0);
           }
         }
-      }
-      if constexpr (kDim > 0) {
-        // The first half's products beside the second half's exponentials.
-        __builtin_amdgcn_sched_group_barrier(kValu, kHalfValu, 0);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+        if (t == 0) {
 #pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kMfma, NP, 0);
-          __builtin_amdgcn_sched_group_barrier(kValu, kHalfValu / (2 * NT), 0);
-          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+          for (int i = 0; i < 8; ++i) {
+            if (i * kSteps / 8 == step) weights(1, 2 * i);
+          }
+          if (kDim > 0) __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int i = 0; i < 2 * NT - 4; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kMfma, NP, 0);
-          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 4 * NP, 0);
       }
     }
     if (grp + 1 < groups) put(grp + 1, buf ^ 1);
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   l = Sum2(l);
   if (!there) return;
   const float base = m == -INFINITY ? 0.0f : m;
-  const float to_out = Exp2(mv - base - kWeightBits) / l;
+  const float to_out = Exp2(mv - base - kPromptBits) / l;
   T* out = static_cast<T*>(a.out) + (s.q.row0 + token) * a.out_stride +
            static_cast<int64_t>(q_head) * D;
 #pragma unroll

@@ -152,9 +152,10 @@ def allowed(out, weighted, size, peak, dim, tokens, kind):
     relative error (the row's maximum moves too) and 2^-21 of their own; a weight
     is rounded to 2^-11 (one half) or 2^-21 (two); sums over the tokens add
     tokens * 2^-24, numerator and denominator each.  All of it acts on sum p |v|.
-    A weight (times its page's scale) is held relative to 2^15 / the row's
-    largest, and a half's numbers end in steps of 2^-24 there: each token's is off
-    by 2^-40 of the largest besides, times a code of at most peak over it.
+    A weight (times its page's scale) is held so that the row's largest lies in
+    [2^11, 2^15], and a half's numbers end in steps of 2^-24: each token's is off
+    by half a step, 2^-25 / 2^11 = 2^-36 of the largest, besides, times a code of
+    at most peak over it.
     The output is rounded once, by half a step of its type.  2^-126: results
     below the normal numbers."""
     half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[kind]
@@ -162,5 +163,5 @@ def allowed(out, weighted, size, peak, dim, tokens, kind):
     weight = 2.0 ** -11 if kind == "bf16" else 2.0 ** -21
     rel = 4 * logit + 2 * (2.0 ** -21 + tokens * 2.0 ** -24) + weight
     floor = 2.0 ** -24 if kind == "f16" else 2.0 ** -126
-    least = (tokens * 2.0 ** -40 * peak)[:, None] if tokens else 0.0
+    least = (tokens * 2.0 ** -36 * peak)[:, None] if tokens else 0.0
     return half * np.abs(out) + rel[:, None] * (1 + half) * weighted + least + floor
