@@ -312,19 +312,23 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
       }
       const float base = m == -INFINITY ? 0.0f : m;
       const float base_v = mv == -INFINITY ? 0.0f : mv;
+      // A weight is 2^(s - base + c), c = log2 of the value scale + base - base_v +
+      // 11, of which the row's sum wants 2^(s - base): the chunk's own sum times
+      // 2^-c.  (Where c < -60 the weights are no half-precision number either way.)
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        to_half[t] = ci[t].value_scale * Exp2(base - base_v + kPromptBits);
+        to_half[t] = fmaxf(ci[t].log_value_scale - base_v + kPromptBits, -60.0f - base);
       }
       // The weights of the first 32 tokens; then their products with the weights
       // of the others in between, as the two units take turns; then the others'.
       // Operands are asked for kAhead products before theirs.
       F16x8 w[2][2][NP];
       auto weights = [&](int t, int i) {  // elements i, i + 1
-        const float e0 = Exp2(fmaf(x[t][i], f[t], -base));
-        const float e1 = Exp2(fmaf(x[t][i + 1], f[t], -base));
-        l += e0 + e1;
-        SplitWeights(e0 * to_half[t], e1 * to_half[t], w[t][i >> 3], i & 7);
+        const float y0 = Exp2(fmaf(x[t][i], f[t], to_half[t]));
+        const float y1 = Exp2(fmaf(x[t][i + 1], f[t], to_half[t]));
+        sum[t] += y0 + y1;
+        SplitWeights(y0, y1, w[t][i >> 3], i & 7);
       };
       constexpr int kSteps = 2 * NT;
       F16x8 v[2 * kSteps];
@@ -357,6 +361,8 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
           if (kDim > 0) __builtin_amdgcn_sched_barrier(0);
         }
       }
+      l += sum[0] * Exp2(-base - to_half[0]);
+      l += sum[1] * Exp2(-base - to_half[1]);
     }
     if (grp + 1 < groups) put(grp + 1, buf ^ 1);
   }
