@@ -67,6 +67,7 @@ struct Kv8AttendArgs {
 void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream);
 // The form of it for many rows (kv8_prompt.hip).
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream);
+size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 // Each key head's queries summed, in order, in float32: sums[batch][heads * dim].
 void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, const void* q,

@@ -165,5 +165,148 @@ __device__ __forceinline__ void SplitWeights(float y0, float y1, F16x8 (&w)[NP],
   }
 }
 
+// Four numbers of an output row; vec: they lie on four elements' bytes.
+template <typename T>
+__device__ __forceinline__ void StoreRow4(T* p, bool vec, F32x4 o) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const T4 x = __builtin_convertvector(o, T4);
+  if (vec) {
+    *reinterpret_cast<T4*>(p) = x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = x[e];
+  }
+}
+
+// ---- lists cut into pieces ------------------------------------------------------
+// Where a launch has fewer workgroups than the chip runs at once, each row
+// block's list is cut into pieces of equal numbers of 64-token groups, by the
+// batch's sizes alone (the lengths themselves are on the device); a second launch
+// joins them.
+constexpr int kMostPieces = 64;
+struct Plan {
+  int group = 1;     // query heads per key head
+  int64_t rows = 1;  // of a request and key head, at most
+  int block = 16;    // rows of a workgroup
+  int blocks = 1;    // of a request and key head, at most
+  int pieces = 1;    // a list is cut into at most this many
+  int piece = 1;     // groups of 64 tokens in a piece
+  float* part = nullptr;    // [batch][key heads][rows][pieces][dim]
+  float2* stats = nullptr;  // [batch][key heads][rows][pieces]: (m, l), l < 0: no token
+};
+__device__ __forceinline__ int64_t PartSlot(const Plan& p, int heads, int r, int head, int row) {
+  return ((static_cast<int64_t>(r) * heads + head) * p.rows + row) * p.pieces;
+}
+// The pieces that a span's list is cut into.
+__device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {
+  const int groups = (s.chunks + 3) / 4;
+  return min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
+}
+
+// One row's pieces.  Grid (key heads * rows, batch): the pieces' factors first, in LDS, so that the sums' loads wait for nothing; the
+// threads beyond a row's quads take every 256 / quads-th piece, and their sums
+// are added in that order.
+template <typename T>
+__global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
+  __shared__ float factor[kMostPieces];
+  __shared__ F32x4 part_sum[256];
+  const Kv8View& c = a.c;
+  const int D = c.dim, quads = D / 4;
+  const int r = blockIdx.y, head = blockIdx.x % c.heads;
+  const int at = blockIdx.x / c.heads, first = at / p.block * p.block;
+  Span s;
+  if (!FindSpan(a, p.group, r, first, p.block, &s)) return;
+  const int pieces = Pieces(p, s);
+  if (pieces == 1 || at >= s.rows) return;
+  const int64_t slot0 = PartSlot(p, c.heads, r, head, at);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int shares = 256 / quads;  // threads per quad
+  const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
+  if (threadIdx.x < kWave) {
+    float2 st = make_float2(-INFINITY, -1.0f);
+    if (lane < pieces) st = p.stats[slot0 + lane];
+    const bool some = !(st.y < 0.0f);
+    float peak = some ? st.x : -INFINITY;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+    const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
+    float sum = some ? st.y * e : 0.0f;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+    factor[lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+  }
+  // (loads that do not need the factors are on their way meanwhile)
+  constexpr int kAhead = 4;
+  const float* part = p.part + slot0 * D + d;
+  F32x4 x[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int z = share + i * shares;
+    x[i] = F32x4{0, 0, 0, 0};
+    if (share < shares && z < pieces) {
+      x[i] = *reinterpret_cast<const F32x4*>(part + z * D);
+    }
+  }
+  __syncthreads();
+  F32x4 o = {0, 0, 0, 0};
+  if (share < shares) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int z = share + i * shares;
+      if (z < pieces) o += x[i] * factor[z];
+    }
+#pragma unroll 4
+    for (int z = share + kAhead * shares; z < pieces; z += shares) {
+      o += *reinterpret_cast<const F32x4*>(part + z * D) * factor[z];
+    }
+  }
+  part_sum[threadIdx.x] = o;
+  __syncthreads();
+  if (share > 0) return;
+  for (int i = 1; i < shares; ++i) o += part_sum[i * quads + threadIdx.x];
+  const int tok = at / p.group;
+  T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
+           static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
+  StoreRow4(out, reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0, o);
+}
+
+// Pieces of at least `least` groups, until there are `target` workgroups.
+inline void CutLists(Plan* p, const Kv8View& c, const dsd_kv8_batch& b, int target, int least) {
+  p->blocks = static_cast<int>((p->rows + p->block - 1) / p->block);
+  const int64_t groups = (static_cast<int64_t>(b.max_pages) * c.page + 63) / 64;
+  const int64_t units = static_cast<int64_t>(c.heads) * p->blocks * b.batch;
+  int64_t want = target / (units > 0 ? units : 1);
+  if (want > (groups + least - 1) / least) want = (groups + least - 1) / least;
+  if (want > kMostPieces) want = kMostPieces;
+  p->pieces = static_cast<int>(want > 1 ? want : 1);
+  const int64_t piece = (groups + p->pieces - 1) / p->pieces;
+  p->piece = static_cast<int>(piece > 1 ? piece : 1);
+}
+
+inline size_t PlanSlots(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
+  return static_cast<size_t>(b.batch) * c.heads * p.rows * p.pieces;
+}
+inline size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
+  return p.pieces == 1 ? 0 : PlanSlots(c, b, p) * (sizeof(float) * c.dim + sizeof(float2));
+}
+// The pieces' places in the call's workspace; without one lists stay whole.
+inline void PlaceParts(Plan* p, const Kv8AttendArgs& a) {
+  if (p->pieces > 1 && (a.workspace == nullptr || a.workspace_bytes < PlanBytes(a.c, a.b, *p))) {
+    p->pieces = 1;
+    p->piece = 1;
+  }
+  if (p->pieces == 1) return;
+  p->part = static_cast<float*>(a.workspace);
+  p->stats = reinterpret_cast<float2*>(p->part + PlanSlots(a.c, a.b, *p) * a.c.dim);
+}
+
+template <typename T>
+void Merge(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
+  if (p.pieces == 1) return;
+  const dim3 grid(static_cast<unsigned>(a.c.heads * p.rows), a.b.batch);
+  Kv8MergeKernel<T><<<grid, 256, 0, stream>>>(a, p);
+  DSD_HIP_CHECK(hipGetLastError());
+}
+
 }  // namespace
 }  // namespace dsdk

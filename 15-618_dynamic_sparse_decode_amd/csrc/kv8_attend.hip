@@ -20,23 +20,6 @@
 namespace dsdk {
 namespace {
 
-// A launch as its kernels see it.
-struct Plan {
-  int group = 1;   // query heads per key head
-  int tiles = 1;   // row tiles of a request and key head, at most
-  int pieces = 1;  // a list is cut into at most this many
-  int piece = 1;   // groups of 64 tokens in a piece
-  int rows = 16;   // rows of a tile held in the workspace
-  float* part = nullptr;    // [batch][heads * tiles][pieces][rows][dim]
-  float2* stats = nullptr;  // [batch][heads * tiles][pieces][rows]: (m, l), l < 0: no token
-};
-
-// The pieces that a span's list is cut into.
-__device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {
-  const int groups = (s.chunks + 3) / 4;
-  return min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
-}
-
 // Grid (key heads * row tiles, batch, pieces); W waves, each of which takes
 // every W-th group of 64 tokens of the piece for all of the tile's 16 rows.
 // Lane (n, g) = (lane % 16, lane / 16).  Logits come out transposed, S^T = K
@@ -349,87 +332,15 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
       const int tok = at / p.group;
       T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
                static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(some ? o[e] / sum : 0.0f);
+      const F32x4 zero = {0, 0, 0, 0};
+      StoreRow4(out, reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0,
+                some ? o / sum : zero);
     } else {
-      const int64_t slot =
-          ((static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces + blockIdx.z) * p.rows + k;
+      const int64_t slot = PartSlot(p, c.heads, r, head, at) + blockIdx.z;
       *reinterpret_cast<F32x4*>(p.part + slot * D + d) = o;
       if (d == 0) p.stats[slot] = make_float2(peak, some ? sum : -1.0f);
     }
   }
-}
-
-// One row's pieces.  Grid (key heads * row tiles, batch, rows of a tile): the
-// pieces' factors first, in LDS, so that the sums' loads wait for nothing; the
-// threads beyond a row's quads take every 256 / quads-th piece, and their sums
-// are added in that order.
-constexpr int kMostPieces = 64;
-template <typename T>
-__global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
-  __shared__ float factor[kMostPieces];
-  __shared__ F32x4 part_sum[256];
-  const Kv8View& c = a.c;
-  const int D = c.dim, quads = D / 4;
-  const int r = blockIdx.y, head = blockIdx.x % c.heads, first = blockIdx.x / c.heads * 16;
-  const int k = blockIdx.z, at = first + k;
-  Span s;
-  if (!FindSpan(a, p.group, r, first, 16, &s)) return;
-  const int pieces = Pieces(p, s);
-  if (pieces == 1 || at >= s.rows) return;
-  const int64_t slot0 =
-      (static_cast<int64_t>(r) * gridDim.x + blockIdx.x) * p.pieces * p.rows + k;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int shares = 256 / quads;  // threads per quad
-  const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
-  if (threadIdx.x < kWave) {
-    float2 st = make_float2(-INFINITY, -1.0f);
-    if (lane < pieces) st = p.stats[slot0 + static_cast<int64_t>(lane) * p.rows];
-    const bool some = !(st.y < 0.0f);
-    float peak = some ? st.x : -INFINITY;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
-    const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
-    float sum = some ? st.y * e : 0.0f;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-    factor[lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
-  }
-  // (loads that do not need the factors are on their way meanwhile)
-  constexpr int kAhead = 4;
-  const float* part = p.part + slot0 * D + d;
-  const int64_t step = static_cast<int64_t>(p.rows) * D;
-  F32x4 x[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    const int z = share + i * shares;
-    x[i] = F32x4{0, 0, 0, 0};
-    if (share < shares && z < pieces) {
-      x[i] = *reinterpret_cast<const F32x4*>(part + z * step);
-    }
-  }
-  __syncthreads();
-  F32x4 o = {0, 0, 0, 0};
-  if (share < shares) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int z = share + i * shares;
-      if (z < pieces) o += x[i] * factor[z];
-    }
-#pragma unroll 4
-    for (int z = share + kAhead * shares; z < pieces; z += shares) {
-      o += *reinterpret_cast<const F32x4*>(part + z * step) * factor[z];
-    }
-  }
-  part_sum[threadIdx.x] = o;
-  __syncthreads();
-  if (share > 0) return;
-  for (int i = 1; i < shares; ++i) o += part_sum[i * quads + threadIdx.x];
-  const int tok = at / p.group;
-  T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
-           static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(o[e]);
 }
 
 // Grid (256 numbers of a row each, batch).
@@ -448,35 +359,20 @@ __global__ __launch_bounds__(256) void Kv8GroupQueriesKernel(const T* q, int64_t
 
 constexpr int kWaves = 4;
 
-// How a batch's lists are cut, by its sizes alone (the lengths themselves are
-// on the device): two workgroups fit a CU (registers), 512 the chip, and lists
-// are cut until there are as many, each piece at least a group of 64 tokens a
-// wave.
+// Two workgroups fit a CU (registers), 512 the chip.
 constexpr int kTarget = 512;
 Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal) {
   Plan p;
   p.group = q_heads / c.heads;
-  const int64_t rows = static_cast<int64_t>(causal ? b.max_tokens : 1) * p.group;
-  p.tiles = static_cast<int>((rows + 15) / 16);
-  p.rows = static_cast<int>(std::min<int64_t>(rows, 16));
-  const int64_t groups = (static_cast<int64_t>(b.max_pages) * c.page + 63) / 64;
-  const int64_t units = static_cast<int64_t>(c.heads) * p.tiles * b.batch;
-  const int64_t want = std::min<int64_t>(
-      {kTarget / std::max<int64_t>(units, 1), (groups + kWaves - 1) / kWaves, kMostPieces});
-  p.pieces = static_cast<int>(std::max<int64_t>(want, 1));
-  p.piece = static_cast<int>(std::max<int64_t>((groups + p.pieces - 1) / p.pieces, 1));
+  p.rows = static_cast<int64_t>(causal ? b.max_tokens : 1) * p.group;
+  p.block = 16;
+  CutLists(&p, c, b, kTarget, kWaves);
   return p;
 }
 
 // Whether a prompt call has rows enough for kv8_prompt.hip.
 bool ManyRows(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
   return static_cast<int64_t>(b.max_tokens) * (q_heads / c.heads) > 64;
-}
-
-size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
-  if (p.pieces == 1) return 0;
-  return static_cast<size_t>(b.batch) * c.heads * p.tiles * p.pieces * p.rows *
-         (sizeof(float) * c.dim + sizeof(float2));
 }
 
 size_t LdsBytes(int dim) {
@@ -496,15 +392,12 @@ void WithKernel(int dim, F&& f) {
 
 template <typename T, int FMT>
 void Launch(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
-  const dim3 grid(a.c.heads * p.tiles, a.b.batch, p.pieces);
+  const dim3 grid(a.c.heads * p.blocks, a.b.batch, p.pieces);
   WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
     kernel<<<grid, kWaves * kWave, LdsBytes(a.c.dim), stream>>>(a, p);
   });
   DSD_HIP_CHECK(hipGetLastError());
-  if (p.pieces > 1) {
-    Kv8MergeKernel<T><<<dim3(grid.x, grid.y, p.rows), 256, 0, stream>>>(a, p);
-    DSD_HIP_CHECK(hipGetLastError());
-  }
+  Merge<T>(a, p, stream);
 }
 
 template <typename T>
@@ -530,8 +423,10 @@ void PreloadType(const Kv8View& c) {
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
   if (b.batch == 0) return 0;
   const size_t one = PlanBytes(c, b, MakePlan(c, b, q_heads, false));
-  if (ManyRows(c, b, q_heads)) return one;
-  return std::max(one, PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
+  if (b.max_tokens == 0) return one;
+  return std::max(one, ManyRows(c, b, q_heads)
+                           ? Kv8PromptWorkspaceBytes(c, b, q_heads)
+                           : PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
 }
 
 void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, const void* q,
@@ -561,16 +456,7 @@ void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream) {
   if (a.b.batch == 0 || (a.causal && a.b.tokens == 0)) return;
   if (a.causal && ManyRows(a.c, a.b, a.q_heads)) return LaunchKv8Prompt(a, stream);
   Plan p = MakePlan(a.c, a.b, a.q_heads, a.causal);
-  if (p.pieces > 1) {
-    if (a.workspace == nullptr || a.workspace_bytes < PlanBytes(a.c, a.b, p)) {
-      p.pieces = 1;
-      p.piece = 1;
-    } else {
-      const size_t slots = static_cast<size_t>(a.b.batch) * a.c.heads * p.tiles * p.pieces * p.rows;
-      p.part = static_cast<float*>(a.workspace);
-      p.stats = reinterpret_cast<float2*>(p.part + slots * a.c.dim);
-    }
-  }
+  PlaceParts(&p, a);
   switch (a.type) {
     case DSD_TYPE_F32: return LaunchType<float>(a, p, stream);
     case DSD_TYPE_BF16: return LaunchType<__bf16>(a, p, stream);

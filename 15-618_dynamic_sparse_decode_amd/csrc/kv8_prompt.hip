@@ -57,14 +57,14 @@ size_t LdsBytes(int dim) {
          2 * 4 * sizeof(ChunkInfo) + sizeof(int) * dim;
 }
 
-// Grid: (key heads * blocks of 128 rows, the last rows first, batch).  Wave w
+// Grid: (key heads * blocks of 128 rows, the last rows first, batch, pieces).  Wave w
 // has rows [32 w, 32 w + 32) of the block, lane (n, h) = (lane % 32, lane / 32)
 // row n.  Logits come out transposed, S^T = K Q^T in two tiles of 32 tokens
 // dealt so that lane (n, h) holds all 16 tokens of chunk 2 t + h for row n, and
 // go into O^T = V^T P^T as they stand.
 template <typename T, int FMT, int NU, int kDim>
-__global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void Kv8PromptKernel(Kv8AttendArgs a,
-                                                                           int group, int blocks) {
+__global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void
+Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>;
   constexpr int KS = 4 * NU, NT = 2 * NU;
   constexpr int kMfma = 0x008, kDsRead = 0x100;  // (the scheduler's groups)
@@ -75,10 +75,14 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int n = lane & 31, h = lane >> 5;
   const int r = blockIdx.y, head = blockIdx.x % c.heads;
-  const int first = (blocks - 1 - static_cast<int>(blockIdx.x) / c.heads) * kRows;
+  const int first = (plan.blocks - 1 - static_cast<int>(blockIdx.x) / c.heads) * kRows;
+  const int group = plan.group;
   Span s;
   if (!FindSpan(a, group, r, first, kRows, &s)) return;
-  const int groups = (s.chunks + 3) / 4;
+  const int pieces = Pieces(plan, s), piece = blockIdx.z;
+  if (piece >= pieces) return;
+  const int begin = piece * plan.piece;
+  const int groups = piece == pieces - 1 ? (s.chunks + 3) / 4 : begin + plan.piece;
 
   _Float16* key_tiles = smem;
   _Float16* value_tiles = smem + 2 * KeyHalves(D);
@@ -185,7 +189,7 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   F16x8 q[KS][NQ];
   float to_logit;  // what a product with codes lacks but the page's scale; >= 0
   for (int i = threadIdx.x; i < D; i += kThreads) nan_from[i] = 0x7fffffff;
-  stage(0);
+  stage(begin);
   {
     const T* qp = static_cast<const T*>(a.q) + (s.q.row0 + token) * a.q_stride +
                   static_cast<int64_t>(q_head) * D;
@@ -227,9 +231,9 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   // (m and mv follow within kSlack)
 
   __syncthreads();
-  fetch(0);
-  put(0, 0);
-  for (int grp = 0; grp < groups; ++grp) {
+  fetch(begin);
+  put(begin, begin & 1);
+  for (int grp = begin; grp < groups; ++grp) {
     const int buf = grp & 1;
     __syncthreads();
     if (grp + 1 < groups) {
@@ -370,20 +374,41 @@ __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void K
   l = Sum2(l);
   if (!there) return;
   const float base = m == -INFINITY ? 0.0f : m;
-  const float to_out = Exp2(mv - base - kPromptBits) / l;
+  float to_out = Exp2(mv - base - kPromptBits);
+  float* part = nullptr;
+  if (pieces > 1) {
+    const int64_t slot = PartSlot(plan, c.heads, r, head, row) + piece;
+    part = plan.part + slot * D;
+    if (h == 0) plan.stats[slot] = make_float2(m, sees > begin * kGroup ? l : -1.0f);
+  } else {
+    to_out /= l;
+  }
   T* out = static_cast<T*>(a.out) + (s.q.row0 + token) * a.out_stride +
            static_cast<int64_t>(q_head) * D;
+  const bool even = reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int d = 32 * t + 2 * i + 4 * h;
       if (kDim > 0 || d < D) {
+        F32x4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float o = acc[t][i + e] * to_out;
-          if (FMT == DSD_KV8_E4M3 && nan_from[d + e] < sees) o = __builtin_nanf("");
-          out[d + e] = static_cast<T>(o);
+        for (int e = 0; e < 4; ++e) o[e] = acc[t][i + e] * to_out;
+        if constexpr (FMT == DSD_KV8_E4M3) {
+          const int4 nan = *reinterpret_cast<const int4*>(nan_from + d);
+          const int least = min(min(nan.x, nan.y), min(nan.z, nan.w));
+          if (least < sees) {
+            if (nan.x < sees) o[0] = __builtin_nanf("");
+            if (nan.y < sees) o[1] = __builtin_nanf("");
+            if (nan.z < sees) o[2] = __builtin_nanf("");
+            if (nan.w < sees) o[3] = __builtin_nanf("");
+          }
+        }
+        if (pieces > 1) {
+          *reinterpret_cast<F32x4*>(part + d) = o;
+        } else {
+          StoreRow4(out + d, even, o);
         }
       }
     }
@@ -400,16 +425,26 @@ void WithKernel(int dim, F&& f) {
   return f(Kv8PromptKernel<T, FMT, 4, 0>);
 }
 
+constexpr int kTarget = 512;  // workgroups the chip runs at once
+Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  Plan p;
+  p.group = q_heads / c.heads;
+  p.rows = static_cast<int64_t>(b.max_tokens) * p.group;
+  p.block = kRows;
+  CutLists(&p, c, b, kTarget, 8);
+  return p;
+}
+
 template <typename T, int FMT>
 void Launch(const Kv8AttendArgs& a, hipStream_t stream) {
-  const int group = a.q_heads / a.c.heads;
-  const int blocks =
-      static_cast<int>((static_cast<int64_t>(a.b.max_tokens) * group + kRows - 1) / kRows);
+  Plan p = MakePlan(a.c, a.b, a.q_heads);
+  PlaceParts(&p, a);
+  const dim3 grid(a.c.heads * p.blocks, a.b.batch, p.pieces);
   WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
-    kernel<<<dim3(a.c.heads * blocks, a.b.batch), kThreads, LdsBytes(a.c.dim), stream>>>(a, group,
-                                                                                      blocks);
+    kernel<<<grid, kThreads, LdsBytes(a.c.dim), stream>>>(a, p);
   });
   DSD_HIP_CHECK(hipGetLastError());
+  Merge<T>(a, p, stream);
 }
 
 template <typename T>
@@ -439,6 +474,10 @@ void PreloadKv8Prompt(const Kv8View& c) {
   PreloadType<float>(c);
   PreloadType<__bf16>(c);
   PreloadType<_Float16>(c);
+}
+
+size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  return PlanBytes(c, b, MakePlan(c, b, q_heads));
 }
 
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream) {
