@@ -270,12 +270,60 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   StoreRow4(out, reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0, o);
 }
 
-// Pieces of at least `least` groups, until there are `target` workgroups.
-inline void CutLists(Plan* p, const Kv8View& c, const dsd_kv8_batch& b, int target, int least) {
-  p->blocks = static_cast<int>((p->rows + p->block - 1) / p->block);
-  const int64_t groups = (static_cast<int64_t>(b.max_pages) * c.page + 63) / 64;
-  const int64_t units = static_cast<int64_t>(c.heads) * p->blocks * b.batch;
-  int64_t want = target / (units > 0 ? units : 1);
+// The same for few pieces and many rows: a wave a row, four a workgroup.  Grid
+// (key heads * rows / 4, batch).
+constexpr int kFewPieces = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void Kv8MergeRowsKernel(Kv8AttendArgs a, Plan p) {
+  const Kv8View& c = a.c;
+  const int D = c.dim, quads = D / 4;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int r = blockIdx.y;
+  const int64_t index = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (index >= c.heads * p.rows) return;
+  const int head = static_cast<int>(index / p.rows);
+  const int at = static_cast<int>(index - head * p.rows), first = at / p.block * p.block;
+  Span s;
+  if (!FindSpan(a, p.group, r, first, p.block, &s)) return;
+  const int pieces = Pieces(p, s);
+  if (pieces == 1 || at >= s.rows) return;
+  const int64_t slot0 = PartSlot(p, c.heads, r, head, at);
+  float2 st = make_float2(-INFINITY, -1.0f);
+  if (lane < pieces) st = p.stats[slot0 + lane];
+  const float* part = p.part + slot0 * D + 4 * lane;
+  F32x4 x[kFewPieces];
+#pragma unroll
+  for (int z = 0; z < kFewPieces; ++z) {
+    x[z] = F32x4{0, 0, 0, 0};
+    if (lane < quads && z < pieces) x[z] = *reinterpret_cast<const F32x4*>(part + z * D);
+  }
+  const bool some = !(st.y < 0.0f);
+  float peak = some ? st.x : -INFINITY;
+#pragma unroll
+  for (int o = 1; o < kFewPieces; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+  const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
+  float sum = some ? st.y * e : 0.0f;
+#pragma unroll
+  for (int o = 1; o < kFewPieces; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+  const float factor = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+  F32x4 o = {0, 0, 0, 0};
+#pragma unroll
+  for (int z = 0; z < kFewPieces; ++z) {
+    const float f = __shfl(factor, z, kWave);
+    if (z < pieces) o += x[z] * f;
+  }
+  if (lane >= quads) return;
+  const int tok = at / p.group, d = 4 * lane;
+  T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
+           static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
+  StoreRow4(out, reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0, o);
+}
+
+// Into `want` pieces, at most kMostPieces, of at least `least` groups.
+inline int64_t ListGroups(const Kv8View& c, const dsd_kv8_batch& b) {
+  return (static_cast<int64_t>(b.max_pages) * c.page + 63) / 64;
+}
+inline void CutLists(Plan* p, int64_t groups, int64_t want, int64_t least) {
   if (want > (groups + least - 1) / least) want = (groups + least - 1) / least;
   if (want > kMostPieces) want = kMostPieces;
   p->pieces = static_cast<int>(want > 1 ? want : 1);
@@ -303,8 +351,13 @@ inline void PlaceParts(Plan* p, const Kv8AttendArgs& a) {
 template <typename T>
 void Merge(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.pieces == 1) return;
-  const dim3 grid(static_cast<unsigned>(a.c.heads * p.rows), a.b.batch);
-  Kv8MergeKernel<T><<<grid, 256, 0, stream>>>(a, p);
+  const int64_t rows = a.c.heads * p.rows;
+  if (p.pieces <= kFewPieces && rows * a.b.batch >= 4096) {
+    const dim3 grid(static_cast<unsigned>((rows + 3) / 4), a.b.batch);
+    Kv8MergeRowsKernel<T><<<grid, 256, 0, stream>>>(a, p);
+  } else {
+    Kv8MergeKernel<T><<<dim3(static_cast<unsigned>(rows), a.b.batch), 256, 0, stream>>>(a, p);
+  }
   DSD_HIP_CHECK(hipGetLastError());
 }
 

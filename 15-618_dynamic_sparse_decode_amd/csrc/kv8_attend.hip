@@ -366,7 +366,9 @@ Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal
   p.group = q_heads / c.heads;
   p.rows = static_cast<int64_t>(causal ? b.max_tokens : 1) * p.group;
   p.block = 16;
-  CutLists(&p, c, b, kTarget, kWaves);
+  p.blocks = static_cast<int>((p.rows + p.block - 1) / p.block);
+  const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
+  CutLists(&p, ListGroups(c, b), kTarget / std::max<int64_t>(units, 1), kWaves);
   return p;
 }
 
@@ -415,6 +417,7 @@ template <typename T>
 void PreloadType(const Kv8View& c) {
   c.format == DSD_KV8_INT8 ? PreloadDim<T, DSD_KV8_INT8>(c) : PreloadDim<T, DSD_KV8_E4M3>(c);
   PreloadKernel(Kv8MergeKernel<T>);
+  PreloadKernel(Kv8MergeRowsKernel<T>);
   PreloadKernel(Kv8GroupQueriesKernel<T>);
 }
 

@@ -431,7 +431,24 @@ Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
   p.group = q_heads / c.heads;
   p.rows = static_cast<int64_t>(b.max_tokens) * p.group;
   p.block = kRows;
-  CutLists(&p, c, b, kTarget, 8);
+  p.blocks = static_cast<int>((p.rows + kRows - 1) / kRows);
+  const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
+  const int64_t most = kTarget / std::max<int64_t>(units, 1);
+  // A group takes a workgroup about 1.5 us; pieces cost the second launch, 5 us,
+  // and a write and a read of their sums at about 3 TB/s.
+  const int64_t groups = ListGroups(c, b);
+  const double rows = static_cast<double>(b.batch) * c.heads * static_cast<double>(p.rows);
+  const double piece_us = rows * c.dim * 8 / 3e6;
+  int64_t best = 1;
+  double best_us = 1.5 * static_cast<double>(groups);
+  for (int64_t n = 2; n <= std::min<int64_t>(most, kMostPieces); ++n) {
+    const double us = 1.5 * static_cast<double>((groups + n - 1) / n) + 5.0 + piece_us * n;
+    if (us < best_us) {
+      best_us = us;
+      best = n;
+    }
+  }
+  CutLists(&p, groups, best, 1);
   return p;
 }
 
