@@ -3186,6 +3186,12 @@ void RequireHeads(const dsd_kv8* cache, int q_heads) {
   Require(q_heads <= 65536, "at most 65536 query heads");
 }
 
+// A launch counts a request's query rows over all heads.
+void RequireQueryRows(const dsd_kv8_batch* b, int q_heads) {
+  Require(static_cast<int64_t>(b->max_tokens) * std::max(1, q_heads) <= 0x7fffffff,
+          "max_tokens * num_q_heads must fit 31 bits");
+}
+
 int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, bool causal, int type, int num_q_heads,
               const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
               void* workspace, size_t workspace_bytes, unsigned long long* d_fail, void* stream) {
@@ -3194,6 +3200,7 @@ int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, bool causal, int type,
     const size_t size = TypeSize(type);
     RequireHeads(cache, num_q_heads);
     Require(num_q_heads > 0, "num_q_heads must be positive");
+    if (causal) RequireQueryRows(batch, num_q_heads);
     if (batch->batch == 0 || (causal && batch->tokens == 0)) return;
     RequireRows(cache, q, q_stride, num_q_heads, size);
     RequireRows(cache, out, out_stride, num_q_heads, size);
@@ -3425,6 +3432,7 @@ int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, in
     Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0,
             "sizes must be non-negative");
     RequireHeads(cache, num_q_heads);
+    RequireQueryRows(batch, num_q_heads);
     *bytes = num_q_heads > 0 ? dsdk::Kv8WorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
   });
 }
@@ -3500,14 +3508,8 @@ int dsd_kv8_sparse_create(dsd_kv8* cache, int num_q_heads, int top_k, int max_ba
     if (status != DSD_OK) throw dsdk::HipError(g_last_error);
     dsd_kv8_batch b = {};
     b.batch = max_batch;
-    b.max_pages = std::max(1, top_k);
-    // (fewer requests may be cut into more pieces: the most any batch takes)
-    size_t most = 0;
-    for (int n = 1; n <= max_batch; ++n) {
-      b.batch = n;
-      most = std::max(most, dsdk::Kv8WorkspaceBytes(c, b, num_q_heads));
-    }
-    if (most > 0) step->workspace.Reserve(most);
+    const size_t bytes = dsdk::Kv8WorkspaceBytes(c, b, num_q_heads);
+    if (bytes > 0) step->workspace.Reserve(bytes);
     *out = step.release();
   });
 }

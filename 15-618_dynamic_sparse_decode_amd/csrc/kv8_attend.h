@@ -337,6 +337,12 @@ inline size_t PlanSlots(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p)
 inline size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
   return p.pieces == 1 ? 0 : PlanSlots(c, b, p) * (sizeof(float) * c.dim + sizeof(float2));
 }
+// What any batch needs at most whose rows per request are no more: lists are cut
+// into as many pieces as keep the workgroups within `target`.
+inline size_t MostPartBytes(const Kv8View& c, const Plan& p, int target) {
+  const size_t rows = static_cast<size_t>(p.rows < p.block ? p.rows : p.block);
+  return target * rows * (sizeof(float) * c.dim + sizeof(float2));
+}
 // The pieces' places in the call's workspace; without one lists stay whole.
 inline void PlaceParts(Plan* p, const Kv8AttendArgs& a) {
   if (p->pieces > 1 && (a.workspace == nullptr || a.workspace_bytes < PlanBytes(a.c, a.b, *p))) {

@@ -410,7 +410,12 @@ void LaunchType(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
 
 template <typename T, int FMT>
 void PreloadDim(const Kv8View& c) {
-  WithKernel<T, FMT>(c.dim, [](auto kernel) { PreloadKernel(kernel); });
+  WithKernel<T, FMT>(c.dim, [&](auto kernel) {
+    PreloadKernel(kernel);
+    DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(LdsBytes(c.dim))));
+  });
 }
 
 template <typename T>
@@ -425,11 +430,14 @@ void PreloadType(const Kv8View& c) {
 
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
   if (b.batch == 0) return 0;
-  const size_t one = PlanBytes(c, b, MakePlan(c, b, q_heads, false));
-  if (b.max_tokens == 0) return one;
-  return std::max(one, ManyRows(c, b, q_heads)
-                           ? Kv8PromptWorkspaceBytes(c, b, q_heads)
-                           : PlanBytes(c, b, MakePlan(c, b, q_heads, true)));
+  dsd_kv8_batch one = b;
+  one.max_tokens = 1;
+  size_t bytes = MostPartBytes(c, MakePlan(c, one, q_heads, false), kTarget);
+  if (b.max_tokens > 1) {
+    bytes = std::max(bytes, MostPartBytes(c, MakePlan(c, b, q_heads, true), kTarget));
+    if (ManyRows(c, b, q_heads)) bytes = std::max(bytes, Kv8PromptWorkspaceBytes(c, b, q_heads));
+  }
+  return bytes;
 }
 
 void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, const void* q,

@@ -494,7 +494,7 @@ void PreloadKv8Prompt(const Kv8View& c) {
 }
 
 size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
-  return PlanBytes(c, b, MakePlan(c, b, q_heads));
+  return MostPartBytes(c, MakePlan(c, b, q_heads), kTarget);
 }
 
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream) {

@@ -739,8 +739,9 @@ int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
  * Logits, sums and outputs before their one rounding are float32; out has q's
  * type.  Row r of q and out is request r.
  * workspace (16-byte aligned): dsd_kv8_workspace_bytes of device memory lets
- * long lists spread over workgroups; calls that may overlap (streams, graphs)
- * need one each.  NULL or smaller: the lists are not spread. */
+ * long lists spread over workgroups; it needs no initial contents, keeps none
+ * between calls, and calls that may overlap (streams, graphs) need one each.
+ * NULL or less than the batch needs: the lists are not spread. */
 int dsd_kv8_attend(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
                    int num_q_heads, const void* q, int64_t q_stride, void* out,
                    int64_t out_stride, float scale, void* workspace,
@@ -756,7 +757,7 @@ int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
                           void* out, int64_t out_stride, float scale,
                           void* workspace, size_t workspace_bytes,
                           unsigned long long* d_fail, void* stream);
-/* Workspace of dsd_kv8_attend and dsd_kv8_attend_prompt for batches of at most
+/* Workspace of dsd_kv8_attend and dsd_kv8_attend_prompt for any batch of at most
  * these sizes (the pointers are not read). */
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                             int num_q_heads, size_t* bytes);

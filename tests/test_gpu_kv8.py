@@ -523,6 +523,63 @@ def test_attend_scales_that_differ_widely(gpu):
             check_attention(pair, batch, kind, q, out, scale=1.5)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_attend_unaligned_rows_and_negative_scale(gpu, kind):
+    """Rows that start on any element, at any stride; a negative scale."""
+    import torch
+    rng = np.random.default_rng(17)
+    pair = Pair(gpu, 2, 64, 16, 16)
+    pair.fill(11)
+    for causal, past, new in ((False, None, None), (True, [30, 7, 0], [3, 40, 1])):
+        tokens = 3 if not causal else sum(new)
+        lists = [[0, 1, 2], [3, 4, 5, 6], [7]]
+        batch = Batch(gpu, lists, past, new)
+        for heads in (4, 18):
+            width = heads * 64 + 7
+            flat = rows(rng, kind, 1, 1, tokens * width + 1).view(-1)[1:].view(tokens, width)
+            q = flat[:, 3:3 + heads * 64].unflatten(1, (heads, 64))
+            wide = torch.full((tokens, width + 2), 9.0, device="cuda", dtype=q.dtype)
+            out = wide[:, 1:1 + heads * 64].unflatten(1, (heads, 64))
+            attend(pair, batch, kind, q, out, causal=causal, scale=-0.21)
+            check_attention(pair, batch, kind, q, out, causal=causal, scale=-0.21)
+            assert bool((wide[:, 0] == 9.0).all()) and bool((wide[:, 1 + heads * 64:] == 9.0).all())
+
+
+@pytest.mark.parametrize("kind,fmt", [("bf16", kv8.E4M3), ("f32", kv8.INT8)])
+@pytest.mark.parametrize("heads,kv,dim,page,past,new", [
+    (8, 1, 128, 16, [9000], [40]),       # one block of rows, its list in pieces
+    (8, 2, 128, 64, [5000, 40], [70, 130]),
+    (4, 1, 64, 16, [12000], [33]),
+    (8, 1, 256, 128, [6000], [20]),
+])
+def test_prompt_chunk_behind_a_long_context(gpu, heads, kv, dim, page, past, new, kind, fmt):
+    import torch
+    rng = np.random.default_rng(dim + past[0])
+    lengths = [p + n for p, n in zip(past, new)]
+    capacity = sum(-(-n // page) for n in lengths)
+    pair = Pair(gpu, kv, dim, page, capacity, fmt)
+    pair.fill(dim)
+    lists = lists_for(rng, lengths, page, capacity)
+    q = rows(rng, kind, sum(new), heads, dim)
+    batch = Batch(gpu, lists, past, new)
+    assert pair.cache.workspace_bytes(batch.batch, heads) > 0
+    for workspace in (True, False):
+        out = torch.full_like(q, 9.0)
+        attend(pair, batch, kind, q, out, causal=True, workspace=workspace)
+        check_attention(pair, batch, kind, q, out, causal=True)
+    # a NaN value in the middle of a piece, seen by the last rows only
+    if fmt == kv8.E4M3:
+        token = past[0] + new[0] - 5
+        page_id = lists[0][token // page]
+        want = torch.full_like(q, 9.0)
+        attend(pair, batch, kind, q, want, causal=True)
+        pair.values[page_id, 0, token % page // 16, 3, token % 16] = 0x7f
+        attend(pair, batch, kind, q, out, causal=True)
+        G = heads // kv
+        assert bool(out[new[0] - 5:new[0], :G, 3].isnan().all())
+        assert torch.equal(out[:new[0] - 5], want[:new[0] - 5])
+
+
 def test_attend_nonfinite(gpu):
     """Infinite and NaN queries give what the formula gives; other rows of the
     tile are untouched by them."""
@@ -670,6 +727,9 @@ def test_refusals(gpu):
                     **{n: t.data_ptr() for n, t in batch.keep.items()})
         with pytest.raises(gpu.InvalidArgument, match=what):
             pair.cache.attend(gpu.Kv8Batch(**{**good, **bad}), **base)
+    with pytest.raises(gpu.InvalidArgument, match="31 bits"):
+        huge = dict(good, tokens=1 << 30, max_tokens=1 << 30)
+        pair.cache.attend_prompt(gpu.Kv8Batch(**huge), **base)
     with pytest.raises(gpu.InvalidArgument, match="token_offsets"):
         good = dict(good, token_offsets=0)
         pair.cache.attend_prompt(gpu.Kv8Batch(**good), **base)
