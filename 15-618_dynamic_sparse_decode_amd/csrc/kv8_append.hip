@@ -192,29 +192,29 @@ __device__ __forceinline__ Unit UnitOf(int u, const Kv8Rotation& rot) {
   return x;
 }
 
-// The sines of 16 tokens in LDS: (cos, sin) of token o's pair 8 u + i at
-// [o][i][u], so that the lanes of a row, one unit each, read next to each
-// other.
+// The sines in LDS: (cos, sin) of token o's pair 8 u + i at [o][i ^ o % 4][u], so
+// that the lanes of a row, one unit each, read next to each other, and the rows
+// beside them other banks.
 __device__ __forceinline__ int SineAt(int o, int i, int u, int turning) {
-  return (o * 8 + i) * turning + u;
+  return (o * 8 + (i ^ (o & 3))) * turning + u;
 }
 
 // Pair i of a unit whose elements are x[at..at + 8) at a, x[at + 8..at + 16) at
-// b: its place from `at` on and its numbers turned.  cs: the unit's first pair,
-// the others `step` apart.
+// b: its place from `at` on and its numbers turned.  cs: token o's pairs of the
+// unit, `step` apart.
 struct Turned {
   int i0, i1;
   double y0, y1;
 };
 template <typename X>
 __device__ __forceinline__ Turned TurnPair(const X& x, int at, int i, const double2* cs, int step,
-                                           bool interleaved) {
+                                           int o, bool interleaved) {
   Turned t;
   t.i0 = interleaved ? 2 * i : i;
   t.i1 = interleaved ? 2 * i + 1 : 8 + i;
   const double p = static_cast<double>(x[at + t.i0]);
   const double q = static_cast<double>(x[at + t.i1]);
-  const double2 w = cs[i * step];
+  const double2 w = cs[(i ^ (o & 3)) * step];
   t.y0 = fma(p, w.x, -(q * w.y));
   t.y1 = fma(q, w.x, p * w.y);
   return t;
@@ -362,10 +362,10 @@ __device__ __forceinline__ unsigned TurnKeys(const Kv8AppendArgs& a, const Part&
     const int o = i / units, u = i - o * units;
     if (o >= p.lo && o < p.hi) {
       if (u < turning) {
-        const double2* at = cs + SineAt(o, 0, u, turning);
+        const double2* at = cs + (o * 8 * turning + u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const Turned z = TurnPair(x.x, 16 * j, e, at, turning, kInterleaved);
+          const Turned z = TurnPair(x.x, 16 * j, e, at, turning, o, kInterleaved);
           if constexpr (FMT == DSD_KV8_E4M3) {
             y[16 * j + z.i0] = ToOdd(z.y0);
             y[16 * j + z.i1] = ToOdd(z.y1);
@@ -455,7 +455,7 @@ __device__ __forceinline__ void StoreKeys(const Kv8AppendArgs& a, uint8_t* block
           for (int k = 0; k < 4; ++k) {
             Turned t;
             if (u < turning) {
-              t = TurnPair(x.x, 16 * j, e + k, cs + SineAt(o, 0, u, turning), turning,
+              t = TurnPair(x.x, 16 * j, e + k, cs + (o * 8 * turning + u), turning, o,
                            kInterleaved);
             } else {
               t.y0 = static_cast<double>(x.x[16 * j + (kInterleaved ? 2 * (e + k) : e + k)]);
@@ -616,11 +616,11 @@ __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const 
     x.Load8(8, from + w.b, vec);
     // two pairs at a time: whole words of results
     if (u < turning) {
-      const double2* at_cs = cs + SineAt(o, 0, u, turning);
+      const double2* at_cs = cs + (o * 8 * turning + u);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const Turned y = TurnPair(x, 0, e, at_cs, turning, kInterleaved);
-        const Turned z = TurnPair(x, 0, e + 1, at_cs, turning, kInterleaved);
+        const Turned y = TurnPair(x, 0, e, at_cs, turning, o, kInterleaved);
+        const Turned z = TurnPair(x, 0, e + 1, at_cs, turning, o, kInterleaved);
         if constexpr (kInterleaved) {
           x.Set2(y.i0, static_cast<float>(y.y0), static_cast<float>(y.y1));
           x.Set2(z.i0, static_cast<float>(z.y0), static_cast<float>(z.y1));
@@ -638,8 +638,7 @@ __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const 
 
 // A malformed request may have no workgroup that looks at it: the last one does.
 __device__ __forceinline__ void CheckRequests(const Kv8AppendArgs& a) {
-  if (a.b.max_tokens > 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 &&
-      threadIdx.x < kWave) {
+  if (a.b.max_tokens > 1 && blockIdx.x == gridDim.x - 1 && threadIdx.x < kWave) {
     for (int r = threadIdx.x; r < a.b.batch; r += kWave) {
       Kv8Request q;
       if (!Kv8ReadTokens(a.b, r, a.c.page, &q)) ReportFailure(a.fail, kFailShape);
@@ -720,8 +719,8 @@ struct Lane {
   }
 };
 
-// Pages of at most four chunks.  Grid (pages' workgroups, groups of `per` key
-// heads): 2 * per * chunks waves, wave w the keys (w even) or values of head
+// Pages of at most four chunks.  A workgroup for each page and group of `per` key
+// heads, a page's one after the other (their rows lie side by side): 2 * per * chunks waves, wave w the keys (w even) or values of head
 // w / 2 % per of the group, chunk w / (2 * per); then all of them the group's
 // queries.  Every number is read once and stays in its lane until its code is
 // known.  LDS: the sines of a page's tokens, a 16 x dim tile and the sums of
@@ -732,18 +731,19 @@ __global__ __launch_bounds__(kMostWaves* kWave) void Kv8AppendKernel(Kv8AppendAr
                                                                      bool vec) {
   extern __shared__ __align__(16) unsigned char smem[];
   CheckRequests(a);
+  const int groups = (a.c.heads + per - 1) / per;
   Task t;
-  if (!FindTask(a, blockIdx.x, &t)) return;
+  if (!FindTask(a, blockIdx.x / groups, &t)) return;
   using L = Lane<T, FMT, NU, kInterleaved>;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int heads = a.c.heads, D = a.c.dim, chunks = a.c.chunks, group = a.q_heads / heads;
-  const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
+  const int h0 = blockIdx.x % groups * per, h1 = min(h0 + per, heads);
   const bool keys = (wave & 1) == 0;
   const int within = wave / 2 % per, chunk = wave / (2 * per);
   const int h = h0 + within;
   const bool mine = h < h1;
   double2* cs = reinterpret_cast<double2*>(smem);
-  const double2* my_cs = cs + SineAt(16 * chunk, 0, 0, a.rot.pairs / 8);
+  const double2* my_cs = cs + 128 * chunk * (a.rot.pairs / 8);
   uint8_t* tiles = smem + sizeof(double2) * 16 * chunks * a.rot.pairs;
   uint8_t* tile = tiles + wave / 2 * 16 * D;
   float* all_sums = reinterpret_cast<float*>(tiles + per * chunks * 16 * D);
@@ -822,15 +822,16 @@ __global__ __launch_bounds__(kMostWaves* kWave) void Kv8AppendPageKernel(Kv8Appe
                                                                          bool vec) {
   extern __shared__ __align__(16) unsigned char smem[];
   CheckRequests(a);
+  const int groups = (a.c.heads + per - 1) / per;
   Task t;
-  if (!FindTask(a, blockIdx.x, &t)) return;
+  if (!FindTask(a, blockIdx.x / groups, &t)) return;
   if (!InPool(t.page, a.c.capacity)) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
     return;
   }
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int heads = a.c.heads, D = a.c.dim, group = a.q_heads / heads;
-  const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
+  const int h0 = blockIdx.x % groups * per, h1 = min(h0 + per, heads);
   const int h = h0 + wave / 2;
   const bool mine = h < h1, keys = (wave & 1) == 0;
   double2* cs = reinterpret_cast<double2*>(smem);
@@ -919,7 +920,7 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
   const int64_t units = a.b.max_tokens > 1
                             ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
                             : a.b.batch;
-  const dim3 grid(static_cast<unsigned>(units), (a.c.heads + per - 1) / per);
+  const unsigned grid = static_cast<unsigned>(units * ((a.c.heads + per - 1) / per));
   WithKernel<T>(a.c, a.rot.interleaved != 0, [&](auto kernel) {
     kernel<<<grid, 2 * per * Across(a.c) * kWave, LdsBytes(a.c, a.rot.pairs), stream>>>(
         a, per, vec);

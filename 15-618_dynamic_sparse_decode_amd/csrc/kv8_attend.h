@@ -358,7 +358,7 @@ template <typename T>
 void Merge(const Kv8AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.pieces == 1) return;
   const int64_t rows = a.c.heads * p.rows;
-  if (p.pieces <= kFewPieces && rows * a.b.batch >= 4096) {
+  if (p.pieces <= kFewPieces && rows * a.b.batch >= 1024) {
     const dim3 grid(static_cast<unsigned>((rows + 3) / 4), a.b.batch);
     Kv8MergeRowsKernel<T><<<grid, 256, 0, stream>>>(a, p);
   } else {
