@@ -1036,6 +1036,8 @@ class Kv8SparseStep:
     def run(self, batch: int, total_candidates: int, max_candidates: int, dtype: int, q: int,
             q_stride: int, cand_offsets: int, cand_ids: int, out: int, out_stride: int,
             selected: int = 0, selected_counts: int = 0, stream: int = 0) -> None:
+        if not self.cache.handle:
+            raise InvalidArgument(1, "the step's cache is closed")
         status = self._lib.dsd_kv8_sparse_run(
             self.handle, batch, total_candidates, max_candidates, dtype, q, q_stride, cand_offsets,
             cand_ids, out, out_stride, selected or None, selected_counts or None, stream)

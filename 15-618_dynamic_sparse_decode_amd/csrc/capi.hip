@@ -3182,8 +3182,8 @@ void RequireRows(const dsd_kv8* cache, const void* p, int64_t stride, int heads,
 void RequireHeads(const dsd_kv8* cache, int q_heads) {
   Require(q_heads >= 0 && q_heads % cache->view.heads == 0,
           "num_q_heads must be a multiple of num_kv_heads");
-  // (a launch's first dimension counts its heads)
-  Require(q_heads <= 65536, "at most 65536 query heads");
+  // (kernels divide by a head count's 32-bit reciprocal, exact up to here)
+  Require(q_heads <= 8192, "at most 8192 query heads");
 }
 
 // A launch counts a request's query rows over all heads.
@@ -3362,7 +3362,8 @@ int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved, const 
     }
     DSD_HIP_CHECK(hipDeviceSynchronize());
     if (pairs > 0) {
-      cache->table.Reserve(table.size());
+      // (of the largest size at once: graphs captured before keep a valid address)
+      cache->table.Reserve(static_cast<size_t>(cache->view.dim / 2) * 4 * 256);
       DSD_HIP_CHECK(hipMemcpy(cache->table.ptr, table.data(), sizeof(double2) * table.size(),
                               hipMemcpyHostToDevice));
     }
@@ -3449,11 +3450,14 @@ struct dsd_kv8_sparse {
   dsd_sparse_ctx* ctx = nullptr;
   DeviceBuffer<unsigned char> workspace;
   bool used = false;
-  hipStream_t last = nullptr;  // of the last step (the default one: null)
+  hipStream_t last = nullptr;  // of the last step outside a graph (the default one: null)
 
   // Steps share the scratch: one on another stream follows the last one.
   void OrderOn(hipStream_t s) {
     if (used && last != s) {
+      // (an event recorded on it now would draw this stream into the graph)
+      Require(last == nullptr || !StreamCapturing(last),
+              "the last step's stream is being captured into a graph");
       DSD_HIP_CHECK(hipEventRecord(ctx->ev_switch, last));
       DSD_HIP_CHECK(hipStreamWaitEvent(s, ctx->ev_switch, 0));
     }
@@ -3554,7 +3558,6 @@ int dsd_kv8_sparse_run(dsd_kv8_sparse* step, int batch, int total_candidates, in
     if (d_selected_counts != nullptr) L.counts = d_selected_counts;
     if (s != nullptr && StreamCapturing(s)) {
       L.epoch_src = ctx->d_epoch.ptr;  // (the select's helpers stay out of a graph)
-      step->used = false;
     } else {
       step->OrderOn(s);
     }

@@ -8,9 +8,10 @@
 // 256 a pair, in 64 bits (32-bit angles are off by whole hundredths of a radian
 // at a million positions); the turns are 64-bit too: a key's code then falls on
 // the right side of every rounding border.  (Forming sines in place cost 25
-// registers, a quarter of the waves, and three times the instructions.)  The codes of a page share one scale s >= largest / M (M =
-// 448 or 127), so a token that needs a larger one takes the page's earlier
-// codes with it: code <- nearest(code * old / s).
+// registers, a quarter of the waves, and three times the instructions.)  The
+// codes of a page share one scale s >= largest / M (M = 448 or 127), so a token
+// that needs a larger one takes the page's earlier codes with it: code <-
+// nearest(code * old / s).
 //
 // Bound by HBM: queries, keys and values are read once, rotated queries and
 // codes written once.  A workgroup takes one page's new tokens of some key
@@ -20,6 +21,7 @@
 #include "kv8_device.h"
 
 #include <algorithm>
+#include <stdexcept>
 
 namespace dsdk {
 namespace {
@@ -720,7 +722,9 @@ struct Lane {
 };
 
 // Pages of at most four chunks.  A workgroup for each page and group of `per` key
-// heads, a page's one after the other (their rows lie side by side): 2 * per * chunks waves, wave w the keys (w even) or values of head
+// heads, a page's one after the other (their rows lie side by side; head groups in
+// the grid's second dimension took 331 us in place of 321 on the longest case
+// below): 2 * per * chunks waves, wave w the keys (w even) or values of head
 // w / 2 % per of the group, chunk w / (2 * per); then all of them the group's
 // queries.  Every number is read once and stays in its lane until its code is
 // known.  LDS: the sines of a page's tokens, a 16 x dim tile and the sums of
@@ -920,10 +924,15 @@ void LaunchType(const Kv8AppendArgs& a, hipStream_t stream) {
   const int64_t units = a.b.max_tokens > 1
                             ? a.b.tokens / a.c.page + 2 * static_cast<int64_t>(a.b.batch)
                             : a.b.batch;
-  const unsigned grid = static_cast<unsigned>(units * ((a.c.heads + per - 1) / per));
+  const int64_t workgroups = units * ((a.c.heads + per - 1) / per);
+  const int threads = 2 * per * Across(a.c) * kWave;
+  // (a launch counts its threads in 32 bits)
+  if (workgroups > 0xffffffffll / threads) {
+    throw std::invalid_argument("too many tokens and heads for one call");
+  }
+  const unsigned grid = static_cast<unsigned>(workgroups);
   WithKernel<T>(a.c, a.rot.interleaved != 0, [&](auto kernel) {
-    kernel<<<grid, 2 * per * Across(a.c) * kWave, LdsBytes(a.c, a.rot.pairs), stream>>>(
-        a, per, vec);
+    kernel<<<grid, threads, LdsBytes(a.c, a.rot.pairs), stream>>>(a, per, vec);
   });
   DSD_HIP_CHECK(hipGetLastError());
 }

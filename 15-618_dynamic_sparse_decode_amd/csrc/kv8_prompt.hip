@@ -95,11 +95,19 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
   const int page_bytes = c.page * D;
   int slot0 = 0, slots = 0, stage_end = 0;
+  // Whether a page so far was outside the cache: it holds no token, in the middle
+  // of a list, and what it stands for (page 0) is masked.
+  bool bad = false;
   auto stage = [&](int g0) {
     stage_end = min(groups, g0 + per_stage);
     slot0 = 4 * g0 / c.chunks;
     slots = (min(4 * stage_end, s.chunks) - 1) / c.chunks + 1 - slot0;
-    for (int i = threadIdx.x; i < slots; i += kThreads) info[i] = ReadPage(a, s, head, slot0 + i);
+    bool mine = false;
+    for (int i = threadIdx.x; i < slots; i += kThreads) {
+      info[i] = ReadPage(a, s, head, slot0 + i);
+      mine = mine || info[i].tokens == 0;
+    }
+    return mine;
   };
   // Chunk i of the list: its page and its part of it; tokens from its first on.
   auto place = [&](int i, int* sub) {
@@ -138,7 +146,7 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
       chunk_info[4 * buf + threadIdx.x] = {k.key_scale, k.value_scale,
                                            __builtin_amdgcn_logf(k.value_scale), k.tokens};
     }
-    const bool tail = (grp + 1) * kGroup > s.q.past + s.q.n;
+    const bool tail = bad || (grp + 1) * kGroup > s.q.past + s.q.n;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int i = threadIdx.x + kThreads * j;
@@ -152,7 +160,11 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
         unsigned w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
         if (tail) {
           // Codes behind the request's tokens may be anything, and 0 * NaN is not 0.
-          const int tokens = s.q.past + s.q.n - grp * kGroup - 16 * k;
+          int tokens = s.q.past + s.q.n - grp * kGroup - 16 * k;
+          if (bad) {
+            int sub;
+            tokens = min(tokens, place(4 * grp + k, &sub).tokens);
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int have = min(max(tokens - 4 * e, 0), 4);
@@ -189,7 +201,7 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   F16x8 q[KS][NQ];
   float to_logit;  // what a product with codes lacks but the page's scale; >= 0
   for (int i = threadIdx.x; i < D; i += kThreads) nan_from[i] = 0x7fffffff;
-  stage(begin);
+  const bool bad_here = stage(begin);
   {
     const T* qp = static_cast<const T*>(a.q) + (s.q.row0 + token) * a.q_stride +
                   static_cast<int64_t>(q_head) * D;
@@ -230,7 +242,7 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   float mv = -INFINITY;  // of s + log2(value scale): acc is relative to it
   // (m and mv follow within kSlack)
 
-  __syncthreads();
+  bad = __syncthreads_or(bad_here) != 0;
   fetch(begin);
   put(begin, begin & 1);
   for (int grp = begin; grp < groups; ++grp) {
@@ -238,8 +250,8 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
     __syncthreads();
     if (grp + 1 < groups) {
       if (grp + 1 == stage_end) {
-        stage(grp + 1);
-        __syncthreads();
+        const bool more_bad = stage(grp + 1);
+        bad = __syncthreads_or(bad || more_bad) != 0;
       }
       fetch(grp + 1);
     }
@@ -282,11 +294,12 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
         ci[t] = chunk_info[4 * buf + 2 * t + h];
         f[t] = fmaxf(to_logit * ci[t].key_scale, kKv8Tiny);
       }
-      const bool whole = (grp + 1) * kGroup <= all_see;
+      const bool whole = (grp + 1) * kGroup <= all_see && !bad;
       if (!whole) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int count = sees - (grp * kGroup + 32 * t + 16 * h);
+          int count = sees - (grp * kGroup + 32 * t + 16 * h);
+          if (bad) count = min(count, ci[t].tokens);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             if (i >= count) x[t][i] = -INFINITY;
@@ -375,13 +388,14 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   if (!there) return;
   const float base = m == -INFINITY ? 0.0f : m;
   float to_out = Exp2(mv - base - kPromptBits);
+  const bool none = (bad && m == -INFINITY) || sees <= begin * kGroup;  // no token here
   float* part = nullptr;
   if (pieces > 1) {
     const int64_t slot = PartSlot(plan, c.heads, r, head, row) + piece;
     part = plan.part + slot * D;
-    if (h == 0) plan.stats[slot] = make_float2(m, sees > begin * kGroup ? l : -1.0f);
+    if (h == 0) plan.stats[slot] = make_float2(m, none ? -1.0f : l);
   } else {
-    to_out /= l;
+    to_out /= none ? 1.0f : l;
   }
   T* out = static_cast<T*>(a.out) + (s.q.row0 + token) * a.out_stride +
            static_cast<int64_t>(q_head) * D;

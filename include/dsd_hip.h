@@ -683,7 +683,8 @@ int dsd_kv8_device_arrays(const dsd_kv8* cache, dsd_kv8_arrays* out);
  * after creation) to head_dim; interleaved 0: pair i is dims (i, i +
  * rotary_dim / 2), 1: (2 i, 2 i + 1).  inv_freq: rotary_dim / 2 host doubles.
  * Angles and products are 64-bit, so positions of millions keep their
- * angles.  Synchronous; not while a call on the cache runs. */
+ * angles.  Synchronous; not while a call on the cache runs.  A captured append
+ * keeps the rotation's form of its capture: capture it again after a change. */
 int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved,
                          const double* inv_freq, double magnitude);
 
@@ -734,7 +735,7 @@ int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
 
 /* Attention of one query token a request over every token of its list's pages
  * (token_counts each): out = softmax(scale * q K^T) V.  num_q_heads is a
- * multiple of num_kv_heads; query head h reads key head h / (num_q_heads /
+ * multiple of num_kv_heads up to 8192; query head h reads key head h / (num_q_heads /
  * num_kv_heads).  scale 0: 1 / sqrt(D).  A request without tokens gets zeros.
  * Logits, sums and outputs before their one rounding are float32; out has q's
  * type.  Row r of q and out is request r.
@@ -772,8 +773,9 @@ int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
  * The handle holds the scratch for max_batch requests of max_total_candidates
  * pages in all; the cache must outlive it.  Steps on one handle share the
  * scratch: a step on a stream other than the last step's first waits for that
- * stream, which must still be valid.  On a capturing stream the step is
- * recorded into the graph, and the caller orders replays and other steps. */
+ * stream, which must still be valid and not be capturing (refused).  On a
+ * capturing stream the step is recorded into the graph, and the caller orders
+ * the graph's replays against other steps. */
 typedef struct dsd_kv8_sparse dsd_kv8_sparse;
 int dsd_kv8_sparse_create(dsd_kv8* cache, int num_q_heads, int top_k,
                           int max_batch, int max_total_candidates,

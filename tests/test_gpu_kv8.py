@@ -964,3 +964,153 @@ def test_sparse_step_refuses(gpu):
             step.status()
         step.status()
         assert not bool(q.any())
+
+
+# ---- calls at the edges ---------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,fmt", [("bf16", kv8.E4M3), ("f32", kv8.INT8)])
+@pytest.mark.parametrize("dim,page,past,new,spread", [
+    (128, 16, 30, 150, False),
+    (96, 48, 0, 200, False),
+    (64, 16, 9000, 70, True),  # the list in pieces, and beyond the pages staged at once
+])
+def test_prompt_skips_pages_outside_the_cache(gpu, dim, page, past, new, spread, kind, fmt):
+    """A page id outside the cache holds no token, whatever page 0 holds."""
+    import torch
+    rng = np.random.default_rng(dim + new)
+    kv, G = 2, 2
+    need = -(-(past + new) // page)
+    pair = Pair(gpu, kv, dim, page, need, fmt)
+    pair.fill(dim)
+    if fmt == kv8.E4M3:
+        pair.values[0] = 0x7f  # (page 0 is in no list)
+    ids = np.roll(np.arange(need), -1)  # 1, 2, .., 0
+    gone = sorted({0, need // 2, need - 1})
+    for where in ([need - 1], [0, need - 1], gone):
+        lists = ids.copy()
+        lists[where] = -3
+        q = rows(rng, kind, new, kv * G, dim)
+        out = torch.full_like(q, 9.0)
+        fail = torch.zeros(1, dtype=torch.int64, device="cuda")
+        batch = Batch(gpu, [lists.tolist()], [past], [new])
+        attend(pair, batch, kind, q, out, causal=True, workspace=spread, fail=fail)
+        assert int(fail) & 0xffffffff == 3
+        held = np.repeat(~np.isin(np.arange(need), where), page)[:past + new]
+        keys, values, most = pair.model.rows(np.maximum(lists, 0), past + new)
+        sees = np.repeat(np.cumsum(held)[past:past + new], G)
+        for h in range(kv):
+            mine = as64(q)[:, h * G:(h + 1) * G].reshape(new * G, dim)
+            have = as64(out)[:, h * G:(h + 1) * G].reshape(new * G, dim)
+            some = sees > 0
+            want, weighted, size, peak = kv8.attend(
+                mine[some], keys[h][held], values[h][held], 1 / np.sqrt(dim), sees[some],
+                most[h][held])
+            may = kv8.allowed(want, weighted, size, peak, dim, int(held.sum()), kind)
+            assert (np.abs(have[some] - want) <= may).all(), (where, h)
+            assert not have[~some].any()
+
+
+def test_head_counts_and_closed_caches_are_refused(gpu):
+    import torch
+    pair = Pair(gpu, 1, 16, 16, 2, rubbish=False)
+    lists = Batch(gpu, [[0]], [0], [1])
+    x = torch.zeros(1, 8200, 16, device="cuda")
+    with pytest.raises(gpu.InvalidArgument, match="8192"):
+        append(pair, lists, "f32", x, x[:, :1], x[:, :1], x)
+    with pytest.raises(gpu.InvalidArgument, match="8192"):
+        attend(pair, lists, "f32", x, x, workspace=False)
+    with pytest.raises(gpu.InvalidArgument, match="8192"):
+        gpu.Kv8SparseStep(pair.cache, 8193, 1, 1, 1)
+    wide = torch.randn(1, 8192, 16, device="cuda")  # the most that are taken
+    turned, out = torch.empty_like(wide), torch.empty_like(wide)
+    append(pair, lists, "f32", wide, wide[:, :1], wide[:, :1], turned)
+    assert torch.equal(turned, wide)
+    attend(pair, lists, "f32", wide, out)
+    assert int(pair.counts[0]) == 1
+    # (not the token's value bit for bit: its weight is 2^(s - m) with m = s rounded,
+    # which is 1 to 2^-24 of s, held to 2^-22 in the product and as it is in the sum)
+    model_append(pair, lists, wide[:, :1], wide[:, :1], [])
+    check_attention(pair, Batch(gpu, [[0]]), "f32", wide, out)
+    step = gpu.Kv8SparseStep(pair.cache, 1, 1, 1, 1)
+    pair.cache.close()
+    with pytest.raises(gpu.InvalidArgument, match="closed"):
+        step.run(1, 1, 1, 0, x.data_ptr(), 16, lists.keep["page_offsets"].data_ptr(),
+                 lists.keep["page_ids"].data_ptr(), x.data_ptr(), 16)
+    with pytest.raises(gpu.InvalidArgument, match="non-null"):
+        append(pair, lists, "f32", None, x[:, :1], x[:, :1], None)
+    step.close()
+
+
+def test_captured_append_outlives_other_rotations(gpu):
+    import torch
+    rng = np.random.default_rng(41)
+    pair = Pair(gpu, 1, 128, 16, 4)
+    pair.cache.set_rotation(16, inv_freq(16))
+    batch = Batch(gpu, [[2, 1]], [0], [20])
+    q, k = rows(rng, "bf16", 20, 3, 128), rows(rng, "bf16", 20, 1, 128)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    append(pair, batch, "bf16", q, k, k, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append(pair, batch, "bf16", q, k, k, out, stream=torch.cuda.current_stream().cuda_stream)
+    for rotary in (128, 0, 64):
+        pair.cache.set_rotation(rotary, inv_freq(rotary) if rotary else [])
+        pair.cache.set_rotation(16, inv_freq(16))
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_sparse_step_without_pages_and_beside_captures(gpu):
+    import torch
+    rng = np.random.default_rng(43)
+    heads, kv, dim, page = 4, 2, 64, 16
+    pair = Pair(gpu, kv, dim, page, 40, rubbish=False)
+    pair.cache.set_rotation(dim, inv_freq(dim))
+    lists = [list(range(40)), []]
+    prompt = Batch(gpu, lists, [0, 0], [630, 0])
+    k = rows(rng, "bf16", 630, kv, dim)
+    append(pair, prompt, "bf16", None, k, k, None)
+    q = rows(rng, "bf16", 2, heads, dim)
+    cand = Batch(gpu, lists)
+    none = Batch(gpu, [[], []])
+    out = torch.full_like(q, 9.0)
+
+    def args(b, total):
+        return (2, total, total, 1, q.data_ptr(), q.stride(0), b.keep["page_offsets"].data_ptr(),
+                b.keep["page_ids"].data_ptr(), out.data_ptr(), out.stride(0))
+
+    for top_k, b, total in ((0, cand, 40), (5, none, 0), (0, none, 0)):
+        with gpu.Kv8SparseStep(pair.cache, heads, top_k, 2, 40) as step:
+            out.fill_(9.0)
+            step.run(*args(b, total))
+            step.status()
+            assert not bool(out.any()), (top_k, total)
+    with gpu.Kv8SparseStep(pair.cache, heads, 5, 2, 40) as step:
+        step.run(*args(cand, 40))
+        step.status()
+        want = out.clone()
+        assert bool(want[0].any()) and not bool(want[1].any())
+        side, other = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        step.run(*args(cand, 40), stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step.run(*args(cand, 40), stream=torch.cuda.current_stream().cuda_stream)
+            # a step elsewhere cannot follow a stream that is being captured
+            with pytest.raises(gpu.InvalidArgument, match="captured"):
+                step.run(*args(cand, 40), stream=other.cuda_stream)
+        for stream in (other.cuda_stream, 0, side.cuda_stream):
+            out.fill_(9.0)
+            torch.cuda.synchronize()
+            step.run(*args(cand, 40), stream=stream)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            out.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        step.status()
