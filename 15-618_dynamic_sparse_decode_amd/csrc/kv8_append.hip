@@ -606,16 +606,27 @@ __device__ __forceinline__ void Queries(const Kv8AppendArgs& a, bool vec, const 
   if (mine >= per_step) return;
   const Unit w = UnitOf(u, a.rot);
   const unsigned inverse = 0xffffffffu / static_cast<unsigned>(row_heads) + 1u;
-  for (int i = mine; i < (p.hi - p.lo) * row_heads; i += per_step) {
+  // The next row's numbers are asked for before this one's are turned.
+  const int end = (p.hi - p.lo) * row_heads;
+  Packed<T, 16> next;
+  int next_o = 0;
+  T* next_out = nullptr;
+  auto load = [&](int i) {
     const int k = row_heads == 1 ? i : static_cast<int>(__umulhi(i, inverse));
-    const int o = p.lo + k;
+    next_o = p.lo + k;
     const int64_t head = static_cast<int64_t>(h0 + i - k * row_heads) * a.c.dim;
-    const int64_t at = t.row + p.c0 + o;
+    const int64_t at = t.row + p.c0 + next_o;
     const T* from = static_cast<const T*>(a.q) + at * a.q_stride + head;
-    T* out = static_cast<T*>(a.q_out) + at * a.out_stride + head;
-    Packed<T, 16> x;
-    x.Load8(0, from + w.a, vec);
-    x.Load8(8, from + w.b, vec);
+    next_out = static_cast<T*>(a.q_out) + at * a.out_stride + head;
+    next.Load8(0, from + w.a, vec);
+    next.Load8(8, from + w.b, vec);
+  };
+  if (mine < end) load(mine);
+  for (int i = mine; i < end; i += per_step) {
+    Packed<T, 16> x = next;
+    const int o = next_o;
+    T* out = next_out;
+    if (i + per_step < end) load(i + per_step);
     // two pairs at a time: whole words of results
     if (u < turning) {
       const double2* at_cs = cs + (o * 8 * turning + u);
