@@ -288,19 +288,36 @@ __device__ __forceinline__ void FillSines(const Kv8AppendArgs& a, const Task& t,
   const double2* table = a.rot.table + p;
   double2 high = {1.0, 0.0};
   unsigned known = 0xffffffffu;  // whose upper bytes `high` is of
-  for (int o = lo + k; o < hi; o += step) {
-    const int at =
-        a.b.positions != nullptr ? a.b.positions[t.row + c0 + o] : t.index + c0 + o;
-    const unsigned far = at < 0 ? 0u - static_cast<unsigned>(at) : static_cast<unsigned>(at);
-    if (far >> 8 != known) {
-      known = far >> 8;
-      high = Times(Times(table[(256u + ((far >> 8) & 255u)) * pairs],
-                         table[(512u + ((far >> 16) & 255u)) * pairs]),
-                   table[(768u + (far >> 24)) * pairs]);
-      high = {high.x * a.rot.magnitude, high.y * a.rot.magnitude};
+  // (four tokens' entries on their way at once: the tables are in L2)
+  constexpr int kAhead = 4;
+  for (int o0 = lo + k; o0 < hi; o0 += kAhead * step) {
+    int at[kAhead];
+    double2 low[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int o = c0 + min(o0 + i * step, hi - 1);
+      at[i] = a.b.positions != nullptr ? a.b.positions[t.row + o] : t.index + o;
     }
-    const double2 w = Times(table[(far & 255u) * pairs], high);
-    cs[SineAt(o, p & 7, p >> 3, pairs / 8)] = {w.x, at < 0 ? -w.y : w.y};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const unsigned far = at[i] < 0 ? 0u - static_cast<unsigned>(at[i]) : static_cast<unsigned>(at[i]);
+      low[i] = table[(far & 255u) * pairs];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int o = o0 + i * step;
+      if (o >= hi) break;
+      const unsigned far = at[i] < 0 ? 0u - static_cast<unsigned>(at[i]) : static_cast<unsigned>(at[i]);
+      if (far >> 8 != known) {
+        known = far >> 8;
+        high = Times(Times(table[(256u + ((far >> 8) & 255u)) * pairs],
+                           table[(512u + ((far >> 16) & 255u)) * pairs]),
+                     table[(768u + (far >> 24)) * pairs]);
+        high = {high.x * a.rot.magnitude, high.y * a.rot.magnitude};
+      }
+      const double2 w = Times(low[i], high);
+      cs[SineAt(o, p & 7, p >> 3, pairs / 8)] = {w.x, at[i] < 0 ? -w.y : w.y};
+    }
   }
 }
 
