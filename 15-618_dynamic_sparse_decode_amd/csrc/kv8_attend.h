@@ -203,9 +203,9 @@ __device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {
   return min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
 }
 
-// One row's pieces.  Grid (key heads * rows, batch): the pieces' factors first, in LDS, so that the sums' loads wait for nothing; the
-// threads beyond a row's quads take every 256 / quads-th piece, and their sums
-// are added in that order.
+// One row's pieces.  Grid (key heads * rows, batch): the pieces' factors first, in
+// LDS, while the first parts are on their way; the threads beyond a row's quads
+// take every 256 / quads-th piece, and their sums are added in that order.
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   __shared__ float factor[kMostPieces];
@@ -271,7 +271,8 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
 }
 
 // The same for few pieces and many rows: a wave a row, four a workgroup.  Grid
-// (key heads * rows / 4, batch).
+// (key heads * rows / 4, batch).  1024 rows are a quarter of the waves that the
+// chip holds; 2048 rows of 4 pieces took 6.5 us, with a workgroup a row 7.8.
 constexpr int kFewPieces = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8MergeRowsKernel(Kv8AttendArgs a, Plan p) {
