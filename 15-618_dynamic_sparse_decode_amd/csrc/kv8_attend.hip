@@ -369,9 +369,34 @@ __global__ __launch_bounds__(256) void Kv8GroupQueriesKernel(const T* q, int64_t
 
 constexpr int kWaves = 4;
 
-// Two workgroups fit a CU (registers), 512 the chip; a piece has a group of 64
-// tokens for each of its four waves at least.
+// Two workgroups fit a CU (registers), 512 the chip.
 constexpr int kTarget = 512;
+
+// Pieces that lists of so many groups are cut into, `units` workgroups to a piece.
+// In us: a launch about 5.5; a step, a group for each of the four waves, 1.15 and
+// more where workgroups share the memory's rate, up to 5.9 TB/s; the merge, with
+// its launch, 3.5 to 5.9.  Heads of 128 (32 / 8), bf16, us whole and in pieces:
+// one of 512 tokens 8.2 and 10.3, of 2000 15.0 and 10.4, of 32000 158 and 22; 16
+// of 1000 12.9 and 16.8, of 2000 17.7 and 19.9, of 8000 64 and 56; 32 of 500 11.7
+// and 17.1.  Lists are seldom equally long, and pieces end more evenly: of choices
+// within 3% the one with most pieces.
+int64_t PiecesWanted(int64_t groups, int64_t most, int64_t units, int dim) {
+  const int64_t steps = (groups + kWaves - 1) / kWaves;
+  const double share = 8.7e-5 * dim;  // us of a step's bytes of one workgroup
+  auto cost = [&](int64_t n) {
+    const double workgroups = static_cast<double>(units * n);
+    const double step = std::max(1.15 + 0.6 * share * workgroups, share * workgroups);
+    const double merge = n > 1 ? 3.5 + 2.4 * std::min(1.0, workgroups / 256) : 0.0;
+    return 5.5 + static_cast<double>((steps + n - 1) / n) * step + merge;
+  };
+  most = std::min(most, steps);
+  double best = cost(1);
+  for (int64_t n = 2; n <= most; ++n) best = std::min(best, cost(n));
+  int64_t n = most;
+  while (n > 1 && cost(n) > 1.03 * best) --n;
+  return n;
+}
+
 Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal) {
   Plan p;
   p.group = q_heads / c.heads;
@@ -379,7 +404,9 @@ Plan MakePlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool causal
   p.block = 16;
   p.blocks = static_cast<int>((p.rows + p.block - 1) / p.block);
   const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
-  CutLists(&p, ListGroups(c, b), kTarget / std::max<int64_t>(units, 1), kWaves);
+  const int64_t groups = ListGroups(c, b);
+  const int64_t most = std::min<int64_t>(kTarget / std::max<int64_t>(units, 1), kMostPieces);
+  CutLists(&p, groups, PiecesWanted(groups, std::max<int64_t>(most, 1), units, c.dim), kWaves);
   return p;
 }
 
