@@ -9,7 +9,7 @@
 // wave's products run beside another's exponentials.
 //
 // Measured (kernel times): one prompt of 8192 tokens, 32 bf16 query heads of 128
-// over 8 key heads, 605-620 us for 550 GFLOP (900 TFLOP/s; a large bf16 matrix
+// over 8 key heads, 600-630 us for 550 GFLOP (870-910 TFLOP/s; a large bf16 matrix
 // product alone reaches 1356 here), the matrix units busy 43 % of the time and
 // the vector units about 60 %; 16 prompts of 1-700 tokens 82 us (27 GFLOP: the
 // longest prompts' last rows end it).  On the way there (the long prompt):
