@@ -28,6 +28,8 @@
 namespace dsdk {
 namespace {
 
+constexpr float kMostFactor = 100.0f;  // powers of two beyond which weights are formed in steps
+
 // Grid (key heads * row tiles, batch, pieces); W waves, each of which takes
 // every W-th group of 64 tokens of the piece for all of the tile's 16 rows.
 // Lane (n, g) = (lane % 16, lane / 16).  Logits come out transposed, S^T = K
@@ -200,7 +202,8 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
       most *= f;
       seen = seen || count > 0;
       const float m_new = fmaxf(m, Max4(most));
-      const float mv_new = fmaxf(mv, Max4(most + __builtin_amdgcn_logf(now.value_scale)));
+      const float log_v = __builtin_amdgcn_logf(now.value_scale);
+      const float mv_new = fmaxf(mv, Max4(most + log_v));
       const float base = m_new == -INFINITY ? 0.0f : m_new;
       const float base_v = mv_new == -INFINITY ? 0.0f : mv_new;
       if (__ballot(m_new > m || mv_new > mv) != 0) {
@@ -211,15 +214,28 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
         m = m_new;
         mv = mv_new;
       }
-      const float to_half = now.value_scale * Exp2(base - base_v + kWeightBits);
+      // A weight is p * to_half, p = 2^(s - base).  Where the largest p's values are
+      // next to nothing (a page of zeros has the scale 2^-126) the two factors reach
+      // 2^141 and more, the product 2^15 all the same: such a lane's 2^rise goes
+      // from to_half to p, and to_half is formed in two steps.
+      const float up = base - base_v + kWeightBits;
+      float to_half = now.value_scale * Exp2(up);
+      float start = -base, to_sum = 1.0f;
+      if (__ballot(up > kMostFactor || log_v + up > kMostFactor) != 0) {  // seldom
+        const float rise = fmaxf(ceilf(log_v + up - kMostFactor), 0.0f);
+        const float lift = up - rise > 0.5f * kMostFactor ? 0.5f * kMostFactor : 0.0f;
+        to_half = now.value_scale * Exp2(lift) * Exp2(up - rise - lift);
+        start = rise - base;
+        to_sum = Exp2(-rise);
+      }
       F16x8 w[2][NP];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float e0 = Exp2(fmaf(x[t][i], f, -base));
-          const float e1 = Exp2(fmaf(x[t][i + 1], f, -base));
-          l += e0 + e1;
+          const float e0 = Exp2(fmaf(x[t][i], f, start));
+          const float e1 = Exp2(fmaf(x[t][i + 1], f, start));
+          l = fmaf(e0 + e1, to_sum, l);
           SplitWeights(e0 * to_half, e1 * to_half, w[t >> 1], 4 * (t & 1) + i);
         }
       }
