@@ -24,6 +24,16 @@ __device__ __forceinline__ float Sum4(float x) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// 2^x as a product of two: Exp2 gives nothing below 2^-126, and a row whose values
+// have scales near that has factors below it.  Of x >= -64 the second is one.
+struct Power {
+  float most, rest;
+};
+__device__ __forceinline__ Power PowerOf(float x) {
+  const bool low = x < -64.0f;
+  return {Exp2(low ? x + 64.0f : x), low ? 0x1p-64f : 1.0f};
+}
+
 // Eight codes (two words) as half-precision numbers.
 template <int FMT>
 __device__ __forceinline__ F16x8 Numbers8(unsigned w0, unsigned w1) {
@@ -184,6 +194,13 @@ __device__ __forceinline__ void StoreRow4(T* p, bool vec, F32x4 o) {
 // batch's sizes alone (the lengths themselves are on the device); a second launch
 // joins them.
 constexpr int kMostPieces = 64;
+// A row's piece: its sum of weights is l * 2^m, of weights times values its part *
+// 2^(m + top).  (The parts are relative to a maximum of their own: a page whose
+// tokens weigh 2^-150 of another's may have values 2^150 times as large.)
+struct PieceStats {
+  float m, l;  // l < 0: no token
+  float top;
+};
 struct Plan {
   int group = 1;     // query heads per key head
   int64_t rows = 1;  // of a request and key head, at most
@@ -192,7 +209,7 @@ struct Plan {
   int pieces = 1;    // a list is cut into at most this many
   int piece = 1;     // groups of 64 tokens in a piece
   float* part = nullptr;    // [batch][key heads][rows][pieces][dim]
-  float2* stats = nullptr;  // [batch][key heads][rows][pieces]: (m, l), l < 0: no token
+  PieceStats* stats = nullptr;  // [batch][key heads][rows][pieces]
 };
 __device__ __forceinline__ int64_t PartSlot(const Plan& p, int heads, int r, int head, int row) {
   return ((static_cast<int64_t>(r) * heads + head) * p.rows + row) * p.pieces;
@@ -203,12 +220,36 @@ __device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {
   return min(p.pieces, max(1, (groups + p.piece - 1) / p.piece));
 }
 
+// The factors that join a row's pieces (`some`: this lane's has a token): its own of
+// each lane's piece, then `last` of their sum.  The first kLanes lanes have pieces.
+template <int kLanes>
+__device__ __forceinline__ float JoinFactor(const PieceStats& st, bool some, Power* last) {
+  float peak = some ? st.m : -INFINITY;
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+  const float base = peak == -INFINITY ? 0.0f : peak;
+  float sum = some ? st.l * Exp2(st.m - base) : 0.0f;
+  const float x = some ? st.m - base + st.top : -INFINITY;
+  float top = x;
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) {
+    sum += __shfl_xor(sum, o, kWave);
+    top = fmaxf(top, __shfl_xor(top, o, kWave));
+  }
+  top = top == -INFINITY ? 0.0f : top;
+  Power to_out = PowerOf(top);
+  if (__ballot(some) != 0) to_out.most /= sum;
+  *last = {__shfl(to_out.most, 0, kWave), __shfl(to_out.rest, 0, kWave)};
+  return Exp2(x - top);
+}
+
 // One row's pieces.  Grid (key heads * rows, batch): the pieces' factors first, in
 // LDS, while the first parts are on their way; the threads beyond a row's quads
 // take every 256 / quads-th piece, and their sums are added in that order.
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   __shared__ float factor[kMostPieces];
+  __shared__ Power last;
   __shared__ F32x4 part_sum[256];
   const Kv8View& c = a.c;
   const int D = c.dim, quads = D / 4;
@@ -223,17 +264,11 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   const int shares = 256 / quads;  // threads per quad
   const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
   if (threadIdx.x < kWave) {
-    float2 st = make_float2(-INFINITY, -1.0f);
+    PieceStats st = {-INFINITY, -1.0f, 0.0f};
     if (lane < pieces) st = p.stats[slot0 + lane];
-    const bool some = !(st.y < 0.0f);
-    float peak = some ? st.x : -INFINITY;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
-    const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
-    float sum = some ? st.y * e : 0.0f;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-    factor[lane] = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+    Power to_out;
+    factor[lane] = JoinFactor<kWave>(st, !(st.l < 0.0f), &to_out);
+    if (lane == 0) last = to_out;
   }
   // (loads that do not need the factors are on their way meanwhile)
   constexpr int kAhead = 4;
@@ -264,6 +299,7 @@ __global__ __launch_bounds__(256) void Kv8MergeKernel(Kv8AttendArgs a, Plan p) {
   __syncthreads();
   if (share > 0) return;
   for (int i = 1; i < shares; ++i) o += part_sum[i * quads + threadIdx.x];
+  o = o * last.most * last.rest;
   const int tok = at / p.group;
   T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
            static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
@@ -289,7 +325,7 @@ __global__ __launch_bounds__(256) void Kv8MergeRowsKernel(Kv8AttendArgs a, Plan 
   const int pieces = Pieces(p, s);
   if (pieces == 1 || at >= s.rows) return;
   const int64_t slot0 = PartSlot(p, c.heads, r, head, at);
-  float2 st = make_float2(-INFINITY, -1.0f);
+  PieceStats st = {-INFINITY, -1.0f, 0.0f};
   if (lane < pieces) st = p.stats[slot0 + lane];
   const float* part = p.part + slot0 * D + 4 * lane;
   F32x4 x[kFewPieces];
@@ -298,15 +334,8 @@ __global__ __launch_bounds__(256) void Kv8MergeRowsKernel(Kv8AttendArgs a, Plan 
     x[z] = F32x4{0, 0, 0, 0};
     if (lane < quads && z < pieces) x[z] = *reinterpret_cast<const F32x4*>(part + z * D);
   }
-  const bool some = !(st.y < 0.0f);
-  float peak = some ? st.x : -INFINITY;
-#pragma unroll
-  for (int o = 1; o < kFewPieces; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
-  const float e = some ? Exp2(st.x - (peak == -INFINITY ? 0.0f : peak)) : 0.0f;
-  float sum = some ? st.y * e : 0.0f;
-#pragma unroll
-  for (int o = 1; o < kFewPieces; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-  const float factor = (__ballot(some) != 0 ? 1.0f / sum : 1.0f) * e;
+  Power last;
+  const float factor = JoinFactor<kFewPieces>(st, !(st.l < 0.0f), &last);
   F32x4 o = {0, 0, 0, 0};
 #pragma unroll
   for (int z = 0; z < kFewPieces; ++z) {
@@ -314,6 +343,7 @@ __global__ __launch_bounds__(256) void Kv8MergeRowsKernel(Kv8AttendArgs a, Plan 
     if (z < pieces) o += x[z] * f;
   }
   if (lane >= quads) return;
+  o = o * last.most * last.rest;
   const int tok = at / p.group, d = 4 * lane;
   T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
            static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
@@ -336,13 +366,13 @@ inline size_t PlanSlots(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p)
   return static_cast<size_t>(b.batch) * c.heads * p.rows * p.pieces;
 }
 inline size_t PlanBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
-  return p.pieces == 1 ? 0 : PlanSlots(c, b, p) * (sizeof(float) * c.dim + sizeof(float2));
+  return p.pieces == 1 ? 0 : PlanSlots(c, b, p) * (sizeof(float) * c.dim + sizeof(PieceStats));
 }
 // What any batch needs at most whose rows per request are no more: lists are cut
 // into as many pieces as keep the workgroups within `target`.
 inline size_t MostPartBytes(const Kv8View& c, const Plan& p, int target) {
   const size_t rows = static_cast<size_t>(p.rows < p.block ? p.rows : p.block);
-  return target * rows * (sizeof(float) * c.dim + sizeof(float2));
+  return target * rows * (sizeof(float) * c.dim + sizeof(PieceStats));
 }
 // The pieces' places in the call's workspace; without one lists stay whole.
 inline void PlaceParts(Plan* p, const Kv8AttendArgs& a) {
@@ -352,7 +382,7 @@ inline void PlaceParts(Plan* p, const Kv8AttendArgs& a) {
   }
   if (p->pieces == 1) return;
   p->part = static_cast<float*>(a.workspace);
-  p->stats = reinterpret_cast<float2*>(p->part + PlanSlots(a.c, a.b, *p) * a.c.dim);
+  p->stats = reinterpret_cast<PieceStats*>(p->part + PlanSlots(a.c, a.b, *p) * a.c.dim);
 }
 
 template <typename T>

@@ -333,16 +333,18 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
     const int k = i / quads, d = 4 * (i - k * quads);
     const int at = first + k;
     if (at >= s.rows) break;
-    float peak = -INFINITY;
+    float peak = -INFINITY, top = -INFINITY;
     bool some = false;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (!(s_l[w * 16 + k] < 0.0f)) {
         peak = fmaxf(peak, s_m[w * 16 + k]);
+        top = fmaxf(top, s_mv[w * 16 + k]);
         some = true;
       }
     }
     const float base = peak == -INFINITY ? 0.0f : peak;
+    top = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     F32x4 o = {0, 0, 0, 0};
 #pragma unroll
@@ -350,20 +352,22 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
       if (!(s_l[w * 16 + k] < 0.0f)) {
         sum += s_l[w * 16 + k] * Exp2(s_m[w * 16 + k] - base);
         o += *reinterpret_cast<const F32x4*>(s_acc + (w * 16 + k) * (D + 4) + d) *
-             Exp2(s_mv[w * 16 + k] - base - kWeightBits);
+             Exp2(s_mv[w * 16 + k] - top);
       }
     }
+    const float x = top - base - kWeightBits;  // o lacks 2^x
     if (pieces == 1) {
       const int tok = at / p.group;
       T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
                static_cast<int64_t>(head * p.group + at - tok * p.group) * D + d;
       const F32x4 zero = {0, 0, 0, 0};
+      const Power to_out = PowerOf(x);
       StoreRow4(out, reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0,
-                some ? o / sum : zero);
+                some ? o * (to_out.most / sum) * to_out.rest : zero);
     } else {
       const int64_t slot = PartSlot(p, c.heads, r, head, at) + blockIdx.z;
       *reinterpret_cast<F32x4*>(p.part + slot * D + d) = o;
-      if (d == 0) p.stats[slot] = make_float2(peak, some ? sum : -1.0f);
+      if (d == 0) p.stats[slot] = {peak, some ? sum : -1.0f, x};
     }
   }
 }

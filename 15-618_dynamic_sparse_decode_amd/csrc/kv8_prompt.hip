@@ -397,15 +397,21 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
   l = Sum2(l);
   if (!there) return;
   const float base = m == -INFINITY ? 0.0f : m;
-  float to_out = Exp2(mv - base - kPromptBits);
+  const float lacks = (mv == -INFINITY ? 0.0f : mv) - base - kPromptBits;  // acc: 2^lacks
+  Power to_out = PowerOf(lacks);
   const bool none = (bad && m == -INFINITY) || sees <= begin * kGroup;  // no token here
   float* part = nullptr;
   if (pieces > 1) {
     const int64_t slot = PartSlot(plan, c.heads, r, head, row) + piece;
     part = plan.part + slot * D;
-    if (h == 0) plan.stats[slot] = make_float2(m, none ? -1.0f : l);
+    if (h == 0) plan.stats[slot] = {m, none ? -1.0f : l, lacks};
+    to_out = {1.0f, 1.0f};
   } else {
-    to_out /= none ? 1.0f : l;
+    to_out.most /= none ? 1.0f : l;
+  }
+  if (__ballot(to_out.rest != 1.0f) != 0) {  // seldom
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] *= to_out.rest;
   }
   T* out = static_cast<T*>(a.out) + (s.q.row0 + token) * a.out_stride +
            static_cast<int64_t>(q_head) * D;
@@ -418,7 +424,7 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
       if (kDim > 0 || d < D) {
         F32x4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = acc[t][i + e] * to_out;
+        for (int e = 0; e < 4; ++e) o[e] = acc[t][i + e] * to_out.most;
         if constexpr (FMT == DSD_KV8_E4M3) {
           const int4 nan = *reinterpret_cast<const int4*>(nan_from + d);
           const int least = min(min(nan.x, nan.y), min(nan.z, nan.w));

@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache where value scales are extreme: values that are
-all zero, whose page scale is the least there is, 2^-126."""
+all zero, whose page scale is the least there is, 2^-126, values as small and as
+large as float32 has, and both in one list."""
 from __future__ import annotations
 
 import numpy as np
@@ -124,3 +125,38 @@ def test_zero_values_through_append_and_sparse_step(gpu, kind, fmt):
         kept = Batch(gpu, [selected[r, :int(counts[r])].tolist() for r in range(2)])
         check_attention(pair, kept, kind, q, out)
         assert not bool(out[0, heads // kv:].any()) and not bool(out[1].any())
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt", [kv8.E4M3, kv8.INT8])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("spread", [1.0, 40.0])
+def test_value_scales_far_apart(gpu, spread, kind, fmt, form):
+    """Value scales from 2^-126 to 2^100 in one list and in lists of their own,
+    with logits that differ by little and by more than a hundred."""
+    rng = np.random.default_rng(6)
+    page, heads, capacity = 16, 4, 48
+    pair = Pair(gpu, 2, 64, page, capacity, fmt)
+    pair.fill(8)
+    powers = rng.permutation(np.linspace(-126, 100, capacity).round())
+    set_values(pair, range(capacity), codes=True, scale=np.exp2(powers))
+    order = np.argsort(powers).tolist()
+    lists = [list(range(capacity)), order, order[::-1], order[:5], order[:20], order[14:18], order[24:30],
+             order[40:], order[:1], order[-1:], order[:8] + order[28:36], order[30:34] + order[:12]]
+    check_form(pair, form, kind, lists, rng, heads, spread)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt", [kv8.E4M3, kv8.INT8])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [-126, -120, 117])
+def test_smallest_and_largest_values(gpu, power, kind, fmt, form):
+    """Every value scale next to the ends of float32: numbers that float32 and
+    bf16 hold come out, and the sum before its division does not overflow."""
+    rng = np.random.default_rng(7)
+    page, capacity = 16, 130
+    pair = Pair(gpu, 2, 64, page, capacity, fmt)
+    pair.fill(9)
+    set_values(pair, range(capacity), codes=True, scale=np.exp2(power + rng.integers(0, 3, capacity)))
+    lists = [list(range(capacity)), [4, 7, 9, 1, 2], [5], list(range(40)) * 4]
+    check_form(pair, form, kind, lists, rng, 4, 0.1)
