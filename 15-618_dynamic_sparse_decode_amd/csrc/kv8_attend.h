@@ -8,6 +8,10 @@
 namespace dsdk {
 namespace {
 
+// Maxima beyond which a logit's products are rounded before the maximum is taken off:
+// one is off by half its last place, 2^-7 here and whole powers of two further out,
+// and the exponential of what a fused product keeps of it would grow by as much.
+constexpr float kFar = 0x1p18f;
 constexpr float kWeightBits = 15.0f;  // weights reach 2^15 (half precision ends at 2^16)
 
 // The larger (sum) of the four lanes that share lane % 16.

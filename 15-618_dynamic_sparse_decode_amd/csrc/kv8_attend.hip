@@ -9,7 +9,7 @@
 // the logits afterwards, in float32.  Weights p = 2^(s - m) (s in the log2
 // domain, m the running maximum) meet the value codes the same way, as p * v *
 // 2^(m - n + 15) with v the page's value scale and n the running maximum of s +
-// log2 v, so at most 2^15 whatever the scales: half precision rounds them to
+// log2 v, so at most 2^15 whatever the scales and logits: half precision rounds them to
 // 2^-11, or 2^-22 as two terms where the output is finer than bf16.  All sums
 // are float32.
 //
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = F32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  float mv = -INFINITY;  // of s + log2(value scale): acc is relative to it
+  float top = -INFINITY;  // of s + log2(value scale), less m: acc is relative to it
   bool seen = false;
 
   // The list's pages are staged in LDS, so that a group's addresses are known
@@ -202,39 +202,49 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
       most *= f;
       seen = seen || count > 0;
       const float m_new = fmaxf(m, Max4(most));
-      const float log_v = __builtin_amdgcn_logf(now.value_scale);
-      const float mv_new = fmaxf(mv, Max4(most + log_v));
       const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float base_v = mv_new == -INFINITY ? 0.0f : mv_new;
-      if (__ballot(m_new > m || mv_new > mv) != 0) {
+      const float log_v = __builtin_amdgcn_logf(now.value_scale);
+      const float was = top + (m - base);
+      const float top_new = fmaxf(was, Max4(most - base + log_v));
+      const float base_top = top_new == -INFINITY ? 0.0f : top_new;
+      if (__ballot(m_new > m || top_new > was) != 0) {
         l *= Exp2(m - base);
-        const float shrink = Exp2(mv - base_v);
+        const float shrink = Exp2(was - base_top);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] *= shrink;
         m = m_new;
-        mv = mv_new;
+        top = top_new;
       }
       // A weight is p * to_half, p = 2^(s - base).  Where the largest p's values are
       // next to nothing (a page of zeros has the scale 2^-126) the two factors reach
       // 2^141 and more, the product 2^15 all the same: such a lane's 2^rise goes
       // from to_half to p, and to_half is formed in two steps.
-      const float up = base - base_v + kWeightBits;
+      const float up = kWeightBits - base_top;
       float to_half = now.value_scale * Exp2(up);
-      float start = -base, to_sum = 1.0f;
-      if (__ballot(up > kMostFactor || log_v + up > kMostFactor) != 0) {  // seldom
+      float slope = f, start = -base, to_sum = 1.0f;
+      if (__ballot(up > kMostFactor || log_v + up > kMostFactor || fabsf(base) > kFar) != 0) {  // seldom
         const float rise = fmaxf(ceilf(log_v + up - kMostFactor), 0.0f);
         const float lift = up - rise > 0.5f * kMostFactor ? 0.5f * kMostFactor : 0.0f;
         to_half = now.value_scale * Exp2(lift) * Exp2(up - rise - lift);
         start = rise - base;
         to_sum = Exp2(-rise);
+        if (fabsf(base) > kFar) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][i] = x[t][i] * f - base;
+          }
+          slope = 1.0f;
+          start = rise;
+        }
       }
       F16x8 w[2][NP];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float e0 = Exp2(fmaf(x[t][i], f, start));
-          const float e1 = Exp2(fmaf(x[t][i + 1], f, start));
+          const float e0 = Exp2(fmaf(x[t][i], slope, start));
+          const float e1 = Exp2(fmaf(x[t][i + 1], slope, start));
           l = fmaf(e0 + e1, to_sum, l);
           SplitWeights(e0 * to_half, e1 * to_half, w[t >> 1], 4 * (t & 1) + i);
         }
@@ -308,18 +318,18 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
     }
   }
 
-  // The waves' streams, through LDS: [W][16] m, l and mv, [W][16][D + 4] acc.
+  // The waves' streams, through LDS: [W][16] m, l and top, [W][16][D + 4] acc.
   __syncthreads();
   float* s_m = lds;
   float* s_l = lds + 16 * W;
-  float* s_mv = lds + 32 * W;
+  float* s_top = lds + 32 * W;
   float* s_acc = lds + 48 * W;
   l = Sum4(l);
   const bool any = Max4(seen ? 1.0f : 0.0f) > 0.0f;
   if (g == 0) {
     s_m[wave * 16 + n] = m;
     s_l[wave * 16 + n] = any ? l : -1.0f;
-    s_mv[wave * 16 + n] = mv;
+    s_top[wave * 16 + n] = top;
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -333,29 +343,36 @@ __global__ __launch_bounds__(W* kWave, NU <= 2 ? 2 : 1) void Kv8AttendKernel(Kv8
     const int k = i / quads, d = 4 * (i - k * quads);
     const int at = first + k;
     if (at >= s.rows) break;
-    float peak = -INFINITY, top = -INFINITY;
+    float peak = -INFINITY;
     bool some = false;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (!(s_l[w * 16 + k] < 0.0f)) {
         peak = fmaxf(peak, s_m[w * 16 + k]);
-        top = fmaxf(top, s_mv[w * 16 + k]);
         some = true;
       }
     }
     const float base = peak == -INFINITY ? 0.0f : peak;
-    top = top == -INFINITY ? 0.0f : top;
+    float most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (!(s_l[w * 16 + k] < 0.0f)) {
+        most = fmaxf(most, s_m[w * 16 + k] - base + s_top[w * 16 + k]);
+      }
+    }
+    most = most == -INFINITY ? 0.0f : most;
     float sum = 0.0f;
     F32x4 o = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (!(s_l[w * 16 + k] < 0.0f)) {
-        sum += s_l[w * 16 + k] * Exp2(s_m[w * 16 + k] - base);
+        const float e = s_m[w * 16 + k] - base;
+        sum += s_l[w * 16 + k] * Exp2(e);
         o += *reinterpret_cast<const F32x4*>(s_acc + (w * 16 + k) * (D + 4) + d) *
-             Exp2(s_mv[w * 16 + k] - top);
+             Exp2(e + s_top[w * 16 + k] - most);
       }
     }
-    const float x = top - base - kWeightBits;  // o lacks 2^x
+    const float x = most - kWeightBits;  // o lacks 2^x
     if (pieces == 1) {
       const int tok = at / p.group;
       T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +

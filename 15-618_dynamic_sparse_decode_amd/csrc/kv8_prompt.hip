@@ -249,8 +249,8 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
-  float mv = -INFINITY;  // of s + log2(value scale): acc is relative to it
-  // (m and mv follow within kSlack)
+  float top = -INFINITY;  // of s + log2(value scale), less m: acc is relative to it
+  // (m and top follow within kSlack)
 
   bad = __syncthreads_or(bad_here) != 0;
   fetch(begin);
@@ -325,27 +325,42 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
         most[t] *= f[t];
       }
       const float m_new = fmaxf(m, Max2(fmaxf(most[0], most[1])));
-      const float mv_new = fmaxf(
-          mv, Max2(fmaxf(most[0] + ci[0].log_value_scale, most[1] + ci[1].log_value_scale)));
-      if (__ballot(m_new > m + kSlack || mv_new > mv + kSlack) != 0) {
+      const float base_was = m == -INFINITY ? 0.0f : m;
+      const float top_new = Max2(fmaxf(most[0] - base_was + ci[0].log_value_scale,
+                                       most[1] - base_was + ci[1].log_value_scale));
+      if (__ballot(m_new - m > kSlack || top_new - top > kSlack) != 0) {
         const float from = m_new == -INFINITY ? 0.0f : m_new;
-        const float from_v = mv_new == -INFINITY ? 0.0f : mv_new;
+        const float was = top + (m - from);
+        top = fmaxf(was, Max2(fmaxf(most[0] - from + ci[0].log_value_scale,
+                                    most[1] - from + ci[1].log_value_scale)));
         l *= Exp2(m - from);
-        const float shrink = Exp2(mv - from_v);
+        const float shrink = Exp2(was - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] *= shrink;
         m = m_new;
-        mv = mv_new;
       }
       const float base = m == -INFINITY ? 0.0f : m;
-      const float base_v = mv == -INFINITY ? 0.0f : mv;
-      // A weight is 2^(s - base + c), c = log2 of the value scale + base - base_v +
-      // 11, of which the row's sum wants 2^(s - base): the chunk's own sum times
-      // 2^-c.  (Where c < -60 the weights are no half-precision number either way.)
-      float sum[2] = {0.0f, 0.0f};
+      const float base_top = top == -INFINITY ? 0.0f : top;
+      // A weight is 2^(s - base + lift), lift = log2 of the value scale - base_top + 11,
+      // of which the row's sum wants 2^(s - base): the chunk's own sum times 2^-lift
+      // (what lift - base loses to its rounding is then an error of s, in both sums).
+      // (Where lift < -60 the weights are no half-precision number either way.)
+      float sum[2] = {0.0f, 0.0f}, lift[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        to_half[t] = fmaxf(ci[t].log_value_scale - base_v + kPromptBits, -60.0f - base);
+        lift[t] = fmaxf(ci[t].log_value_scale - base_top + kPromptBits, -60.0f);
+        to_half[t] = lift[t] - base;
+      }
+      if (__ballot(fabsf(base) > kFar) != 0) {  // seldom
+        if (fabsf(base) > kFar) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[t][i] = x[t][i] * f[t] - base;
+            f[t] = 1.0f;
+            to_half[t] = lift[t];
+          }
+        }
       }
       // The weights of the first 32 tokens; then their products with the weights
       // of the others in between, as the two units take turns; then the others'.
@@ -388,16 +403,15 @@ Kv8PromptKernel(Kv8AttendArgs a, Plan plan) {
           if (kDim > 0) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      l += sum[0] * Exp2(-base - to_half[0]);
-      l += sum[1] * Exp2(-base - to_half[1]);
+      l += sum[0] * Exp2(-lift[0]);
+      l += sum[1] * Exp2(-lift[1]);
     }
     if (grp + 1 < groups) put(grp + 1, buf ^ 1);
   }
 
   l = Sum2(l);
   if (!there) return;
-  const float base = m == -INFINITY ? 0.0f : m;
-  const float lacks = (mv == -INFINITY ? 0.0f : mv) - base - kPromptBits;  // acc: 2^lacks
+  const float lacks = (top == -INFINITY ? 0.0f : top) - kPromptBits;  // acc: 2^lacks
   Power to_out = PowerOf(lacks);
   const bool none = (bad && m == -INFINITY) || sees <= begin * kGroup;  // no token here
   float* part = nullptr;
