@@ -512,8 +512,9 @@ size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) 
   size_t bytes = MostPartBytes(c, MakePlan(c, one, q_heads, false), kTarget);
   if (b.max_tokens > 1) {
     bytes = std::max(bytes, MostPartBytes(c, MakePlan(c, b, q_heads, true), kTarget));
-    if (ManyRows(c, b, q_heads)) bytes = std::max(bytes, Kv8PromptWorkspaceBytes(c, b, q_heads));
   }
+  // (of one token a request too, where query heads enough share a key head)
+  if (ManyRows(c, b, q_heads)) bytes = std::max(bytes, Kv8PromptWorkspaceBytes(c, b, q_heads));
   return bytes;
 }
 
