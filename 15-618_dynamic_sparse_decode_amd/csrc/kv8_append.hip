@@ -242,6 +242,25 @@ struct Task {
   int index = 0;  // the index in its request of offset 0
 };
 
+// The last request whose workgroups start no later than u, of those whose offsets
+// are in order (-1: none).
+__device__ __forceinline__ int RequestInOrder(const dsd_kv8_batch& b, int ps, int u) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int r = -1;
+  for (int b0 = 0; b0 < b.batch; b0 += kWave) {
+    const int i = b0 + lane;
+    bool mine = false;
+    if (i < b.batch) {
+      const int row = b.token_offsets[i], end = b.token_offsets[i + 1];
+      mine = row >= 0 && end >= row && end <= b.tokens && end - row <= b.max_tokens &&
+             row / ps + 2 * i <= u;
+    }
+    const unsigned long long ours = __ballot(mine);
+    if (ours != 0) r = b0 + kWave - 1 - __builtin_clzll(ours);
+  }
+  return r;
+}
+
 // The task of workgroup u: request r's pages take workgroups from
 // floor(token_offsets[r] / page) + 2 r on, at least as many as its tokens can
 // touch (one each where every request has one token).  Every wave computes
@@ -250,25 +269,38 @@ __device__ __forceinline__ bool FindTask(const Kv8AppendArgs& a, int u, Task* t)
   const dsd_kv8_batch& b = a.b;
   const int ps = a.c.page;
   int r = u, within = 0;
+  Kv8Request q;
+  bool ok = false;
   if (b.max_tokens > 1) {
     const int lane = threadIdx.x & (kWave - 1);
     int below = 0;
+    bool in_order = true;
     for (int b0 = 0; b0 < b.batch; b0 += kWave) {
       const int i = b0 + lane;
       bool mine = false;
       if (i < b.batch) mine = b.token_offsets[i] / ps + 2 * i <= u;
-      const int got = __popcll(__ballot(mine));
+      const unsigned long long ours = __ballot(mine);
+      in_order = in_order && (ours & (ours + 1)) == 0;
+      const int got = __popcll(ours);
       below += got;
       if (got < kWave) break;
     }
     r = below - 1;
+    if (r >= 0) ok = Kv8ReadTokens(b, r, ps, &q);
+    // An offset out of order hides the requests behind it, or those before it: the
+    // one it belongs to is skipped, the others are not.
+    if (!in_order || (r >= 0 && !ok)) {
+      r = RequestInOrder(b, ps, u);
+      if (r >= 0) ok = Kv8ReadTokens(b, r, ps, &q);
+    }
     if (r < 0) return false;
     within = u - (b.token_offsets[r] / ps + 2 * r);
     if (within < 0) return false;
+  } else {
+    if (r >= b.batch) return false;
+    ok = Kv8ReadTokens(b, r, ps, &q);
   }
-  if (r >= b.batch) return false;
-  Kv8Request q;
-  if (!Kv8ReadTokens(b, r, ps, &q)) {
+  if (!ok) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailShape);
     return false;
   }

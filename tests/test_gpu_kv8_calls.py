@@ -1,12 +1,13 @@
 """Calls of the 8-bit cache that the documentation allows, at its edges: what a
-workspace does for."""
+workspace does for, requests beside malformed ones."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import _kv8 as kv8
-from test_gpu_kv8 import Batch, Pair, attend, check_attention, rows
+from test_gpu_kv8 import (Batch, Pair, append, attend, check_attention, device, model_append,
+                          rows)
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,39 @@ def test_workspace_lets_long_lists_spread(gpu, heads, new, kind, fmt):
     larger = Batch(gpu, [list(range(pages))] * 3, [0] * 3, [new + 7] * 3)
     assert (pair.cache.workspace_bytes(larger.batch, heads)
             >= pair.cache.workspace_bytes(batch.batch, heads))
+
+
+@pytest.mark.parametrize("requests", [4, 9, 64, 65, 150])
+@pytest.mark.parametrize("wrong", [700000, -5, 0, 1, 2147483647, -2147483648])
+def test_append_beside_malformed_offsets(gpu, wrong, requests):
+    """One entry of token_offsets is wrong: the two requests that it bounds are
+    reported and skipped, all others are appended."""
+    import torch
+    rng = np.random.default_rng(requests)
+    page, at = 16, requests // 2
+    new = [int(n) for n in rng.integers(3, 40, requests)]
+    past = [int(p) for p in rng.integers(0, 16, requests)]
+    need = [-(-(p + n) // page) for p, n in zip(past, new)]
+    ends = np.cumsum(need)
+    lists = [list(range(e - n, e)) for e, n in zip(ends, need)]
+    pair = Pair(gpu, 2, 64, page, int(ends[-1]), rubbish=False)
+    batch = Batch(gpu, lists, past, new)
+    k, v = (rows(rng, "bf16", batch.tokens, 2, 64) for _ in range(2))
+    first = Batch(gpu, lists, [0] * requests, past)
+    k0, v0 = (rows(rng, "bf16", max(first.tokens, 1), 2, 64) for _ in range(2))
+    append(pair, first, "bf16", None, k0, v0, None)
+    model_append(pair, first, k0, v0, [])
+    offsets = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    offsets[at] = wrong
+    batch.keep["token_offsets"].copy_(device(offsets))
+    fail = torch.zeros(1, dtype=torch.int64, device="cuda")
+    append(pair, batch, "bf16", None, k, v, None, fail)
+    assert int(fail) & 0xffffffff == 2
+    for r in range(requests):
+        rows_of = slice(int(sum(new[:r])), int(sum(new[:r + 1])))
+        if r not in (at - 1, at):
+            one = Batch(gpu, [lists[r]], [past[r]], [new[r]])
+            model_append(pair, one, k[rows_of], v[rows_of], [])
+    pair.check_pages([p for r, l in enumerate(lists) if r not in (at - 1, at) for p in l])
+    # the two are as they were
+    pair.check_pages([l[0] for r, l in enumerate(lists) if r in (at - 1, at) and past[r]])
