@@ -3340,8 +3340,10 @@ int dsd_kv8_set_rotation(dsd_kv8* cache, int rotary_dim, int interleaved, const 
     Require(interleaved == 0 || interleaved == 1, "interleaved must be 0 or 1");
     Require(std::isfinite(magnitude), "magnitude must be finite");
     const int pairs = rotary_dim / 2;
-    // Entry j of a level is the j-th power of its first, in extended precision:
-    // off by 256 * 2^-64 at most.
+    // Entry j of a level is the j-th power of its first, in extended precision.  The
+    // angle's own error comes from inv_freq / 2 pi, held to 2^-63 of it: at most
+    // inv_freq * j * 2^(8 level - 63), so inv_freq * position * 2^-63 over the levels.
+    // The powers add 256 * 2^-64, the entry's rounding to 64 bits 2^-54.
     constexpr long double kTurn = 6.28318530717958647692528676655900576839L;
     std::vector<double2> table(static_cast<size_t>(pairs) * 4 * 256);
     for (int p = 0; p < pairs; ++p) {

@@ -4,7 +4,7 @@
 // Mathematics.  Codes are exact in half precision, so q K^T is a product of
 // half-precision matrices: q scaled by a power of two so that its row's
 // largest element lies in [2^13, 2^14) -- one term for 16-bit queries (what
-// falls below half precision's range is 2^-39 of that element), two for
+// falls below half precision's range is 2^-38 of that element), two for
 // float32 ones -- times the codes; the page's scale and the power of two go on
 // the logits afterwards, in float32.  Weights p = 2^(s - m) (s in the log2
 // domain, m the running maximum) meet the value codes the same way, as p * v *

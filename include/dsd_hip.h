@@ -647,9 +647,10 @@ int dsd_dense_run_batch_device(dsd_pool* pool, int batch,
  * is.  d_fail (may be NULL): memory the device writes
  * a code to when it cannot use an input: 2 a request's offsets or lengths do
  * not fit the batch's sizes (the request is skipped; dsd_kv8_attend gives it
- * zeros), 3 a page id outside the cache (the page holds no token, takes none);
- * the caller clears it before and reads it after the call.  Nothing outside the
- * arrays is touched then. */
+ * zeros), 3 a page id outside the cache (the page holds no token, takes none, and
+ * dsd_kv8_append leaves its tokens' rows of q_out as they were); the caller
+ * clears it before and reads it after the call.  Nothing outside the arrays is
+ * touched then. */
 typedef struct dsd_kv8 dsd_kv8;
 
 enum { DSD_KV8_E4M3 = 0, DSD_KV8_INT8 = 1 };
@@ -737,8 +738,12 @@ int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
  * (token_counts each): out = softmax(scale * q K^T) V.  num_q_heads is a
  * multiple of num_kv_heads up to 8192; query head h reads key head h / (num_q_heads /
  * num_kv_heads).  scale 0: 1 / sqrt(D).  A request without tokens gets zeros.
- * Logits, sums and outputs before their one rounding are float32; out has q's
- * type.  Row r of q and out is request r.
+ * Logits, their maxima, all sums and outputs before their one rounding are float32;
+ * out has q's type.  The matrix units' operands are half precision: codes are exact
+ * in it, 16-bit queries are held to 2^-38 of their row's largest element, float32
+ * ones, as two halves, to 2^-22 of each besides; a softmax weight is rounded to 11 bits where
+ * out is bf16 (which has 8) and to 22, as two halves, where it is float32 or f16.
+ * Row r of q and out is request r.
  * workspace (16-byte aligned): dsd_kv8_workspace_bytes of device memory lets
  * long lists spread over workgroups; it needs no initial contents, keeps none
  * between calls, and calls that may overlap (streams, graphs) need one each.
