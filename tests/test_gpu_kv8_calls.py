@@ -1,13 +1,13 @@
 """Calls of the 8-bit cache that the documentation allows, at its edges: what a
-workspace does for, requests beside malformed ones."""
+workspace does for, requests beside malformed ones, how weights are held."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import _kv8 as kv8
-from test_gpu_kv8 import (Batch, Pair, append, attend, check_attention, device, model_append,
-                          rows)
+from test_gpu_kv8 import (Batch, Pair, append, as64, attend, check_attention, device, lists_for,
+                          model_append, rows)
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,42 @@ def test_append_beside_malformed_offsets(gpu, wrong, requests):
     pair.check_pages([p for r, l in enumerate(lists) if r not in (at - 1, at) for p in l])
     # the two are as they were
     pair.check_pages([l[0] for r, l in enumerate(lists) if r in (at - 1, at) and past[r]])
+
+
+@pytest.mark.parametrize("fmt", [kv8.E4M3, kv8.INT8])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,page,lengths", [
+    (8, 2, 128, 16, [1, 65, 300, 2000]), (20, 1, 64, 64, [500, 129]), (6, 2, 256, 128, [130, 700]),
+])
+def test_weights_of_one_token(gpu, heads, kv, dim, page, lengths, kind, fmt):
+    """Attention of one token with page scales 2^24 apart, by a bound of its own: its
+    weights, times their page's scale, are held so that the row's largest is 2^15
+    (_kv8.allowed has 2^11, which is the many-rows form's).  A half's numbers end in
+    steps of 2^-24, so each is off by 2^-25 / 2^15 = 2^-40 of the largest."""
+    import torch
+    rng = np.random.default_rng(dim)
+    capacity = sum(-(-n // page) for n in lengths)
+    pair = Pair(gpu, kv, dim, page, capacity, fmt)
+    pair.fill(13)
+    m = pair.model
+    m.scales[1] = (m.scales[1] * np.exp2(rng.integers(-18, 7, m.scales[1].shape))).astype(np.float32)
+    pair.value_scales.copy_(torch.from_numpy(m.scales[1]))
+    lists = lists_for(rng, lengths, page, capacity)
+    for l, n in zip(lists, lengths):
+        if n % page:
+            pair.set_counts(l[-1], n % page)
+    q = rows(rng, kind, len(lengths), heads, dim)
+    batch = Batch(gpu, lists)
+    G = heads // kv
+    for workspace in (True, False):
+        out = torch.full_like(q, 9.0)
+        attend(pair, batch, kind, q, out, workspace=workspace)
+        for r, pages in enumerate(lists):
+            keys, values, most = m.rows(np.asarray(pages))
+            tokens = keys.shape[1]
+            for h in range(kv):
+                x, have = as64(q[r, h * G:(h + 1) * G]), as64(out[r, h * G:(h + 1) * G])
+                want, weighted, size, peak = kv8.attend(x, keys[h], values[h], dim ** -0.5, None, most[h])
+                may = (kv8.allowed(want, weighted, size, peak, dim, tokens, kind)
+                       - (tokens * (2.0 ** -36 - 2.0 ** -40) * peak)[:, None])
+                assert (np.abs(have - want) <= may).all(), (r, h)
