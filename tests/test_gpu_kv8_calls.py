@@ -1,13 +1,13 @@
 """Calls of the 8-bit cache that the documentation allows, at its edges: what a
-workspace does for, requests beside malformed ones, how weights are held."""
+workspace does for, requests beside malformed ones, how weights are held, caches beside each other."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import _kv8 as kv8
-from test_gpu_kv8 import (Batch, Pair, append, as64, attend, check_attention, device, lists_for,
-                          model_append, rows)
+from test_gpu_kv8 import (Batch, Pair, append, as64, attend, check_attention, device, inv_freq,
+                          lists_for, model_append, rows)
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,28 @@ def test_weights_of_one_token(gpu, heads, kv, dim, page, lengths, kind, fmt):
                 may = (kv8.allowed(want, weighted, size, peak, dim, tokens, kind)
                        - (tokens * (2.0 ** -36 - 2.0 ** -40) * peak)[:, None])
                 assert (np.abs(have - want) <= may).all(), (r, h)
+
+
+def test_caches_of_different_sizes_side_by_side(gpu):
+    """Handles share kernels, whose LDS goes by each cache's own sizes: the larger
+    ones run as before after smaller ones were made."""
+    import torch
+    rng = np.random.default_rng(44)
+    shapes = [(1, 256, 64), (2, 144, 16), (1, 128, 48), (2, 80, 16), (1, 64, 256), (1, 16, 16)]
+    pairs = [Pair(gpu, kv, dim, page, 6) for kv, dim, page in shapes]
+    for pair in pairs:
+        pair.cache.set_rotation(pair.model.dim // 32 * 32, inv_freq(pair.model.dim // 32 * 32))
+    for pair in pairs + pairs[::-1]:
+        m = pair.model
+        lists, new = [[4, 2]], [m.page + 9]
+        batch = Batch(gpu, lists, [0], new)
+        x = rows(rng, "f32", new[0], 3 * m.heads, m.dim)
+        k, v = x[:, :m.heads], x[:, m.heads:2 * m.heads]
+        out = torch.empty_like(x)
+        append(pair, batch, "f32", x, k, v, out)
+        model_append(pair, batch, k, v, inv_freq(m.dim // 32 * 32))
+        pair.check_pages([4, 2])
+        for q, causal in ((x[:1].contiguous(), False), (x, True)):
+            out = torch.full_like(q, 9.0)
+            attend(pair, batch if causal else Batch(gpu, lists), "f32", q, out, causal=causal)
+            check_attention(pair, batch if causal else Batch(gpu, lists), "f32", q, out, causal=causal)
