@@ -20,11 +20,12 @@
 // values) of one head at a time.
 //
 // Measured (kernel times): 8192 tokens of 32 bf16 query and 8 key heads of 128,
-// pages of 16, 39-40 us for 186 MB, the 4.7 TB/s that a large copy reaches.
+// pages of 16, 40-41 us for 186 MB, 4.6 TB/s (a large copy reaches 4.7); int8 49.
 // Float32, 32 heads of each, 16 prompts of 100-1500 tokens in pages of 64: 310 us
-// for 0.98 GB; the 64-bit turns take a third of the vector units' time, and of the
+// for 0.98 GB (int8 436, which turns each key twice); the 64-bit turns take a third of the vector units' time, and of the
 // waits most are for a page's largest number, with four waves a SIMD (the sines of
-// 64 tokens fill LDS).  One token: 7.2 us, 64 of them 8.2, a chain of offsets ->
+// 64 tokens fill LDS).  Pages of 128, the prompt of 8192: 105 us, int8 125.  One
+// token: 7.2 us, 64 of them 8.2, a chain of offsets ->
 // ids -> scales -> codes after the launch.  Tried on the way: two heads of 16
 // waves in place of one of 8 in pages of 64 (374 us against 331), a loop over a
 // page's chunks in that kernel (spills), the first queries asked for before the

@@ -10,16 +10,18 @@
 // domain, m the running maximum) meet the value codes the same way, as p * v *
 // 2^(m - n + 15) with v the page's value scale and n the running maximum of s +
 // log2 v, so at most 2^15 whatever the scales and logits: half precision rounds them to
-// 2^-11, or 2^-22 as two terms where the output is finer than bf16.  All sums
-// are float32.
+// 2^-11, or 2^-22 as two terms where the output is finer than bf16 (bf16 outputs,
+// whose own rounding is 2^-8, are off by 0.0017 of their size either way; two terms
+// took 12.2 us in place of 11.5 for one request of 1000 tokens, 38.9 in place of
+// 37.6 for drafted tokens).  All sums are float32.
 //
 // Bound by HBM for long lists: a token's codes and scales are read once for all
 // query heads of its key head.  Measured (kernel times): 32 requests of 32768
-// tokens, 8 key heads of 128, pages of 16: 364 us for 2.15 GB, 5.9 TB/s, what
-// reads alone reach here; 64 requests of 32 pages of 64: 43 us, 6.3 TB/s; 16
+// tokens, 8 key heads of 128, pages of 16: 366 us for 2.15 GB, 5.9 TB/s, what
+// reads alone reach here; 64 requests of 32 pages of 64: 44 us, 6.2 TB/s; 16
 // requests of 512-2048 tokens, 32 key heads, float32: 36 us, 5.2 TB/s; 4 of
-// 65536-131072, int8, heads of 64: 40 us, 5.5 TB/s, and 5 for the merge; one of
-// 1000 tokens: 11 us, a chain of ids -> scales and codes -> products.
+// 65536-131072, int8, heads of 64: 42 us, 5.3 TB/s, and 5 for the merge; one of
+// 1000 tokens: 11.6 us, a chain of ids -> scales and codes -> products.
 #include "kv8_attend.h"
 
 #include <algorithm>

@@ -9,10 +9,10 @@
 // wave's products run beside another's exponentials.
 //
 // Measured (kernel times): one prompt of 8192 tokens, 32 bf16 query heads of 128
-// over 8 key heads, 600-630 us for 550 GFLOP (870-910 TFLOP/s; a large bf16 matrix
-// product alone reaches 1356 here), the matrix units busy 43 % of the time and
-// the vector units about 60 %; 16 prompts of 1-700 tokens 82 us (27 GFLOP: the
-// longest prompts' last rows end it).  On the way there (the long prompt):
+// over 8 key heads, 620 us for 550 GFLOP on one card and 665 on another (830-890
+// TFLOP/s; a large bf16 matrix product alone reaches 1356 here), the matrix units
+// busy 42 % of the time and the vector units 56 %; 16 prompts of 1-700 tokens 84 us
+// (27 GFLOP: the longest prompts' last rows end it); f16 rows 925 us, float32 1459.  On the way there (the long prompt):
 // shared groups in LDS in place of 16 rows a workgroup 1230 -> 695 us, operands
 // asked for four products ahead -> 658, products and exponentials in turn and
 // maxima that lag (kSlack) -> 631, the value scale in the exponent -> 621.
