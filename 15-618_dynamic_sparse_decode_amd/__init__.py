@@ -242,6 +242,11 @@ _SIGNATURES = {
                               + [ctypes.c_void_p, ctypes.c_int64] * 2
                               + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
                               + [ctypes.c_void_p] * 2),
+    "dsd_kv8_attend_cross": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                            ctypes.c_int, ctypes.c_int]
+                             + [ctypes.c_void_p, ctypes.c_int64] * 2
+                             + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
+                             + [ctypes.c_void_p] * 2),
     "dsd_kv8_sparse_create": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int] * 4
                               + [ctypes.POINTER(ctypes.c_void_p)]),
     "dsd_kv8_sparse_destroy": (ctypes.c_int, [ctypes.c_void_p]),
@@ -989,6 +994,17 @@ class Kv8Cache:
         """Attention of a request's several query tokens, each over the tokens
         up to its own (dsd_kv8_attend_prompt)."""
         status = self._lib.dsd_kv8_attend_prompt(
+            self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, out, out_stride, scale,
+            workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def attend_cross(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int,
+                     out: int, out_stride: int, scale: float = 0.0, workspace: int = 0,
+                     workspace_bytes: int = 0, fail: int = 0, stream: int = 0) -> None:
+        """Attention of a request's several query tokens, each over all tokens of
+        its listed pages (dsd_kv8_attend_cross)."""
+        status = self._lib.dsd_kv8_attend_cross(
             self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, out, out_stride, scale,
             workspace, workspace_bytes, fail, stream)
         if status:

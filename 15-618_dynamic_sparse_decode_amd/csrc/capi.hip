@@ -3139,8 +3139,9 @@ struct dsd_kv8 {
 
 namespace {
 
-// A batch's sizes and pointers, as the calls need them (tokens: with new ones).
-void RequireKv8Batch(const dsd_kv8* cache, const dsd_kv8_batch* b, bool tokens) {
+// A batch's sizes and pointers, as the calls need them (tokens: rows of several a
+// request; past: behind others).
+void RequireKv8Batch(const dsd_kv8* cache, const dsd_kv8_batch* b, bool tokens, bool past) {
   Require(cache != nullptr && b != nullptr, "cache and batch must be non-null");
   cache->RequireCurrent();
   Require(b->batch >= 0 && b->tokens >= 0 && b->max_tokens >= 0 && b->max_pages >= 0 &&
@@ -3159,8 +3160,9 @@ void RequireKv8Batch(const dsd_kv8* cache, const dsd_kv8_batch* b, bool tokens) 
   // (the kernels read page 0 in place of none)
   Require(b->total_pages == 0 || cache->view.capacity > 0, "the cache holds no page");
   if (tokens) {
-    Require(b->token_offsets != nullptr && b->past_tokens != nullptr,
-            "token_offsets and past_tokens must be non-null");
+    Require(b->token_offsets != nullptr && (!past || b->past_tokens != nullptr),
+            past ? "token_offsets and past_tokens must be non-null"
+                 : "token_offsets must be non-null");
     Require(b->tokens == 0 || b->max_tokens > 0, "max_tokens must be positive");
   }
 }
@@ -3192,16 +3194,19 @@ void RequireQueryRows(const dsd_kv8_batch* b, int q_heads) {
           "max_tokens * num_q_heads must fit 31 bits");
 }
 
-int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, bool causal, int type, int num_q_heads,
+enum class Rows { kOne, kCausal, kAll };  // of a request, and what they see
+
+int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, Rows rows, int type, int num_q_heads,
               const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
               void* workspace, size_t workspace_bytes, unsigned long long* d_fail, void* stream) {
   return Guard([&] {
-    RequireKv8Batch(cache, batch, causal);
+    const bool many = rows != Rows::kOne;
+    RequireKv8Batch(cache, batch, many, rows == Rows::kCausal);
     const size_t size = TypeSize(type);
     RequireHeads(cache, num_q_heads);
     Require(num_q_heads > 0, "num_q_heads must be positive");
-    if (causal) RequireQueryRows(batch, num_q_heads);
-    if (batch->batch == 0 || (causal && batch->tokens == 0)) return;
+    if (many) RequireQueryRows(batch, num_q_heads);
+    if (batch->batch == 0 || (many && batch->tokens == 0)) return;
     RequireRows(cache, q, q_stride, num_q_heads, size);
     RequireRows(cache, out, out_stride, num_q_heads, size);
     Require(std::isfinite(scale), "scale must be finite");
@@ -3212,7 +3217,8 @@ int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, bool causal, int type,
     a.b = *batch;
     a.type = type;
     a.q_heads = num_q_heads;
-    a.causal = causal;
+    a.many = many;
+    a.causal = rows == Rows::kCausal;
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;
@@ -3291,6 +3297,7 @@ int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_p
     dsdk::PreloadKv8Append(v);
     dsdk::PreloadKv8Attend(v);
     dsdk::PreloadKv8Prompt(v);
+    dsdk::PreloadKv8Cross(v);
     *out_cache = cache.release();
   });
 }
@@ -3381,7 +3388,7 @@ int dsd_kv8_append(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num
                    const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride,
                    unsigned long long* d_fail, void* stream) {
   return Guard([&] {
-    RequireKv8Batch(cache, batch, true);
+    RequireKv8Batch(cache, batch, true, true);
     const size_t size = TypeSize(type);
     RequireHeads(cache, num_q_heads);
     if (batch->batch == 0 || batch->tokens == 0) return;
@@ -3415,7 +3422,7 @@ int dsd_kv8_attend(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num
                    const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
                    void* workspace, size_t workspace_bytes, unsigned long long* d_fail,
                    void* stream) {
-  return AttendKv8(cache, batch, false, type, num_q_heads, q, q_stride, out, out_stride, scale,
+  return AttendKv8(cache, batch, Rows::kOne, type, num_q_heads, q, q_stride, out, out_stride, scale,
                    workspace, workspace_bytes, d_fail, stream);
 }
 
@@ -3423,7 +3430,15 @@ int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, 
                           const void* q, int64_t q_stride, void* out, int64_t out_stride,
                           float scale, void* workspace, size_t workspace_bytes,
                           unsigned long long* d_fail, void* stream) {
-  return AttendKv8(cache, batch, true, type, num_q_heads, q, q_stride, out, out_stride, scale,
+  return AttendKv8(cache, batch, Rows::kCausal, type, num_q_heads, q, q_stride, out, out_stride, scale,
+                   workspace, workspace_bytes, d_fail, stream);
+}
+
+int dsd_kv8_attend_cross(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num_q_heads,
+                         const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                         float scale, void* workspace, size_t workspace_bytes,
+                         unsigned long long* d_fail, void* stream) {
+  return AttendKv8(cache, batch, Rows::kAll, type, num_q_heads, q, q_stride, out, out_stride, scale,
                    workspace, workspace_bytes, d_fail, stream);
 }
 

@@ -1,5 +1,5 @@
 // kv8.h -- the 8-bit paged cache (dsd_kv8_*): launch interface of
-// kv8_append.hip, kv8_attend.hip and kv8_prompt.hip.
+// kv8_append.hip, kv8_attend.hip, kv8_prompt.hip and kv8_cross.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -55,7 +55,8 @@ struct Kv8AttendArgs {
   dsd_kv8_batch b = {};
   int type = 0;
   int q_heads = 0;
-  bool causal = false;  // several query tokens a request, each over what precedes it
+  bool many = false;    // several query tokens a request
+  bool causal = false;  // (many:) each over what precedes it, else over all of the list
   const void* q = nullptr;
   void* out = nullptr;
   int64_t q_stride = 0, out_stride = 0;  // elements
@@ -65,8 +66,9 @@ struct Kv8AttendArgs {
   FailReport fail;
 };
 void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream);
-// The form of it for many rows (kv8_prompt.hip).
+// The forms of it for many rows (kv8_prompt.hip: causal; kv8_cross.hip: not).
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream);
+void LaunchKv8Cross(const Kv8AttendArgs& a, hipStream_t stream);
 size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 // Each key head's queries summed, in order, in float32: sums[batch][heads * dim].
@@ -76,5 +78,6 @@ void LaunchKv8GroupQueries(const Kv8View& c, int batch, int type, int q_heads, c
 void PreloadKv8Append(const Kv8View& c);
 void PreloadKv8Attend(const Kv8View& c);
 void PreloadKv8Prompt(const Kv8View& c);
+void PreloadKv8Cross(const Kv8View& c);
 
 }  // namespace dsdk

@@ -84,6 +84,8 @@ __device__ __forceinline__ bool FindSpan(const Kv8AttendArgs& a, int group, int 
   bool ok;
   if (a.causal) {
     ok = Kv8ReadTokens(a.b, r, a.c.page, &s->q);
+  } else if (a.many) {
+    ok = Kv8ReadRows(a.b, r, &s->q) && Kv8ReadList(a.b, r, &s->q);
   } else {
     ok = Kv8ReadList(a.b, r, &s->q);
     s->q.row0 = r;
@@ -92,7 +94,7 @@ __device__ __forceinline__ bool FindSpan(const Kv8AttendArgs& a, int group, int 
   if (!ok || s->q.pages > 0x7fffff00 / a.c.page) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailShape);
     // (a decode request still gets its zeros)
-    if (a.causal) return false;
+    if (a.causal || a.many) return false;
     s->q.pages = 0;
   }
   s->rows = s->q.n * group;
@@ -214,9 +216,18 @@ struct Plan {
   int piece = 1;     // groups of 64 tokens in a piece
   float* part = nullptr;    // [batch][key heads][rows][pieces][dim]
   PieceStats* stats = nullptr;  // [batch][key heads][rows][pieces]
+  // Of pieces that a later launch joins with others', whatever their number: the
+  // slots are [rows of q][key heads][group][stride], this list's from `base` on.
+  int stride = 0;
+  int base = 0;
 };
 __device__ __forceinline__ int64_t PartSlot(const Plan& p, int heads, int r, int head, int row) {
   return ((static_cast<int64_t>(r) * heads + head) * p.rows + row) * p.pieces;
+}
+__device__ __forceinline__ int64_t JoinSlot(const Plan& p, int heads, int row0, int head, int row) {
+  const int token = row / p.group;
+  return ((static_cast<int64_t>(row0 + token) * heads + head) * p.group + row - token * p.group) *
+             p.stride + p.base;
 }
 // The pieces that a span's list is cut into.
 __device__ __forceinline__ int Pieces(const Plan& p, const Span& s) {

@@ -55,6 +55,15 @@ __device__ __forceinline__ bool Kv8ReadTokens(const dsd_kv8_batch& b, int r, int
          q->past <= 0x7fffffff - q->n;
 }
 
+// Rows alone: their request sees all of its list.
+__device__ __forceinline__ bool Kv8ReadRows(const dsd_kv8_batch& b, int r, Kv8Request* q) {
+  q->row0 = b.token_offsets[r];
+  const int end = b.token_offsets[r + 1];
+  if (q->row0 < 0 || end < q->row0 || end > b.tokens || end - q->row0 > b.max_tokens) return false;
+  q->n = end - q->row0;
+  return true;
+}
+
 // Orders one wave's LDS writes before its reads of what other lanes wrote.
 __device__ __forceinline__ void WaveLdsFence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -763,8 +763,17 @@ int dsd_kv8_attend_prompt(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
                           void* out, int64_t out_stride, float scale,
                           void* workspace, size_t workspace_bytes,
                           unsigned long long* d_fail, void* stream);
-/* Workspace of dsd_kv8_attend and dsd_kv8_attend_prompt for any batch of at most
- * these sizes (the pointers are not read). */
+/* The same where every query token of a request sees all tokens of its list's pages
+ * (token_counts each): cross attention of a decoder's tokens to an encoder's states, of
+ * another number than the tokens.  Query token i of request r is row token_offsets[r] +
+ * i; past_tokens is not read.  A request whose list holds no token gets zeros. */
+int dsd_kv8_attend_cross(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
+                         int num_q_heads, const void* q, int64_t q_stride,
+                         void* out, int64_t out_stride, float scale,
+                         void* workspace, size_t workspace_bytes,
+                         unsigned long long* d_fail, void* stream);
+/* Workspace of dsd_kv8_attend, dsd_kv8_attend_prompt and dsd_kv8_attend_cross for any
+ * batch of at most these sizes (the pointers are not read). */
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                             int num_q_heads, size_t* bytes);
 
