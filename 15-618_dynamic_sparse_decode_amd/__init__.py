@@ -247,6 +247,13 @@ _SIGNATURES = {
                              + [ctypes.c_void_p, ctypes.c_int64] * 2
                              + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
                              + [ctypes.c_void_p] * 2),
+    "dsd_kv8_attend_weigh": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                            ctypes.c_int, ctypes.c_int]
+                             + [ctypes.c_void_p, ctypes.c_int64] * 2
+                             + [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]
+                             + [ctypes.c_void_p] * 2),
+    "dsd_kv8_weigh_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                                     ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "dsd_kv8_sparse_create": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int] * 4
                               + [ctypes.POINTER(ctypes.c_void_p)]),
     "dsd_kv8_sparse_destroy": (ctypes.c_int, [ctypes.c_void_p]),
@@ -1009,6 +1016,24 @@ class Kv8Cache:
             workspace, workspace_bytes, fail, stream)
         if status:
             _check(status)
+
+    def attend_weigh(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int,
+                     out: int, out_stride: int, scale: float = 0.0, weights: int = 0,
+                     workspace: int = 0, workspace_bytes: int = 0, fail: int = 0,
+                     stream: int = 0) -> None:
+        """attend, and each token's softmax weight added to weights [capacity][kv
+        heads][page size] (dsd_kv8_attend_weigh)."""
+        status = self._lib.dsd_kv8_attend_weigh(
+            self.handle, batch.pointer, dtype, num_q_heads, q, q_stride, out, out_stride, scale,
+            weights, workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def weigh_workspace_bytes(self, batch: Kv8Batch, num_q_heads: int) -> int:
+        out = ctypes.c_size_t()
+        _check(self._lib.dsd_kv8_weigh_workspace_bytes(self.handle, batch.pointer, num_q_heads,
+                                                       ctypes.byref(out)))
+        return out.value
 
     def workspace_bytes(self, batch: Kv8Batch, num_q_heads: int) -> int:
         out = ctypes.c_size_t()

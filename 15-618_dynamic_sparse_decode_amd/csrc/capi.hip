@@ -3194,39 +3194,62 @@ void RequireQueryRows(const dsd_kv8_batch* b, int q_heads) {
           "max_tokens * num_q_heads must fit 31 bits");
 }
 
+// What a workspace query reads.
+void RequireSizes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int q_heads, const size_t* bytes) {
+  Require(cache != nullptr && batch != nullptr && bytes != nullptr,
+          "cache, batch and bytes must be non-null");
+  Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0 &&
+              batch->total_pages >= 0,
+          "sizes must be non-negative");
+  RequireHeads(cache, q_heads);
+  RequireQueryRows(batch, q_heads);
+}
+
 enum class Rows { kOne, kCausal, kAll };  // of a request, and what they see
+
+// A checked call's arguments; false: nothing to do.
+bool ReadAttend(dsd_kv8* cache, const dsd_kv8_batch* batch, Rows rows, int type, int num_q_heads,
+                const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
+                void* workspace, size_t workspace_bytes, unsigned long long* d_fail,
+                dsdk::Kv8AttendArgs* a) {
+  const bool many = rows != Rows::kOne;
+  RequireKv8Batch(cache, batch, many, rows == Rows::kCausal);
+  const size_t size = TypeSize(type);
+  RequireHeads(cache, num_q_heads);
+  Require(num_q_heads > 0, "num_q_heads must be positive");
+  if (many) RequireQueryRows(batch, num_q_heads);
+  if (batch->batch == 0 || (many && batch->tokens == 0)) return false;
+  RequireRows(cache, q, q_stride, num_q_heads, size);
+  RequireRows(cache, out, out_stride, num_q_heads, size);
+  Require(std::isfinite(scale), "scale must be finite");
+  Require(workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+          "the workspace must be 16-byte aligned");
+  a->c = cache->view;
+  a->b = *batch;
+  a->type = type;
+  a->q_heads = num_q_heads;
+  a->many = many;
+  a->causal = rows == Rows::kCausal;
+  a->q = q;
+  a->out = out;
+  a->q_stride = q_stride;
+  a->out_stride = out_stride;
+  a->scale = scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->view.dim));
+  a->workspace = workspace;
+  a->workspace_bytes = workspace != nullptr ? workspace_bytes : 0;
+  a->fail.word = d_fail;
+  return true;
+}
 
 int AttendKv8(dsd_kv8* cache, const dsd_kv8_batch* batch, Rows rows, int type, int num_q_heads,
               const void* q, int64_t q_stride, void* out, int64_t out_stride, float scale,
               void* workspace, size_t workspace_bytes, unsigned long long* d_fail, void* stream) {
   return Guard([&] {
-    const bool many = rows != Rows::kOne;
-    RequireKv8Batch(cache, batch, many, rows == Rows::kCausal);
-    const size_t size = TypeSize(type);
-    RequireHeads(cache, num_q_heads);
-    Require(num_q_heads > 0, "num_q_heads must be positive");
-    if (many) RequireQueryRows(batch, num_q_heads);
-    if (batch->batch == 0 || (many && batch->tokens == 0)) return;
-    RequireRows(cache, q, q_stride, num_q_heads, size);
-    RequireRows(cache, out, out_stride, num_q_heads, size);
-    Require(std::isfinite(scale), "scale must be finite");
-    Require(workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
-            "the workspace must be 16-byte aligned");
     dsdk::Kv8AttendArgs a;
-    a.c = cache->view;
-    a.b = *batch;
-    a.type = type;
-    a.q_heads = num_q_heads;
-    a.many = many;
-    a.causal = rows == Rows::kCausal;
-    a.q = q;
-    a.out = out;
-    a.q_stride = q_stride;
-    a.out_stride = out_stride;
-    a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->view.dim));
-    a.workspace = workspace;
-    a.workspace_bytes = workspace != nullptr ? workspace_bytes : 0;
-    a.fail.word = d_fail;
+    if (!ReadAttend(cache, batch, rows, type, num_q_heads, q, q_stride, out, out_stride, scale,
+                    workspace, workspace_bytes, d_fail, &a)) {
+      return;
+    }
     dsdk::LaunchKv8Attend(a, reinterpret_cast<hipStream_t>(stream));
   });
 }
@@ -3298,6 +3321,7 @@ int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_p
     dsdk::PreloadKv8Attend(v);
     dsdk::PreloadKv8Prompt(v);
     dsdk::PreloadKv8Cross(v);
+    dsdk::PreloadKv8Weigh(v);
     *out_cache = cache.release();
   });
 }
@@ -3445,13 +3469,34 @@ int dsd_kv8_attend_cross(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, i
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int num_q_heads,
                             size_t* bytes) {
   return Guard([&] {
-    Require(cache != nullptr && batch != nullptr && bytes != nullptr,
-            "cache, batch and bytes must be non-null");
-    Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0,
-            "sizes must be non-negative");
-    RequireHeads(cache, num_q_heads);
-    RequireQueryRows(batch, num_q_heads);
+    RequireSizes(cache, batch, num_q_heads, bytes);
     *bytes = num_q_heads > 0 ? dsdk::Kv8WorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
+  });
+}
+
+int dsd_kv8_attend_weigh(dsd_kv8* cache, const dsd_kv8_batch* batch, int type, int num_q_heads,
+                         const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                         float scale, float* weights, void* workspace, size_t workspace_bytes,
+                         unsigned long long* d_fail, void* stream) {
+  return Guard([&] {
+    dsdk::Kv8AttendArgs a;
+    if (!ReadAttend(cache, batch, Rows::kOne, type, num_q_heads, q, q_stride, out, out_stride,
+                    scale, workspace, workspace_bytes, d_fail, &a)) {
+      return;
+    }
+    Require(weights != nullptr && reinterpret_cast<uintptr_t>(weights) % sizeof(float) == 0,
+            "weights must be non-null and aligned");
+    Require(a.workspace_bytes >= dsdk::Kv8WeighBytes(a.c, a.b, num_q_heads),
+            "the workspace is smaller than dsd_kv8_weigh_workspace_bytes");
+    dsdk::LaunchKv8Weigh(a, weights, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                                  int num_q_heads, size_t* bytes) {
+  return Guard([&] {
+    RequireSizes(cache, batch, num_q_heads, bytes);
+    *bytes = num_q_heads > 0 ? dsdk::Kv8WeighWorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
   });
 }
 

@@ -69,6 +69,10 @@ void LaunchKv8Attend(const Kv8AttendArgs& a, hipStream_t stream);
 // The forms of it for many rows (kv8_prompt.hip: causal; kv8_cross.hip: not).
 void LaunchKv8Prompt(const Kv8AttendArgs& a, hipStream_t stream);
 void LaunchKv8Cross(const Kv8AttendArgs& a, hipStream_t stream);
+// kv8_weigh.hip; the first: what this batch's call needs.
+size_t Kv8WeighBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
+size_t Kv8WeighWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
+void LaunchKv8Weigh(const Kv8AttendArgs& a, float* weights, hipStream_t stream);
 size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 // Each key head's queries summed, in order, in float32: sums[batch][heads * dim].
@@ -79,5 +83,6 @@ void PreloadKv8Append(const Kv8View& c);
 void PreloadKv8Attend(const Kv8View& c);
 void PreloadKv8Prompt(const Kv8View& c);
 void PreloadKv8Cross(const Kv8View& c);
+void PreloadKv8Weigh(const Kv8View& c);
 
 }  // namespace dsdk

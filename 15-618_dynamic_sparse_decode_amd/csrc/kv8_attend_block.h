@@ -2,6 +2,8 @@
 // workgroup of the 8-bit cache's attention kernels for few rows does.
 #pragma once
 
+#include <algorithm>
+
 #include "kv8_attend.h"
 
 namespace dsdk {
@@ -18,10 +20,12 @@ constexpr float kMostFactor = 100.0f;  // powers of two beyond which weights are
 // operand of O^T = V^T P^T as they stand (the order of a product's inner index
 // is free), whose first operand, 16 tokens of one dim, is one load of the
 // values' layout.  No number crosses lanes but for the maxima.
+// kJoin: a later launch joins the piece with others.  kWeigh: logits (times log2 e) go
+// to `logits` as well, [query heads][places of all lists], and the sums to p.stats.
 // kDim: head_dim where it is 64 * NU (no bounds tests), else 0.
-template <typename T, int FMT, int NU, int kDim, int W, bool kJoin>
+template <typename T, int FMT, int NU, int kDim, int W, bool kJoin, bool kWeigh = false>
 __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& p, int unit, int r,
-                                            int piece, float* lds) {
+                                            int piece, float* lds, float* logits = nullptr) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>, NT = 4 * NU;
   const Kv8View& c = a.c;
   const int D = kDim > 0 ? kDim : c.dim, tiles = kDim > 0 ? NT : D / 16;
@@ -173,6 +177,14 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
         }
       }
       const float f = fmaxf(to_logit * now.key_scale, kKv8Tiny);
+      if constexpr (kWeigh) {
+        if (there && 4 * grp + g < s.chunks) {
+          float* to = logits + static_cast<int64_t>(head * p.group + row) * a.b.total_pages * c.page +
+                      static_cast<int64_t>(s.q.list) * c.page + (4 * grp + g) * 16;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) *reinterpret_cast<F32x4*>(to + 4 * t) = x[t] * f;
+        }
+      }
       float most = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -352,6 +364,9 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
       }
     }
     const float x = most - kWeightBits;  // o lacks 2^x
+    if (kWeigh && pieces == 1 && d == 0) {
+      p.stats[PartSlot(p, c.heads, r, head, at)] = {peak, some ? sum : -1.0f, x};
+    }
     if (!kJoin && pieces == 1) {
       const int tok = at / p.group;
       T* out = static_cast<T*>(a.out) + (s.q.row0 + tok) * a.out_stride +
@@ -375,6 +390,47 @@ inline size_t AttendLdsBytes(int dim) {
   const size_t joined = sizeof(float) * (48 * kAttendWaves + kAttendWaves * 16 * (dim + 4));
   const size_t staged = sizeof(PageInfo) * kStage;
   return joined > staged ? joined : staged;
+}
+
+// Two workgroups fit a CU (registers), 512 the chip.
+constexpr int kAttendTarget = 512;
+
+// Pieces that lists of so many groups are cut into, `units` workgroups to a piece.
+// In us: a launch about 5.5; a step, a group for each of the four waves, 1.15 and
+// more where workgroups share the memory's rate, up to 5.9 TB/s; the merge, with
+// its launch, 3.5 to 5.9.  Heads of 128 (32 / 8), bf16, us whole and in pieces:
+// one of 512 tokens 8.2 and 10.3, of 2000 15.0 and 10.4, of 32000 158 and 22; 16
+// of 1000 12.9 and 16.8, of 2000 17.7 and 19.9, of 8000 64 and 56; 32 of 500 11.7
+// and 17.1.  Lists are seldom equally long, and pieces end more evenly: of choices
+// within 3% the one with most pieces.
+inline int64_t PiecesWanted(int64_t groups, int64_t most, int64_t units, int dim) {
+  const int64_t steps = (groups + kAttendWaves - 1) / kAttendWaves;
+  const double share = 8.7e-5 * dim;  // us of a step's bytes of one workgroup
+  auto cost = [&](int64_t n) {
+    const double workgroups = static_cast<double>(units * n);
+    const double step = std::max(1.15 + 0.6 * share * workgroups, share * workgroups);
+    const double merge = n > 1 ? 3.5 + 2.4 * std::min(1.0, workgroups / 256) : 0.0;
+    return 5.5 + static_cast<double>((steps + n - 1) / n) * step + merge;
+  };
+  most = std::min(most, steps);
+  double best = cost(1);
+  for (int64_t n = 2; n <= most; ++n) best = std::min(best, cost(n));
+  int64_t n = most;
+  while (n > 1 && cost(n) > 1.03 * best) --n;
+  return n;
+}
+
+inline Plan AttendPlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, bool many) {
+  Plan p;
+  p.group = q_heads / c.heads;
+  p.rows = static_cast<int64_t>(many ? b.max_tokens : 1) * p.group;
+  p.block = 16;
+  p.blocks = static_cast<int>((p.rows + p.block - 1) / p.block);
+  const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
+  const int64_t groups = ListGroups(c, b);
+  const int64_t most = std::min<int64_t>(kAttendTarget / std::max<int64_t>(units, 1), kMostPieces);
+  CutLists(&p, groups, PiecesWanted(groups, std::max<int64_t>(most, 1), units, c.dim), kAttendWaves);
+  return p;
 }
 
 }  // namespace

@@ -1,0 +1,176 @@
+// kv8_weigh.hip -- dsd_kv8_attend_weigh (gfx950): dsd_kv8_attend, and each token's softmax
+// weight, summed over the query heads of its key head, added to the caller's array.
+//
+// Mathematics.  A weight is 2^(s - m) / l with s the logit in the log2 domain and m, l
+// its row's maximum and sum, which are known once the whole list has been read.  Reading
+// the keys a second time would be half of the bytes again; the logits are 4 bytes a token
+// and query head beside 2 dim / group of codes (a sixteenth at 4 heads of 128), so the
+// attention writes them to the workspace and a second launch turns them into weights.
+// Sums over a group's heads are float32, in order; a token's own sum takes one atomic
+// addition (a page that several requests list gets all of theirs, in any order).
+#include "kv8_attend_block.h"
+
+namespace dsdk {
+namespace {
+
+// Grid (key heads * row tiles, batch, pieces).
+template <typename T, int FMT, int NU, int kDim>
+__global__ __launch_bounds__(kAttendWaves* kWave, NU <= 2 ? 2 : 1) void Kv8AttendLogitsKernel(
+    Kv8AttendArgs a, Plan p, float* logits) {
+  extern __shared__ __align__(16) float lds[];
+  AttendBlock<T, FMT, NU, kDim, kAttendWaves, false, true>(a, p, blockIdx.x, blockIdx.y, blockIdx.z,
+                                                           lds, logits);
+}
+
+// Grid (blocks of 256 places, key heads, batch); a block takes every gridDim.x-th 256 of
+// its list.
+constexpr int kRowTile = 64;
+__global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, const float* logits,
+                                                      float* weights) {
+  __shared__ float row_base[kRowTile], row_inv[kRowTile];
+  const Kv8View& c = a.c;
+  const int r = blockIdx.z, head = blockIdx.y;
+  Span s;
+  if (!FindSpan(a, p.group, r, 0, p.group, &s)) return;
+  const int places = s.chunks * 16;
+  if (static_cast<int>(blockIdx.x) * 256 >= places) return;
+  const int pieces = Pieces(p, s);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int64_t row_places = static_cast<int64_t>(a.b.total_pages) * c.page;
+  const float* from = logits + static_cast<int64_t>(head) * p.group * row_places +
+                      static_cast<int64_t>(s.q.list) * c.page;
+  for (int row0 = 0; row0 < p.group; row0 += kRowTile) {
+    const int rows = min(kRowTile, p.group - row0);
+    __syncthreads();
+    for (int i = wave; i < rows; i += 4) {
+      PieceStats st = {-INFINITY, -1.0f, 0.0f};
+      if (lane < pieces) st = p.stats[PartSlot(p, c.heads, r, head, row0 + i) + lane];
+      const bool some = !(st.l < 0.0f);
+      float peak = some ? st.m : -INFINITY;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+      const float base = peak == -INFINITY ? 0.0f : peak;
+      float sum = some ? st.l * Exp2(st.m - base) : 0.0f;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+      if (lane == 0) {
+        row_base[i] = base;
+        row_inv[i] = 1.0f / sum;
+      }
+    }
+    __syncthreads();
+    for (int at = blockIdx.x * 256 + threadIdx.x; at < places; at += gridDim.x * 256) {
+      const int slot = at / c.page;
+      const int page = a.b.page_ids[s.q.list + slot];
+      if (!InPool(page, c.capacity) || at - slot * c.page >= c.token_counts[page]) continue;
+      float w = 0.0f;
+      const float* x = from + row0 * row_places + at;
+#pragma unroll 4
+      for (int i = 0; i < rows; ++i) w = fmaf(Exp2(x[i * row_places] - row_base[i]), row_inv[i], w);
+      unsafeAtomicAdd(weights + (static_cast<int64_t>(page) * c.heads + head) * c.page + at -
+                          slot * c.page, w);
+    }
+  }
+}
+
+// Calls f with the kernel of a head size.
+template <typename T, int FMT, typename F>
+void WithKernel(int dim, F&& f) {
+  if (dim == 64) return f(Kv8AttendLogitsKernel<T, FMT, 1, 64>);
+  if (dim < 64) return f(Kv8AttendLogitsKernel<T, FMT, 1, 0>);
+  if (dim == 128) return f(Kv8AttendLogitsKernel<T, FMT, 2, 128>);
+  if (dim < 128) return f(Kv8AttendLogitsKernel<T, FMT, 2, 0>);
+  return f(Kv8AttendLogitsKernel<T, FMT, 4, 0>);
+}
+
+// The workspace: parts (of lists in pieces), stats, logits.
+size_t PartBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
+  return p.pieces == 1 ? 0 : PlanSlots(c, b, p) * sizeof(float) * c.dim;
+}
+size_t StatsBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
+  return (PlanSlots(c, b, p) * sizeof(PieceStats) + 15) / 16 * 16;
+}
+size_t LogitBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  return static_cast<size_t>(q_heads) * b.total_pages * c.page * sizeof(float);
+}
+
+template <typename T, int FMT>
+void Launch(const Kv8AttendArgs& a, float* weights, hipStream_t stream) {
+  Plan p = AttendPlan(a.c, a.b, a.q_heads, false);
+  unsigned char* space = static_cast<unsigned char*>(a.workspace);
+  p.part = reinterpret_cast<float*>(space);
+  space += PartBytes(a.c, a.b, p);
+  p.stats = reinterpret_cast<PieceStats*>(space);
+  space += StatsBytes(a.c, a.b, p);
+  float* logits = reinterpret_cast<float*>(space);
+  const dim3 grid(a.c.heads * p.blocks, a.b.batch, p.pieces);
+  WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
+    kernel<<<grid, kAttendWaves * kWave, AttendLdsBytes(a.c.dim), stream>>>(a, p, logits);
+  });
+  DSD_HIP_CHECK(hipGetLastError());
+  Merge<T>(a, p, stream);
+  const int64_t blocks = (static_cast<int64_t>(a.b.max_pages) * a.c.page + 255) / 256;
+  const dim3 over(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(blocks, 1), 65536)),
+                  a.c.heads, a.b.batch);
+  Kv8WeighKernel<<<over, 256, 0, stream>>>(a, p, logits, weights);
+  DSD_HIP_CHECK(hipGetLastError());
+}
+
+template <typename T>
+void LaunchType(const Kv8AttendArgs& a, float* weights, hipStream_t stream) {
+  a.c.format == DSD_KV8_INT8 ? Launch<T, DSD_KV8_INT8>(a, weights, stream)
+                             : Launch<T, DSD_KV8_E4M3>(a, weights, stream);
+}
+
+template <typename T, int FMT>
+void PreloadDim(const Kv8View& c) {
+  WithKernel<T, FMT>(c.dim, [&](auto kernel) {
+    PreloadKernel(kernel);
+    DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(AttendLdsBytes(c.dim))));
+  });
+}
+
+template <typename T>
+void PreloadType(const Kv8View& c) {
+  c.format == DSD_KV8_INT8 ? PreloadDim<T, DSD_KV8_INT8>(c) : PreloadDim<T, DSD_KV8_E4M3>(c);
+  PreloadKernel(Kv8MergeKernel<T>);
+  PreloadKernel(Kv8MergeRowsKernel<T>);
+}
+
+}  // namespace
+
+size_t Kv8WeighBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  if (b.batch == 0) return 0;
+  const Plan p = AttendPlan(c, b, q_heads, false);
+  return PartBytes(c, b, p) + StatsBytes(c, b, p) + LogitBytes(c, b, q_heads);
+}
+
+// Of any batch of at most these sizes: pieces where a launch would have few workgroups,
+// a row's sums where it has many.
+size_t Kv8WeighWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  if (b.batch == 0) return 0;
+  Plan p = AttendPlan(c, b, q_heads, false);
+  const size_t parts = MostPartBytes(c, p, kAttendTarget);
+  p.pieces = 1;
+  return (parts + 15) / 16 * 16 + StatsBytes(c, b, p) + LogitBytes(c, b, q_heads);
+}
+
+void PreloadKv8Weigh(const Kv8View& c) {
+  PreloadType<float>(c);
+  PreloadType<__bf16>(c);
+  PreloadType<_Float16>(c);
+  PreloadKernel(Kv8WeighKernel);
+}
+
+void LaunchKv8Weigh(const Kv8AttendArgs& a, float* weights, hipStream_t stream) {
+  if (a.b.batch == 0) return;
+  switch (a.type) {
+    case DSD_TYPE_F32: return LaunchType<float>(a, weights, stream);
+    case DSD_TYPE_BF16: return LaunchType<__bf16>(a, weights, stream);
+    default: return LaunchType<_Float16>(a, weights, stream);
+  }
+}
+
+}  // namespace dsdk

@@ -777,6 +777,23 @@ int dsd_kv8_attend_cross(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                             int num_q_heads, size_t* bytes);
 
+/* dsd_kv8_attend, and how much each token weighed: weights[page][key head][token of the
+ * page] (float32, [capacity][num_kv_heads][page_size], device memory) grows by the token's
+ * softmax weight, summed over the query heads of its key head.  Places that hold no token
+ * stay as they are; a page that a list names twice, or lists of several requests name, gets
+ * every one's (in any order, so such sums' last places may change from run to run; all
+ * others are the same from run to run).  Where a row's weights are NaN so are its tokens'.
+ * The sums are the caller's: it clears a page's when it hands the page out.
+ * workspace: dsd_kv8_weigh_workspace_bytes (total_pages counts) of device memory, 16-byte
+ * aligned, as dsd_kv8_attend's but required. */
+int dsd_kv8_attend_weigh(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
+                         int num_q_heads, const void* q, int64_t q_stride,
+                         void* out, int64_t out_stride, float scale,
+                         float* weights, void* workspace, size_t workspace_bytes,
+                         unsigned long long* d_fail, void* stream);
+int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                                  int num_q_heads, size_t* bytes);
+
 /* The sparse step (dsd_sparse_run_batch_device) over an 8-bit cache that keeps
  * summaries: every candidate page scored through its summary, the top_k pages
  * of each request kept, attention over those.  A page's score is the sum over
