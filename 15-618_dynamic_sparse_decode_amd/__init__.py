@@ -254,6 +254,11 @@ _SIGNATURES = {
                              + [ctypes.c_void_p] * 2),
     "dsd_kv8_weigh_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
                                                      ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "dsd_kv8_evict": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs)]
+                      + [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2 + [ctypes.c_int]
+                      + [ctypes.c_void_p] * 3 + [ctypes.c_size_t] + [ctypes.c_void_p] * 2),
+    "dsd_kv8_evict_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                                     ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "dsd_kv8_sparse_create": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int] * 4
                               + [ctypes.POINTER(ctypes.c_void_p)]),
     "dsd_kv8_sparse_destroy": (ctypes.c_int, [ctypes.c_void_p]),
@@ -1032,6 +1037,23 @@ class Kv8Cache:
     def weigh_workspace_bytes(self, batch: Kv8Batch, num_q_heads: int) -> int:
         out = ctypes.c_size_t()
         _check(self._lib.dsd_kv8_weigh_workspace_bytes(self.handle, batch.pointer, num_q_heads,
+                                                       ctypes.byref(out)))
+        return out.value
+
+    def evict(self, batch: Kv8Batch, keep: int, first: int, recent: int, weights: int,
+              new_page_ids: int, new_stride: int, new_page_counts: int, kept: int,
+              workspace: int = 0, workspace_bytes: int = 0, fail: int = 0, stream: int = 0) -> None:
+        """Each list cut to `keep` tokens a key head: the first, the last and those
+        that weighed most, moved to new pages (dsd_kv8_evict)."""
+        status = self._lib.dsd_kv8_evict(
+            self.handle, batch.pointer, keep, first, recent, weights, new_page_ids, new_stride,
+            new_page_counts, kept, workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def evict_workspace_bytes(self, batch: Kv8Batch, keep: int) -> int:
+        out = ctypes.c_size_t()
+        _check(self._lib.dsd_kv8_evict_workspace_bytes(self.handle, batch.pointer, keep,
                                                        ctypes.byref(out)))
         return out.value
 

@@ -3322,6 +3322,7 @@ int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_p
     dsdk::PreloadKv8Prompt(v);
     dsdk::PreloadKv8Cross(v);
     dsdk::PreloadKv8Weigh(v);
+    dsdk::PreloadKv8Evict(v);
     *out_cache = cache.release();
   });
 }
@@ -3497,6 +3498,56 @@ int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* bat
   return Guard([&] {
     RequireSizes(cache, batch, num_q_heads, bytes);
     *bytes = num_q_heads > 0 ? dsdk::Kv8WeighWorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
+  });
+}
+
+int dsd_kv8_evict(dsd_kv8* cache, const dsd_kv8_batch* batch, int keep, int first, int recent,
+                  float* weights, const int* new_page_ids, int new_stride, int* new_page_counts,
+                  int* kept, void* workspace, size_t workspace_bytes, unsigned long long* d_fail,
+                  void* stream) {
+  return Guard([&] {
+    RequireKv8Batch(cache, batch, false, false);
+    Require(keep >= 0 && first >= 0 && recent >= 0, "keep, first and recent must be non-negative");
+    Require(static_cast<int64_t>(first) + recent <= keep, "first + recent must be at most keep");
+    if (batch->batch == 0) return;
+    const dsdk::Kv8View& c = cache->view;
+    const int64_t pages = (static_cast<int64_t>(keep) + c.page - 1) / c.page;
+    Require(new_stride >= pages, "new_stride must hold the pages of keep tokens");
+    // (a launch's threads in one direction are counted in 32 bits)
+    Require(pages * c.heads <= 0x400000, "keep is too large");
+    Require(weights != nullptr && reinterpret_cast<uintptr_t>(weights) % sizeof(float) == 0,
+            "weights must be non-null and aligned");
+    Require(new_page_counts != nullptr, "new_page_counts must be non-null");
+    Require(keep == 0 || (new_page_ids != nullptr && kept != nullptr),
+            "new_page_ids and kept must be non-null");
+    Require(keep == 0 || c.capacity > 0, "the cache holds no page");
+    Require(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+            "the workspace must be non-null and 16-byte aligned");
+    Require(workspace_bytes >= dsdk::Kv8EvictWorkspaceBytes(c, *batch, keep),
+            "the workspace is smaller than dsd_kv8_evict_workspace_bytes");
+    dsdk::Kv8EvictArgs a;
+    a.c = c;
+    a.b = *batch;
+    a.keep = keep;
+    a.first = first;
+    a.recent = recent;
+    a.weights = weights;
+    a.new_ids = new_page_ids;
+    a.new_stride = new_stride;
+    a.new_counts = new_page_counts;
+    a.kept = kept;
+    a.kept_tokens = static_cast<int*>(workspace);
+    a.fail.word = d_fail;
+    dsdk::LaunchKv8Evict(a, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int dsd_kv8_evict_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int keep,
+                                  size_t* bytes) {
+  return Guard([&] {
+    RequireSizes(cache, batch, 0, bytes);
+    Require(keep >= 0, "keep must be non-negative");
+    *bytes = dsdk::Kv8EvictWorkspaceBytes(cache->view, *batch, keep);
   });
 }
 

@@ -73,6 +73,23 @@ void LaunchKv8Cross(const Kv8AttendArgs& a, hipStream_t stream);
 size_t Kv8WeighBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WeighWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 void LaunchKv8Weigh(const Kv8AttendArgs& a, float* weights, hipStream_t stream);
+
+// Eviction (kv8_evict.hip).
+struct Kv8EvictArgs {
+  Kv8View c;
+  dsd_kv8_batch b = {};  // the lists
+  int keep = 0, first = 0, recent = 0;
+  float* weights = nullptr;
+  const int* new_ids = nullptr;  // [batch][new_stride]
+  int new_stride = 0;
+  int* new_counts = nullptr;  // [batch], pages
+  int* kept = nullptr;        // [batch][heads][keep], places of the lists
+  int* kept_tokens = nullptr;  // [batch], in the workspace
+  FailReport fail;
+};
+size_t Kv8EvictWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int keep);
+void LaunchKv8Evict(const Kv8EvictArgs& a, hipStream_t stream);
+
 size_t Kv8PromptWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 // Each key head's queries summed, in order, in float32: sums[batch][heads * dim].
@@ -84,5 +101,6 @@ void PreloadKv8Attend(const Kv8View& c);
 void PreloadKv8Prompt(const Kv8View& c);
 void PreloadKv8Cross(const Kv8View& c);
 void PreloadKv8Weigh(const Kv8View& c);
+void PreloadKv8Evict(const Kv8View& c);
 
 }  // namespace dsdk

@@ -794,6 +794,34 @@ int dsd_kv8_attend_weigh(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
 int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                                   int num_q_heads, size_t* bytes);
 
+/* Eviction by what the tokens weighed (dsd_kv8_attend_weigh's sums): each request's list
+ * is cut to at most `keep` tokens.  Of a list of more, each key head keeps its first
+ * `first` tokens, its last `recent` and of those between the ones of the largest weights,
+ * the lower place first among equals (NaN counts as larger than all numbers); first +
+ * recent <= keep.  A list of no more is kept whole.  The lists are those of the requests
+ * alone that shall be cut; a list's pages stay as they are (others may share them).
+ * The kept tokens go, in their order, to new pages, which the lists must not name:
+ * request r's are new_page_ids[r * new_stride ..], device memory, as many as its kept
+ * tokens fill (new_stride at least ceil(keep / page_size)); entries behind those are not
+ * read.  A new page's scale is the least that the largest of its kept numbers (code *
+ * scale) fits: of int8 codes that number / 127, rounded to float, of e4m3 codes a power of
+ * two; numbers are brought to it with one rounding (none where the scale stays the same).
+ * token_counts, summaries (where kept) and the weights go with them; codes and weights
+ * behind the last kept token become zero.
+ * new_page_counts[r]: the pages filled; kept ([batch][num_kv_heads][keep]): where the kept
+ * tokens of each key head were, as places (page of the list * page_size + token of the
+ * page), ascending, -1 behind the last.  A list that does not fit is skipped (code 2, its
+ * count 0, its kept as they were); listed pages outside the cache hold no token, such new
+ * pages take none (code 3).  batch: the lists, as dsd_kv8_attend's.
+ * workspace: dsd_kv8_evict_workspace_bytes, 16-byte aligned, required. */
+int dsd_kv8_evict(dsd_kv8* cache, const dsd_kv8_batch* batch, int keep, int first,
+                  int recent, float* weights, const int* new_page_ids,
+                  int new_stride, int* new_page_counts, int* kept,
+                  void* workspace, size_t workspace_bytes,
+                  unsigned long long* d_fail, void* stream);
+int dsd_kv8_evict_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                                  int keep, size_t* bytes);
+
 /* The sparse step (dsd_sparse_run_batch_device) over an 8-bit cache that keeps
  * summaries: every candidate page scored through its summary, the top_k pages
  * of each request kept, attention over those.  A page's score is the sum over
