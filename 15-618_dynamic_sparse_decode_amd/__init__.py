@@ -121,6 +121,11 @@ class Kv8BatchArgs(ctypes.Structure):
             "positions")]
 
 
+class Kv8PrefixArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("groups", "max_requests", "max_pages", "total_pages")] + [
+        (n, ctypes.c_void_p) for n in ("request_offsets", "page_offsets", "page_ids")]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "dsd_last_error": (ctypes.c_char_p, []),
@@ -247,6 +252,15 @@ _SIGNATURES = {
                              + [ctypes.c_void_p, ctypes.c_int64] * 2
                              + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
                              + [ctypes.c_void_p] * 2),
+    "dsd_kv8_attend_shared": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                             ctypes.POINTER(Kv8PrefixArgs), ctypes.c_int,
+                                             ctypes.c_int]
+                              + [ctypes.c_void_p, ctypes.c_int64] * 2
+                              + [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t]
+                              + [ctypes.c_void_p] * 2),
+    "dsd_kv8_shared_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
+                                                      ctypes.POINTER(Kv8PrefixArgs), ctypes.c_int,
+                                                      ctypes.POINTER(ctypes.c_size_t)]),
     "dsd_kv8_attend_weigh": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Kv8BatchArgs),
                                             ctypes.c_int, ctypes.c_int]
                              + [ctypes.c_void_p, ctypes.c_int64] * 2
@@ -921,6 +935,18 @@ class Kv8Batch:
         self.pointer = ctypes.pointer(self.args)
 
 
+class Kv8Prefix:
+    """The groups of a batch's requests that share a prefix (dsd_kv8_prefix): sizes, and
+    device addresses of the first request of each group (request_offsets) and of the
+    groups' page lists."""
+
+    def __init__(self, groups: int, max_requests: int = 0, max_pages: int = 0, total_pages: int = 0,
+                 request_offsets: int = 0, page_offsets: int = 0, page_ids: int = 0):
+        self.args = Kv8PrefixArgs(groups, max_requests, max_pages, total_pages,
+                                  request_offsets or None, page_offsets or None, page_ids or None)
+        self.pointer = ctypes.pointer(self.args)
+
+
 class Kv8Cache:
     """An 8-bit paged KV cache (dsd_kv8_*): a scale per page and key head,
     grouped query heads, float32 / bf16 / f16 rows.  arrays: device addresses
@@ -1021,6 +1047,24 @@ class Kv8Cache:
             workspace, workspace_bytes, fail, stream)
         if status:
             _check(status)
+
+    def attend_shared(self, batch: Kv8Batch, prefix: Kv8Prefix, dtype: int, num_q_heads: int, q: int,
+                      q_stride: int, out: int, out_stride: int, scale: float = 0.0,
+                      workspace: int = 0, workspace_bytes: int = 0, fail: int = 0,
+                      stream: int = 0) -> None:
+        """attend, each request over its group's prefix and then its own pages; a prefix
+        is read once for all its requests (dsd_kv8_attend_shared)."""
+        status = self._lib.dsd_kv8_attend_shared(
+            self.handle, batch.pointer, prefix.pointer, dtype, num_q_heads, q, q_stride, out,
+            out_stride, scale, workspace, workspace_bytes, fail, stream)
+        if status:
+            _check(status)
+
+    def shared_workspace_bytes(self, batch: Kv8Batch, prefix: Kv8Prefix, num_q_heads: int) -> int:
+        out = ctypes.c_size_t()
+        _check(self._lib.dsd_kv8_shared_workspace_bytes(self.handle, batch.pointer, prefix.pointer,
+                                                        num_q_heads, ctypes.byref(out)))
+        return out.value
 
     def attend_weigh(self, batch: Kv8Batch, dtype: int, num_q_heads: int, q: int, q_stride: int,
                      out: int, out_stride: int, scale: float = 0.0, weights: int = 0,

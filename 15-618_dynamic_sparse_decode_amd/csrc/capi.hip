@@ -3205,6 +3205,13 @@ void RequireSizes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int q_heads,
   RequireQueryRows(batch, q_heads);
 }
 
+void RequirePrefix(const dsd_kv8_prefix* p) {
+  Require(p != nullptr, "prefix must be non-null");
+  Require(p->groups >= 0 && p->max_requests >= 0 && p->max_pages >= 0 && p->total_pages >= 0,
+          "sizes must be non-negative");
+  Require(p->groups <= 65535, "at most 65535 groups per call");
+}
+
 enum class Rows { kOne, kCausal, kAll };  // of a request, and what they see
 
 // A checked call's arguments; false: nothing to do.
@@ -3323,6 +3330,7 @@ int dsd_kv8_create(int num_kv_heads, int head_dim, int page_size, int capacity_p
     dsdk::PreloadKv8Cross(v);
     dsdk::PreloadKv8Weigh(v);
     dsdk::PreloadKv8Evict(v);
+    dsdk::PreloadKv8Shared(v);
     *out_cache = cache.release();
   });
 }
@@ -3472,6 +3480,42 @@ int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch, in
   return Guard([&] {
     RequireSizes(cache, batch, num_q_heads, bytes);
     *bytes = num_q_heads > 0 ? dsdk::Kv8WorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
+  });
+}
+
+int dsd_kv8_attend_shared(dsd_kv8* cache, const dsd_kv8_batch* batch,
+                          const dsd_kv8_prefix* prefix, int type, int num_q_heads, const void* q,
+                          int64_t q_stride, void* out, int64_t out_stride, float scale,
+                          void* workspace, size_t workspace_bytes, unsigned long long* d_fail,
+                          void* stream) {
+  return Guard([&] {
+    dsdk::Kv8AttendArgs a;
+    RequirePrefix(prefix);
+    if (!ReadAttend(cache, batch, Rows::kOne, type, num_q_heads, q, q_stride, out, out_stride,
+                    scale, workspace, workspace_bytes, d_fail, &a)) {
+      return;
+    }
+    Require(prefix->groups == 0 ||
+                (prefix->request_offsets != nullptr && prefix->page_offsets != nullptr),
+            "request_offsets and page_offsets must be non-null");
+    Require(prefix->total_pages == 0 || prefix->page_ids != nullptr,
+            "page_ids must be non-null");
+    Require(prefix->total_pages == 0 || a.c.capacity > 0, "the cache holds no page");
+    Require(static_cast<int64_t>(prefix->max_requests) * num_q_heads <= 0x7fffffff,
+            "max_requests * num_q_heads must fit 31 bits");
+    Require(dsdk::Kv8SharedFits(a, *prefix), "the batch or the groups are too many for one call");
+    Require(a.workspace_bytes >= dsdk::Kv8SharedBytes(a.c, a.b, *prefix, num_q_heads),
+            "the workspace is smaller than dsd_kv8_shared_workspace_bytes");
+    dsdk::LaunchKv8Shared(a, *prefix, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int dsd_kv8_shared_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                                   const dsd_kv8_prefix* prefix, int num_q_heads, size_t* bytes) {
+  return Guard([&] {
+    RequireSizes(cache, batch, num_q_heads, bytes);
+    RequirePrefix(prefix);
+    *bytes = num_q_heads > 0 ? dsdk::Kv8SharedWorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
   });
 }
 

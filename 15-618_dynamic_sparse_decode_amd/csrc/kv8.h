@@ -74,6 +74,13 @@ size_t Kv8WeighBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 size_t Kv8WeighWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
 void LaunchKv8Weigh(const Kv8AttendArgs& a, float* weights, hipStream_t stream);
 
+// Attention behind shared prefixes (kv8_shared.hip): `a` is the requests' own lists.
+bool Kv8SharedFits(const Kv8AttendArgs& a, const dsd_kv8_prefix& p);
+size_t Kv8SharedBytes(const Kv8View& c, const dsd_kv8_batch& b, const dsd_kv8_prefix& p,
+                      int q_heads);
+size_t Kv8SharedWorkspaceBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads);
+void LaunchKv8Shared(const Kv8AttendArgs& a, const dsd_kv8_prefix& p, hipStream_t stream);
+
 // Eviction (kv8_evict.hip).
 struct Kv8EvictArgs {
   Kv8View c;
@@ -102,5 +109,6 @@ void PreloadKv8Prompt(const Kv8View& c);
 void PreloadKv8Cross(const Kv8View& c);
 void PreloadKv8Weigh(const Kv8View& c);
 void PreloadKv8Evict(const Kv8View& c);
+void PreloadKv8Shared(const Kv8View& c);
 
 }  // namespace dsdk

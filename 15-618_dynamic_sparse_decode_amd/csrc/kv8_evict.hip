@@ -489,7 +489,8 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
       Numbers4<FMT>(tile[t * D + d], x);
       sum += x[0];
     }
-    c.summaries[to * D + d] = sum / static_cast<float>(count) * key_scale;
+    c.summaries[to * D + d] =
+        static_cast<float>(static_cast<double>(sum) * static_cast<double>(key_scale) / count);
   }
 }
 

@@ -777,6 +777,35 @@ int dsd_kv8_attend_cross(dsd_kv8* cache, const dsd_kv8_batch* batch, int type,
 int dsd_kv8_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
                             int num_q_heads, size_t* bytes);
 
+/* dsd_kv8_attend for requests that share a prefix: group g's requests are
+ * request_offsets[g] to request_offsets[g + 1] - 1 of the batch, and each of them attends
+ * to the tokens of the group's list and then of its own (out = softmax over both).  The
+ * group's codes are read once for all its requests.  Requests before the first or behind
+ * the last group have no prefix.  max_requests: the most requests of a group; max_pages as
+ * in dsd_kv8_batch.  A group or a list that does not fit its sizes holds no token (code 2);
+ * a request that two groups' ranges cover has no prefix (code 2).
+ * Logits, sums and roundings as dsd_kv8_attend's.  workspace:
+ * dsd_kv8_shared_workspace_bytes (enough for any batch of at most these sizes, whatever the
+ * prefixes), 16-byte aligned, required. */
+typedef struct dsd_kv8_prefix {
+  int groups;
+  int max_requests;
+  int max_pages;
+  int total_pages;            /* entries of page_ids */
+  const int* request_offsets; /* [groups + 1] */
+  const int* page_offsets;    /* [groups + 1] */
+  const int* page_ids;
+} dsd_kv8_prefix;
+int dsd_kv8_attend_shared(dsd_kv8* cache, const dsd_kv8_batch* batch,
+                          const dsd_kv8_prefix* prefix, int type,
+                          int num_q_heads, const void* q, int64_t q_stride,
+                          void* out, int64_t out_stride, float scale,
+                          void* workspace, size_t workspace_bytes,
+                          unsigned long long* d_fail, void* stream);
+int dsd_kv8_shared_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* batch,
+                                   const dsd_kv8_prefix* prefix, int num_q_heads,
+                                   size_t* bytes);
+
 /* dsd_kv8_attend, and how much each token weighed: weights[page][key head][token of the
  * page] (float32, [capacity][num_kv_heads][page_size], device memory) grows by the token's
  * softmax weight, summed over the query heads of its key head.  Places that hold no token
