@@ -11,6 +11,36 @@ namespace {
 
 constexpr float kMostFactor = 100.0f;  // powers of two beyond which weights are formed in steps
 
+// 16 bytes of codes; once: they are not wanted again.
+template <bool kOnce>
+__device__ __forceinline__ uint4 LoadCodes(const uint8_t* p) {
+  if constexpr (kOnce) {
+    typedef unsigned U4 __attribute__((ext_vector_type(4)));
+    const U4 x = __builtin_nontemporal_load(reinterpret_cast<const U4*>(p));
+    return make_uint4(x[0], x[1], x[2], x[3]);
+  } else {
+    return *reinterpret_cast<const uint4*>(p);
+  }
+}
+
+// kWeigh: a wave's logits that are held in LDS, 16 blocks of 4 rows (its LDS behind the
+// staged pages: two workgroups of 72 KB a CU).
+constexpr int kSlotFloats = 4096;
+
+// Where the logits of a key head and 64 tokens of request r's list begin: [4 tokens of
+// four][4 chunks of 16][rows of the key head][4], so that a wave's store of one of its
+// four tiles is 64 bytes and more a chunk side by side, whole lines (rows of a head's
+// tokens each in a line of its own took 497 us in place of the figure in kv8_weigh.hip).
+// A list's first block is a whole one of its own.
+__host__ __device__ inline int64_t LogitBlocks(const Kv8AttendArgs& a) {
+  return static_cast<int64_t>(a.b.total_pages) * a.c.page / 64 + a.b.batch + 1;
+}
+__device__ __forceinline__ int64_t LogitBlock(const Kv8AttendArgs& a, const Plan& p, int head, int r,
+                                              int list, int block) {
+  const int64_t first = static_cast<int64_t>(list) * a.c.page / 64 + r;
+  return (head * LogitBlocks(a) + first + block) * 64 * p.group;
+}
+
 // One piece of request r's list for one tile of 16 rows (unit: key heads * row tiles,
 // the key head fastest); W waves, each of which takes
 // every W-th group of 64 tokens of the piece for all of the tile's 16 rows.
@@ -21,12 +51,16 @@ constexpr float kMostFactor = 100.0f;  // powers of two beyond which weights are
 // is free), whose first operand, 16 tokens of one dim, is one load of the
 // values' layout.  No number crosses lanes but for the maxima.
 // kJoin: a later launch joins the piece with others.  kWeigh: logits (times log2 e) go
-// to `logits` as well, [query heads][places of all lists], and the sums to p.stats.
+// to `logits` as well, and the rows' sums to p.stats.
 // kDim: head_dim where it is 64 * NU (no bounds tests), else 0.
 template <typename T, int FMT, int NU, int kDim, int W, bool kJoin, bool kWeigh = false>
 __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& p, int unit, int r,
                                             int piece, float* lds, float* logits = nullptr) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>, NT = 4 * NU;
+  // The loads of a wave's last group are issued too (its own once more): a wait for the
+  // values then counts the next keys and the stores, whichever path led there, and does
+  // not wait for them.
+  constexpr bool kSteady = kWeigh || kJoin;
   const Kv8View& c = a.c;
   const int D = kDim > 0 ? kDim : c.dim, tiles = kDim > 0 ? NT : D / 16;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
@@ -94,6 +128,27 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
   const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
   const int page_bytes = c.page * D;
   uint4 kw[4][NU], vw[NT];
+  // kWeigh: a wave's logits are kept in LDS and written many blocks at a time: a write
+  // here and there among the reads costs HBM a fifth of its rate, bursts of them a
+  // twentieth (16 bytes read a byte written, alone: 459 us for 2 GiB and 413 of 341
+  // without writes; 355 where the reads leave the caches alone besides).
+  const int tile_rows = min(p.group - first, 16);
+  const int most_held = kSlotFloats / (64 * tile_rows);
+  float* kept = lds + (sizeof(PageInfo) * kStage / sizeof(float)) + wave * kSlotFloats;
+  int held = 0;
+  auto flush = [&](int last) {  // blocks last, last - W, ...
+    const int quads = 16 * tile_rows;
+    for (int i = 0; i < held; ++i) {
+      float* to = logits + LogitBlock(a, p, head, r, s.q.list, last - (held - 1 - i) * W) + first * 4;
+      const float* from = kept + i * 64 * tile_rows;
+      for (int e = lane; e < quads; e += kWave) {
+        const int tg = e / tile_rows;  // (a compile-time 16 rows are no rule)
+        *reinterpret_cast<F32x4*>(to + (tg * (p.group - tile_rows) + e) * 4) =
+            *reinterpret_cast<const F32x4*>(from + 4 * e);
+      }
+    }
+    held = 0;
+  };
   for (int g0 = begin; g0 < end; g0 += per_stage) {
     const int g1 = min(end, g0 + per_stage);
     const int slot0 = 4 * g0 / c.chunks;
@@ -119,7 +174,7 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           if (kDim > 0 || (g + 4 * u) * 16 < D) {
-            kw[t][u] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + 64 * u);
+            kw[t][u] = LoadCodes<kWeigh>(kp + 4 * t * D + 64 * u);
           } else {
             kw[t][u] = make_uint4(0, 0, 0, 0);
           }
@@ -136,7 +191,7 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
                           (sub * D + n) * 16;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        if (t < tiles) vw[t] = *reinterpret_cast<const uint4*>(vp + 256 * t);
+        if (t < tiles) vw[t] = LoadCodes<kWeigh>(vp + 256 * t);
       }
     };
     int grp = g0 + wave;
@@ -162,7 +217,8 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
           }
         }
       }
-      if (more) load_keys(grp + W);
+      const int next = more ? grp + W : grp;
+      if (kSteady || more) load_keys(next);
 
       // Row n's tokens of the chunk: those in the cache that it sees.
       const int count = min(now.tokens, sees - (4 * grp + g) * 16);
@@ -178,11 +234,16 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
       }
       const float f = fmaxf(to_logit * now.key_scale, kKv8Tiny);
       if constexpr (kWeigh) {
-        if (there && 4 * grp + g < s.chunks) {
-          float* to = logits + static_cast<int64_t>(head * p.group + row) * a.b.total_pages * c.page +
-                      static_cast<int64_t>(s.q.list) * c.page + (4 * grp + g) * 16;
+        // (the block's rows of this tile, [4 t][4 g][tile rows][4], in a slot of the wave)
+        if (there) {
+          float* to = kept + held * 64 * tile_rows + (g * tile_rows + n) * 4;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) *reinterpret_cast<F32x4*>(to + 4 * t) = x[t] * f;
+          for (int t = 0; t < 4; ++t) *reinterpret_cast<F32x4*>(to + 16 * t * tile_rows) = x[t] * f;
+        }
+        if (++held == most_held || !more) {
+          WaveLdsFence();
+          flush(grp);
+          WaveLdsFence();
         }
       }
       float most = -INFINITY;
@@ -305,7 +366,7 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
           }
         }
       }
-      if (more) load_values(grp + W);
+      if (kSteady || more) load_values(next);
     }
   }
 
@@ -386,9 +447,10 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
 
 constexpr int kAttendWaves = 4;
 
-inline size_t AttendLdsBytes(int dim) {
+inline size_t AttendLdsBytes(int dim, bool weigh = false) {
   const size_t joined = sizeof(float) * (48 * kAttendWaves + kAttendWaves * 16 * (dim + 4));
-  const size_t staged = sizeof(PageInfo) * kStage;
+  const size_t staged =
+      sizeof(PageInfo) * kStage + (weigh ? sizeof(float) * kSlotFloats * kAttendWaves : 0);
   return joined > staged ? joined : staged;
 }
 

@@ -22,9 +22,10 @@ __global__ __launch_bounds__(kAttendWaves* kWave, NU <= 2 ? 2 : 1) void Kv8Atten
                                                            lds, logits);
 }
 
-// Grid (blocks of 256 places, key heads, batch); a block takes every gridDim.x-th 256 of
-// its list.
+// Grid (shares of a list, key heads, batch): a wave has kBlocks blocks of 64 tokens at a
+// time on their way, lane l their place l.
 constexpr int kRowTile = 64;
+constexpr int kBlocks = 4;
 __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, const float* logits,
                                                       float* weights) {
   __shared__ float row_base[kRowTile], row_inv[kRowTile];
@@ -32,13 +33,13 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
   const int r = blockIdx.z, head = blockIdx.y;
   Span s;
   if (!FindSpan(a, p.group, r, 0, p.group, &s)) return;
-  const int places = s.chunks * 16;
-  if (static_cast<int>(blockIdx.x) * 256 >= places) return;
-  const int pieces = Pieces(p, s);
+  const int blocks = (s.chunks + 3) / 4;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int64_t row_places = static_cast<int64_t>(a.b.total_pages) * c.page;
-  const float* from = logits + static_cast<int64_t>(head) * p.group * row_places +
-                      static_cast<int64_t>(s.q.list) * c.page;
+  const int first = static_cast<int>(blockIdx.x) * 4 * kBlocks;
+  if (first >= blocks) return;
+  const int pieces = Pieces(p, s);
+  const float* from = logits + LogitBlock(a, p, head, r, s.q.list, 0) +
+                      ((lane >> 2 & 3) * 4 + (lane >> 4)) * p.group * 4 + (lane & 3);
   for (int row0 = 0; row0 < p.group; row0 += kRowTile) {
     const int rows = min(kRowTile, p.group - row0);
     __syncthreads();
@@ -59,16 +60,26 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
       }
     }
     __syncthreads();
-    for (int at = blockIdx.x * 256 + threadIdx.x; at < places; at += gridDim.x * 256) {
-      const int slot = at / c.page;
-      const int page = a.b.page_ids[s.q.list + slot];
-      if (!InPool(page, c.capacity) || at - slot * c.page >= c.token_counts[page]) continue;
-      float w = 0.0f;
-      const float* x = from + row0 * row_places + at;
+    for (int b0 = first + wave * kBlocks; b0 < blocks; b0 += gridDim.x * 4 * kBlocks) {
+      float w[kBlocks] = {};
+      const float* x = from + (static_cast<int64_t>(b0) * 64 * p.group + row0 * 4);
 #pragma unroll 4
-      for (int i = 0; i < rows; ++i) w = fmaf(Exp2(x[i * row_places] - row_base[i]), row_inv[i], w);
-      unsafeAtomicAdd(weights + (static_cast<int64_t>(page) * c.heads + head) * c.page + at -
-                          slot * c.page, w);
+      for (int i = 0; i < rows; ++i) {
+        const float base = row_base[i], inv = row_inv[i];
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+          const float y = b0 + k < blocks ? x[k * 64 * p.group + 4 * i] : 0.0f;
+          w[k] = fmaf(Exp2(y - base), inv, w[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int at = (b0 + k) * 64 + lane, slot = at / c.page, off = at - slot * c.page;
+        if (slot >= s.q.pages) continue;
+        const int page = a.b.page_ids[s.q.list + slot];
+        if (!InPool(page, c.capacity) || off >= c.token_counts[page]) continue;
+        unsafeAtomicAdd(weights + (static_cast<int64_t>(page) * c.heads + head) * c.page + off, w[k]);
+      }
     }
   }
 }
@@ -91,7 +102,10 @@ size_t StatsBytes(const Kv8View& c, const dsd_kv8_batch& b, const Plan& p) {
   return (PlanSlots(c, b, p) * sizeof(PieceStats) + 15) / 16 * 16;
 }
 size_t LogitBytes(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
-  return static_cast<size_t>(q_heads) * b.total_pages * c.page * sizeof(float);
+  Kv8AttendArgs a;
+  a.c = c;
+  a.b = b;
+  return static_cast<size_t>(q_heads) * LogitBlocks(a) * 64 * sizeof(float);
 }
 
 template <typename T, int FMT>
@@ -105,12 +119,12 @@ void Launch(const Kv8AttendArgs& a, float* weights, hipStream_t stream) {
   float* logits = reinterpret_cast<float*>(space);
   const dim3 grid(a.c.heads * p.blocks, a.b.batch, p.pieces);
   WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
-    kernel<<<grid, kAttendWaves * kWave, AttendLdsBytes(a.c.dim), stream>>>(a, p, logits);
+    kernel<<<grid, kAttendWaves * kWave, AttendLdsBytes(a.c.dim, true), stream>>>(a, p, logits);
   });
   DSD_HIP_CHECK(hipGetLastError());
   Merge<T>(a, p, stream);
-  const int64_t blocks = (static_cast<int64_t>(a.b.max_pages) * a.c.page + 255) / 256;
-  const dim3 over(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(blocks, 1), 65536)),
+  const int64_t shares = (ListGroups(a.c, a.b) + 4 * kBlocks - 1) / (4 * kBlocks);
+  const dim3 over(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(shares, 1), 65536)),
                   a.c.heads, a.b.batch);
   Kv8WeighKernel<<<over, 256, 0, stream>>>(a, p, logits, weights);
   DSD_HIP_CHECK(hipGetLastError());
@@ -128,7 +142,7 @@ void PreloadDim(const Kv8View& c) {
     PreloadKernel(kernel);
     DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                       hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(AttendLdsBytes(c.dim))));
+                                      static_cast<int>(AttendLdsBytes(c.dim, true))));
   });
 }
 
