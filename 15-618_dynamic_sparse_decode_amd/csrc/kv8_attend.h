@@ -66,11 +66,6 @@ __device__ __forceinline__ F16x8 Numbers8(unsigned w0, unsigned w1) {
   return r;
 }
 
-// The high bit of each byte that is an e4m3 NaN.
-__device__ __forceinline__ unsigned NanBytes(unsigned w) {
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-}
-
 // What a workgroup attends: rows [first, first + some) of request r (row i:
 // token i / group, query head i % group of the key head), chunks of 16 tokens.
 struct Span {

@@ -64,6 +64,11 @@ __device__ __forceinline__ bool Kv8ReadRows(const dsd_kv8_batch& b, int r, Kv8Re
   return true;
 }
 
+// The high bit of each byte that is an e4m3 NaN.
+__device__ __forceinline__ unsigned NanBytes(unsigned w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
 // Orders one wave's LDS writes before its reads of what other lanes wrote.
 __device__ __forceinline__ void WaveLdsFence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

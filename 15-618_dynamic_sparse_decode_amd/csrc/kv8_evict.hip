@@ -1,11 +1,12 @@
 // kv8_evict.hip -- dsd_kv8_evict (gfx950): a list's tokens cut to a budget by what they
 // weighed, the kept ones of each key head moved, in order, to new pages.
 //
-// Mathematics.  Which tokens: per request and key head a selection of the need = keep -
-// first - recent largest of n weights.  A weight's bits, turned so that they order as
-// the numbers do, are searched from the top in digits of 11, 11 and 10 bits: the digit's
-// counts in LDS, from the largest down until `need` is reached.  That leaves the need-th
-// largest key T and how many keys equal to it are kept, the ones of the lowest places.
+// Mathematics.  Which tokens: per request and key head a selection of the `keep` best of
+// n tokens, the better the larger the weight, then the lower the place; the first and the
+// last ones are better than all others.  A weight's bits, turned so that they order as the numbers do, and behind
+// them the place's are searched from the top in digits of up to 11 bits: the digit's
+// counts in LDS, from the best down until `keep` is reached.  Once few candidates share
+// the digits so far each counts those that are better.
 // Then what they become: the numbers code * scale of a new page's tokens (their old pages
 // have scales of their own) share the least scale that their largest fits, and each is
 // rounded once to it.
@@ -22,11 +23,14 @@ constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
 constexpr int kDigit = 11;
 constexpr int kBins = 1 << kDigit;
+constexpr int kFew = 64;  // candidates that rank themselves: as many reads of LDS each
 
-// A weight's bits in the numbers' order; NaN above all, -0 as 0.
+// A weight's bits in the numbers' order; NaN above all, -0 as 0.  Below every number's is
+// kGone (no token), above every one kAlways (kept whatever it weighs).
+constexpr unsigned kGone = 0u, kAlways = 0xffffffffu;
 __device__ __forceinline__ unsigned KeyOf(float w) {
   const unsigned u = __float_as_uint(w + 0.0f);
-  if (w != w) return 0xffffffffu;
+  if (w != w) return kAlways - 1u;
   return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 
@@ -55,23 +59,27 @@ __device__ __forceinline__ int BlockBefore(int x, int* wave_sums, int* total) {
 
 struct SelectLds {
   int bins[kBins];
-  int wave_sums[kSelectWaves], wave_ties[kSelectWaves];
+  int wave_sums[kSelectWaves];
   int first_end, recent_begin;  // places before the one, from the other on are kept
   unsigned found_digit;
-  int found_above;
+  int found_above, found_count;
+  int few;
+  uint2 list[kFew];
 };
 
-// What is searched: places before `first_end` and from `recent_begin` on are kept, `need`
-// of the others, `count` in all.
+// What is searched: places before `first_end` and from `recent_begin` on are kept, with
+// the best of the others `count` in all.
 struct Search {
   Kv8Request q;
   int head, r;
   int places, tiles;  // tiles of 64 places that a wave has
   int first_end, recent_begin;
-  int need, count;
+  int count;
+  int held;  // tokens
 };
 
-template <int kHeld>
+// kPacked: all pages but the last are full, so place i is token i.
+template <int kHeld, bool kPacked>
 __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search& f,
                                              SelectLds& lds);
 
@@ -83,7 +91,7 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
   const Kv8View& c = a.c;
   const int head = blockIdx.x, r = blockIdx.y;
   Kv8Request q;
-  if (!Kv8ReadList(a.b, r, &q) || q.pages > 0x7fffff00 / c.page) {
+  if (!Kv8ReadList(a.b, r, &q) || q.pages > 0x7fff0000 / c.page) {
     if (threadIdx.x == 0) {
       ReportFailure(a.fail, kFailShape);
       if (head == 0) a.new_counts[r] = a.kept_tokens[r] = 0;
@@ -102,16 +110,26 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
   const int share = (q.pages + kSelectThreads - 1) / kSelectThreads;
   const int s0 = min(q.pages, static_cast<int>(threadIdx.x) * share), s1 = min(q.pages, s0 + share);
   int mine = 0;
-  for (int s = s0; s < s1; ++s) mine += count_of(s);
+  bool full = true;
+  for (int s = s0; s < s1; ++s) {
+    const int n = count_of(s);
+    mine += n;
+    full = full && (n == c.page || s == q.pages - 1);
+  }
   if (threadIdx.x == 0) {
     lds.first_end = 0;
     lds.recent_begin = 0x7fffffff;
   }
+  const bool packed = __syncthreads_and(full) != 0;
   int held;
   int rank = BlockBefore(mine, lds.wave_sums, &held);
   const bool all = held <= a.keep;
-  const int need = all ? 0 : a.keep - a.first - a.recent;
-  if (!all) {
+  if (!all && packed) {
+    if (threadIdx.x == 0) {
+      lds.first_end = a.first;
+      if (a.recent > 0) lds.recent_begin = held - a.recent;
+    }
+  } else if (!all) {
     const int from = held - a.recent;  // the rank of the first of the last
     for (int s = s0; s < s1; ++s) {
       const int n = count_of(s);
@@ -119,8 +137,6 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
       if (rank <= from && from < rank + n) lds.recent_begin = s * c.page + from - rank;
       rank += n;
     }
-  } else if (threadIdx.x == 0) {
-    lds.first_end = 0x7fffffff;
   }
   __syncthreads();
   const int count = min(held, a.keep);
@@ -131,84 +147,104 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
 
   const int places = q.pages * c.page;
   const int tiles = ((places + kWave - 1) / kWave + kSelectWaves - 1) / kSelectWaves;
-  const Search f = {q,    head,  r, places, tiles, lds.first_end, lds.recent_begin,
-                    need, count};
+  const Search f = {q, head, r, places, tiles, lds.first_end, lds.recent_begin, count, held};
   if (tiles <= kHeld) {
-    SelectPlaces<kHeld>(a, f, lds);
+    packed ? SelectPlaces<kHeld, true>(a, f, lds) : SelectPlaces<kHeld, false>(a, f, lds);
   } else {
-    SelectPlaces<0>(a, f, lds);
+    packed ? SelectPlaces<0, true>(a, f, lds) : SelectPlaces<0, false>(a, f, lds);
   }
 }
 
 // Wave w has the w-th `tiles` tiles of 64 places, lane l place l of each.
-template <int kHeld>
+template <int kHeld, bool kPacked>
 __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search& f,
                                              SelectLds& lds) {
   const Kv8View& c = a.c;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int tiles = f.tiles;
-  // Places: kGone (no token), kAlways, or a candidate of some key.
-  enum { kGone, kAlways, kCandidate };
   const int base = wave * tiles * kWave + lane;
-  struct Place {
-    int kind;
-    unsigned key;
-  };
-  auto read = [&](int at) {
-    Place p = {kGone, 0u};
-    if (at < f.places) {
-      const int slot = at / c.page, off = at - slot * c.page;
-      const int page = a.b.page_ids[f.q.list + slot];
-      if (InPool(page, c.capacity) && off < c.token_counts[page]) {
-        p.kind = at < f.first_end || at >= f.recent_begin ? kAlways : kCandidate;
-        p.key = KeyOf(a.weights[(static_cast<int64_t>(page) * c.heads + f.head) * c.page + off]);
-      }
+
+  // kBatch tiles are read at a time, without a branch between them (beyond the list: its
+  // last place again), so that their loads are on their way together.
+  constexpr int kBatch = 8;
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
+  auto read = [&](int j0, unsigned* p) {
+    int page[kBatch], off[kBatch];
+    float w[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int at = min(base + (j0 + k) * kWave, f.places - 1);
+      const int slot = c.chunks == 1 ? at >> 4 : static_cast<int>(__umulhi(at >> 4, inverse));
+      off[k] = at - slot * c.page;
+      page[k] = a.b.page_ids[f.q.list + slot];
     }
-    return p;
+    int count[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const bool ok = InPool(page[k], c.capacity);
+      const int64_t at = ok ? page[k] : 0;
+      w[k] = a.weights[(at * c.heads + f.head) * c.page + off[k]];
+      if constexpr (!kPacked) count[k] = ok ? c.token_counts[at] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int at = base + (j0 + k) * kWave;
+      const bool there = kPacked ? at < f.held : at < f.places && off[k] < count[k];
+      p[k] = !there || j0 + k >= tiles
+                 ? kGone
+                 : (at < f.first_end || at >= f.recent_begin ? kAlways : KeyOf(w[k]));
+    }
   };
-  constexpr int kArray = kHeld > 0 ? kHeld : 1;
-  unsigned keys[kArray];
-  unsigned long long gone = 0, always = 0;  // of tile j at bit j
+  unsigned keys[kHeld > 0 ? kHeld : 1];
   if constexpr (kHeld > 0) {
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const Place p = j < tiles ? read(base + j * kWave) : Place{kGone, 0u};
-      keys[j] = p.key;
-      gone |= static_cast<unsigned long long>(p.kind == kGone) << j;
-      always |= static_cast<unsigned long long>(p.kind == kAlways) << j;
+    for (int j0 = 0; j0 < kHeld; j0 += kBatch) {
+      if (j0 < tiles) read(j0, keys + j0);
     }
   }
-  // with(j, place) for the wave's tiles in order.
+  // with(j, key) for the wave's tiles in order.
   auto each = [&](auto&& with) {
     if constexpr (kHeld > 0) {
 #pragma unroll
       for (int j = 0; j < kHeld; ++j) {
-        if (j < tiles) {
-          with(j, Place{(gone >> j & 1) != 0 ? kGone : ((always >> j & 1) != 0 ? kAlways : kCandidate),
-                     keys[j]});
-        }
+        if (j < tiles) with(j, keys[j]);
       }
     } else {
-      for (int j = 0; j < tiles; ++j) with(j, read(base + j * kWave));
+      for (int j0 = 0; j0 < tiles; j0 += kBatch) {
+        unsigned p[kBatch];
+        read(j0, p);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) with(j0 + k, p[k]);
+      }
     }
   };
 
-  // The need-th largest key, a digit at a time: candidates whose digits so far are the
-  // key's are counted by the next one.
-  unsigned key = 0xffffffffu;
-  int ties = 0;  // of the key's equals, that many are kept
-  if (f.need > 0) {
-    int left = f.need;
-    unsigned known = 0;  // the digits so far, and which bits they are
-    unsigned mask = 0;
+  // The count-th best place: of those whose digits so far are its own the next digit is
+  // counted, until few are left, which rank themselves.
+  unsigned key = kGone;
+  int last = -1;  // of the places with its key the last that is kept
+  if (f.count < f.held) {
+    int left = f.count;
+    unsigned key_known = 0, key_mask = 0;  // the digits so far, and which bits they are
+    unsigned place_known = 0, place_mask = 0;
+    auto matches = [&](unsigned p, unsigned turned) {
+      return p != kGone && (p & key_mask) == key_known && (turned & place_mask) == place_known;
+    };
+    auto turned_place = [&](int j) { return 0x7fffffffu - static_cast<unsigned>(base + j * kWave); };
 #pragma unroll 1
-    for (int shift = 32 - kDigit; ; shift = max(shift - kDigit, 0)) {
-      const int width = mask == 0 || shift > 0 ? kDigit : 32 - 2 * kDigit;
+    for (int step = 0;; ++step) {
+      // bits 21.., 10.., 0.. of the key (11, 11, 10 of them), then 20.., 9.., 0.. of the
+      // place turned (11, 11, 9)
+      const bool by_key = step < 3;
+      const int shift = by_key ? max(21 - 11 * step, 0) : max(20 - 11 * (step - 3), 0);
+      const int width = step == 2 ? 10 : (step == 5 ? 9 : kDigit);
       for (int i = threadIdx.x; i < kBins; i += kSelectThreads) lds.bins[i] = 0;
+      if (threadIdx.x == 0) lds.few = 0;
       __syncthreads();
-      each([&](int, const Place& p) {
-        if (p.kind == kCandidate && (p.key & mask) == known) {
-          atomicAdd(&lds.bins[(p.key >> shift) & ((1u << width) - 1u)], 1);
+      each([&](int j, unsigned p) {
+        const unsigned turned = turned_place(j);
+        if (matches(p, turned)) {
+          atomicAdd(&lds.bins[((by_key ? p : turned) >> shift) & ((1u << width) - 1u)], 1);
         }
       });
       __syncthreads();
@@ -221,48 +257,57 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
         const bool second = left > above + n0;
         lds.found_digit = static_cast<unsigned>(second ? b0 - 1 : b0);
         lds.found_above = second ? above + n0 : above;
+        lds.found_count = second ? n1 : n0;
       }
       __syncthreads();
       left -= lds.found_above;
-      known |= lds.found_digit << shift;
-      mask |= ((1u << width) - 1u) << shift;
-      if (shift == 0) break;
+      (by_key ? key_known : place_known) |= lds.found_digit << shift;
+      (by_key ? key_mask : place_mask) |= ((1u << width) - 1u) << shift;
+      const int few = lds.found_count;
+      if (few > kFew) continue;  // (places differ: the last step leaves one)
+      each([&](int j, unsigned p) {
+        const unsigned turned = turned_place(j);
+        if (matches(p, turned)) lds.list[atomicAdd(&lds.few, 1)] = make_uint2(p, turned);
+      });
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < few) {
+        const uint2 mine = lds.list[threadIdx.x];
+        int better = 0;
+#pragma unroll 4
+        for (int i = 0; i < few; ++i) {
+          const uint2 x = lds.list[i];
+          better += x.x > mine.x || (x.x == mine.x && x.y > mine.y) ? 1 : 0;
+        }
+        if (better == left - 1) {
+          lds.found_digit = mine.x;
+          lds.found_above = static_cast<int>(0x7fffffffu - mine.y);
+        }
+      }
+      __syncthreads();
+      key = lds.found_digit;
+      last = lds.found_above;
+      break;
     }
-    key = known;
-    ties = left;
   }
 
-  // What each wave keeps, then where its kept places go.
-  const bool any = f.need > 0;
-  int sure = 0, equal = 0;
-  each([&](int, const Place& p) {
-    const bool candidate = any && p.kind == kCandidate;
-    sure += __popcll(__ballot(p.kind == kAlways || (candidate && p.key > key)));
-    equal += __popcll(__ballot(candidate && p.key == key));
-  });
+  // How many each wave keeps, then where its kept places go.
+  auto keeps = [&](int j, unsigned p) {
+    return p > key || (p == key && base + j * kWave <= last);
+  };
+  int sure = 0;
+  each([&](int j, unsigned p) { sure += static_cast<int>(__popcll(__ballot(keeps(j, p)))); });
   __syncthreads();
-  if (lane == 0) {
-    lds.wave_sums[wave] = sure;
-    lds.wave_ties[wave] = equal;
-  }
+  if (lane == 0) lds.wave_sums[wave] = sure;
   __syncthreads();
-  int at = 0, ties_before = 0;
-  for (int w = 0; w < wave; ++w) {
-    at += lds.wave_sums[w] + max(min(ties - ties_before, lds.wave_ties[w]), 0);
-    ties_before += lds.wave_ties[w];
-  }
+  int at = 0;
+  for (int w = 0; w < wave; ++w) at += lds.wave_sums[w];
   int* kept = a.kept + (static_cast<int64_t>(f.r) * c.heads + f.head) * a.keep;
   const unsigned long long below = (1ull << lane) - 1ull;
-  each([&](int j, const Place& p) {
-    const bool candidate = any && p.kind == kCandidate;
-    const bool tie = candidate && p.key == key;
-    const unsigned long long tied = __ballot(tie);
-    const bool keep = p.kind == kAlways || (candidate && p.key > key) ||
-                      (tie && ties_before + static_cast<int>(__popcll(tied & below)) < ties);
+  each([&](int j, unsigned p) {
+    const bool keep = keeps(j, p);
     const unsigned long long taken = __ballot(keep);
     if (keep) kept[at + __popcll(taken & below)] = base + j * kWave;
-    at += __popcll(taken);
-    ties_before += __popcll(tied);
+    at += static_cast<int>(__popcll(taken));
   });
   for (int i = f.count + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = -1;
 }
@@ -277,15 +322,29 @@ struct Source {
   float value_scale;
 };
 
-// The largest magnitude of four codes' numbers (finite ones).
+typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned Max16(unsigned x, unsigned y) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(U16x2, x),
+                                                                __builtin_bit_cast(U16x2, y)));
+}
+
+// The magnitudes of four codes, which order as their bytes do (0 for NaN).
 template <int FMT>
-__device__ __forceinline__ float MostOf4(unsigned w) {
-  float x[4];
-  Numbers4<FMT>(w, x);
-  float most = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[i]));  // (fmaxf passes over NaN)
-  return most;
+__device__ __forceinline__ unsigned Sizes4(unsigned w) {
+  if constexpr (FMT == DSD_KV8_INT8) {
+    const unsigned sign = (w >> 7) & 0x01010101u;
+    return (w ^ (sign * 0xffu)) + sign;
+  } else {
+    return (w & 0x7f7f7f7fu) & ~((NanBytes(w) >> 7) * 0xffu);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ double NumberOf(unsigned size) {
+  if constexpr (FMT == DSD_KV8_INT8) {
+    return static_cast<double>(size);
+  } else {
+    return static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(size), 0));
+  }
 }
 
 // The least scale whose largest code reaches `most`.
@@ -307,44 +366,104 @@ __device__ __forceinline__ double WaveMost(double x) {
   return x;
 }
 
+// Codes brought from one scale to another.  Exact in 64 bits (Slow4); the quotient of the
+// scales in 32 bits does where it is a power of two (e4m3: a product with a code is exact,
+// one rounding), and of int8 codes where the product lies further from a border between
+// two codes than its error of 127 * 2^-22 (a quarter of the time in 64 bits).
+template <int FMT>
+__device__ __forceinline__ float RatioOf(float had, const Scale& s, bool* fast) {
+  if constexpr (FMT == DSD_KV8_INT8) {
+    *fast = true;
+    return static_cast<float>(static_cast<double>(had) * s.inv64);
+  } else {
+    const unsigned bits = __float_as_uint(had);
+    // (0: a place without a token; its codes are 0)
+    *fast = (bits & 0x807fffffu) == 0u && bits != 0x7f800000u;
+    const int e = static_cast<int>(bits >> 23) - static_cast<int>(__float_as_uint(s.s) >> 23);
+    return e < -126 || bits == 0u ? 0.0f
+                                  : __uint_as_float(static_cast<unsigned>(min(e, 30) + 127) << 23);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ unsigned Slow4(unsigned w, const float (&had)[4], const Scale& s) {
+  float n[4];
+  Numbers4<FMT>(w, n);
+  double y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<double>(n[e]) * static_cast<double>(had[e]);
+  return Codes4<FMT>(y[0], y[1], y[2], y[3], s);
+}
+// *sure: the result stands (int8).
+template <int FMT>
+__device__ __forceinline__ unsigned Quick4(unsigned w, const float (&ratio)[4], bool* sure) {
+  float n[4];
+  Numbers4<FMT>(w, n);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) n[e] *= ratio[e];
+  if constexpr (FMT == DSD_KV8_INT8) {
+    unsigned out = 0;
+    *sure = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float near = rintf(n[e]);
+      *sure = *sure && fabsf(n[e] - near) < 0.5f - 0x1p-13f;
+      out |= (static_cast<unsigned>(static_cast<int>(near)) & 0xffu) << (8 * e);
+    }
+    return out;
+  } else {
+    *sure = true;
+    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(n[0], n[1], 0, false);
+    return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(n[2], n[3], low, true));
+  }
+}
+
 // Grid (key heads * new pages, batch): one new page of one key head.  Waves 2 i have the
 // keys, 2 i + 1 the values of chunks i, i + kWaves / 2, ... of 16 tokens (U of them) in
 // registers, as codes: keys lane l unit l + 64 j (16 dims) of the chunk's [16][dim],
-// values lane l dims l + 64 j, all 16 tokens.  NU = ceil(dim / 64).
-template <int FMT, int NU, int U>
+// values lane l dims l + 64 j, all 16 tokens.  NU = ceil(dim / 64); kDim: head_dim where it
+// is 64 * NU, else 0.
+template <int FMT, int NU, int kDim, int U>
 __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double wave_most[8];
+  __shared__ float key_scale;
   const Kv8View& c = a.c;
-  const int D = c.dim, units = D / 16, ps = c.page;
+  const int D = kDim > 0 ? kDim : c.dim, units = D / 16, ps = c.page;
   const int head = blockIdx.x % c.heads, index = blockIdx.x / c.heads, r = blockIdx.y;
-  const int count = min(a.kept_tokens[r] - index * ps, ps);
-  if (count <= 0) return;
+  // (loads that do not wait for each other)
+  const int* kept = a.kept + (static_cast<int64_t>(r) * c.heads + head) * a.keep + index * ps;
+  int place = 0;
+  if (static_cast<int>(threadIdx.x) < ps && index * ps + static_cast<int>(threadIdx.x) < a.keep) {
+    place = kept[threadIdx.x];
+  }
+  Kv8Request q;
+  const bool listed = Kv8ReadList(a.b, r, &q);
   const int page = a.new_ids[static_cast<int64_t>(r) * a.new_stride + index];
+  const int count = min(a.kept_tokens[r] - index * ps, ps);
+  if (count <= 0 || !listed) return;
   if (!InPool(page, c.capacity)) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
     return;
   }
-  Kv8Request q;
-  if (!Kv8ReadList(a.b, r, &q)) return;
   Source* source = reinterpret_cast<Source*>(smem);
   uint8_t* tile = smem + sizeof(Source) * ps;  // the new keys (for their mean)
-  const int* kept = a.kept + (static_cast<int64_t>(r) * c.heads + head) * a.keep + index * ps;
   const int64_t to = static_cast<int64_t>(page) * c.heads + head;
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
   for (int i = threadIdx.x; i < ps; i += blockDim.x) {
+    if (i >= static_cast<int>(blockDim.x) && i < count) place = kept[i];
     Source s = {-1, 0, 0.0f, 0.0f};
-    float w = 0.0f;
+    float weight = 0.0f;
     if (i < count) {
-      const int place = kept[i], slot = place / ps;
+      const int slot = c.chunks == 1 ? place >> 4 : static_cast<int>(__umulhi(place >> 4, inverse));
       s.off = place - slot * ps;
       s.page = a.b.page_ids[q.list + slot];
       const int64_t at = static_cast<int64_t>(s.page) * c.heads + head;
       s.key_scale = c.key_scales[at];
       s.value_scale = c.value_scales[at];
-      w = a.weights[at * ps + s.off];
+      weight = a.weights[at * ps + s.off];
     }
     source[i] = s;
-    a.weights[to * ps + i] = w;
+    a.weights[to * ps + i] = weight;
   }
   if (threadIdx.x == 0 && head == 0) c.token_counts[page] = count;
   __syncthreads();
@@ -354,7 +473,6 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   const bool is_key = (wave & 1) == 0;
   const int page_bytes = ps * D;
   unsigned w[U][NU][4];
-  double most = 0.0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int chunk = wave / 2 + waves / 2 * u;
@@ -368,7 +486,7 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
 #pragma unroll
       for (int j = 0; j < NU; ++j) {
         const int i = lane + kWave * j;
-        if (i < D) {
+        if (kDim > 0 || i < D) {
           const int token = i / units;
           const Source s = source[16 * chunk + token];
           if (s.page >= 0) {
@@ -393,13 +511,16 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
 #pragma unroll
           for (int j = 0; j < NU; ++j) {
             const int d = lane + kWave * j;
-            if (d < D) w[u][j][t >> 2] |= static_cast<unsigned>(p[d * 16]) << (8 * (t & 3));
+            if (kDim > 0 || d < D) {
+              w[u][j][t >> 2] |= static_cast<unsigned>(p[d * 16]) << (8 * (t & 3));
+            }
           }
         }
       }
     }
   }
-  // The largest number.
+  // The largest number: of a token's codes by their bytes, then of the tokens'.
+  double most = 0.0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int chunk = wave / 2 + waves / 2 * u;
@@ -408,32 +529,52 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
 #pragma unroll
       for (int j = 0; j < NU; ++j) {
         const int i = lane + kWave * j;
-        if (i < D) {
-          float top = 0.0f;
+        if (kDim > 0 || i < D) {
+          unsigned top = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top = fmaxf(top, MostOf4<FMT>(w[u][j][k]));
-          most = fmax(most, static_cast<double>(top) *
+          for (int k = 0; k < 4; ++k) {
+            const unsigned x = Sizes4<FMT>(w[u][j][k]);
+            top = Max16(top, Max16(x & 0x00ff00ffu, (x >> 8) & 0x00ff00ffu));
+          }
+          top = max(top & 0xffffu, top >> 16);
+          most = fmax(most, NumberOf<FMT>(top) *
                                 static_cast<double>(source[16 * chunk + i / units].key_scale));
         }
       }
     } else {
+      // tokens 4 k + {0, 2} and 4 k + {1, 3}; then half of them from each lane's partner,
+      // until a lane has two tokens' of its 8 lanes, of which the wave has 8 groups
+      unsigned top[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        double scale[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          scale[e] = static_cast<double>(source[16 * chunk + 4 * k + e].value_scale);
-        }
+        unsigned even = 0, odd = 0;
 #pragma unroll
         for (int j = 0; j < NU; ++j) {
-          float x[4];
-          Numbers4<FMT>(w[u][j][k], x);
+          const unsigned x = Sizes4<FMT>(w[u][j][k]);
+          even = Max16(even, x & 0x00ff00ffu);
+          odd = Max16(odd, (x >> 8) & 0x00ff00ffu);
+        }
+        top[2 * k] = even;
+        top[2 * k + 1] = odd;
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            most = fmax(most, fabs(static_cast<double>(x[e])) * scale[e]);
-          }
+      for (int half = 4; half >= 1; half >>= 1) {
+        const bool high = (lane & half) != 0;  // keeps the upper half
+#pragma unroll
+        for (int k = 0; k < half; ++k) {
+          const unsigned give = high ? top[k] : top[k + half];
+          const unsigned keep = high ? top[k + half] : top[k];
+          top[k] = Max16(keep, static_cast<unsigned>(__shfl_xor(static_cast<int>(give), half, kWave)));
         }
       }
+#pragma unroll
+      for (int o = 8; o < kWave; o <<= 1) {
+        top[0] = Max16(top[0], static_cast<unsigned>(__shfl_xor(static_cast<int>(top[0]), o, kWave)));
+      }
+      // top[0]: index lane & 7 of the eight
+      const int token = 16 * chunk + 4 * ((lane & 7) >> 1) + (lane & 1);
+      most = fmax(most, NumberOf<FMT>(top[0] & 0xffffu) * static_cast<double>(source[token].value_scale));
+      most = fmax(most, NumberOf<FMT>(top[0] >> 16) * static_cast<double>(source[token + 2].value_scale));
     }
   }
   most = WaveMost(most);
@@ -443,7 +584,7 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   for (int i = wave & 1; i < waves; i += 2) most = fmax(most, wave_most[i]);
   Scale scale;
   scale.Set<FMT>(ScaleForNumber<FMT>(most));
-  if (threadIdx.x == 0) c.key_scales[to] = scale.s;
+  if (threadIdx.x == 0) c.key_scales[to] = key_scale = scale.s;
   if (threadIdx.x == kWave) c.value_scales[to] = scale.s;
 
   // Brought to it.
@@ -451,25 +592,49 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   for (int u = 0; u < U; ++u) {
     const int chunk = wave / 2 + waves / 2 * u;
     if (chunk >= c.chunks) continue;
+    // lane t: of token t % 16
+    const Source mine = source[16 * chunk + (lane & 15)];
+    bool fast;
+    const float ratio = RatioOf<FMT>(is_key ? mine.key_scale : mine.value_scale, scale, &fast);
+    const bool all_fast = __ballot(!fast) == 0;
+    const bool same = __ballot(mine.page >= 0 && ratio != 1.0f) == 0 && all_fast;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int i = lane + kWave * j;
-      if (i >= D) continue;
-      unsigned x[4];
+      if (kDim == 0 && i >= D) continue;
+      if (!same) {
+        const int token = is_key ? i / units : 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float n[4];
-        Numbers4<FMT>(w[u][j][k], n);
-        double y[4];
+        for (int k = 0; k < 4; ++k) {
+          float by[4];
+          bool sure = false;
+          unsigned x = 0;
+          if (all_fast) {
+            if (is_key) {
+              const float mine_by = __shfl(ratio, token, kWave);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float had = is_key ? source[16 * chunk + i / units].key_scale
-                                   : source[16 * chunk + 4 * k + e].value_scale;
-          y[e] = static_cast<double>(n[e]) * static_cast<double>(had);
+              for (int e = 0; e < 4; ++e) by[e] = mine_by;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                by[e] = __uint_as_float(static_cast<unsigned>(__builtin_amdgcn_readlane(
+                    static_cast<int>(__float_as_uint(ratio)), 4 * k + e)));
+              }
+            }
+            x = Quick4<FMT>(w[u][j][k], by, &sure);
+          }
+          if (!sure) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              by[e] = is_key ? source[16 * chunk + token].key_scale
+                             : source[16 * chunk + 4 * k + e].value_scale;
+            }
+            x = Slow4<FMT>(w[u][j][k], by, scale);
+          }
+          w[u][j][k] = x;
         }
-        x[k] = Codes4<FMT>(y[0], y[1], y[2], y[3], scale);
       }
-      const uint4 out = make_uint4(x[0], x[1], x[2], x[3]);
+      const uint4 out = make_uint4(w[u][j][0], w[u][j][1], w[u][j][2], w[u][j][3]);
       const int64_t at = to * page_bytes + chunk * 16 * D + 16 * i;
       *reinterpret_cast<uint4*>((is_key ? c.keys : c.values) + at) = out;
       if (is_key && c.summaries != nullptr) {
@@ -479,18 +644,21 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   }
   if (c.summaries == nullptr) return;
   __syncthreads();
-  __shared__ float key_scale;
-  if (threadIdx.x == 0) key_scale = scale.s;
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float sum = 0.0f;
+  for (int d = 4 * threadIdx.x; d < D; d += 4 * blockDim.x) {
+    float sum[4] = {};
     for (int t = 0; t < count; ++t) {
       float x[4];
-      Numbers4<FMT>(tile[t * D + d], x);
-      sum += x[0];
+      Numbers4<FMT>(*reinterpret_cast<const unsigned*>(tile + t * D + d), x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += x[e];
     }
-    c.summaries[to * D + d] =
-        static_cast<float>(static_cast<double>(sum) * static_cast<double>(key_scale) / count);
+    F32x4 mean;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mean[e] =
+          static_cast<float>(static_cast<double>(sum[e]) * static_cast<double>(key_scale) / count);
+    }
+    *reinterpret_cast<F32x4*>(c.summaries + to * D + d) = mean;
   }
 }
 
@@ -499,22 +667,23 @@ size_t MoveLdsBytes(const Kv8View& c) {
 }
 
 // Calls f with the kernel of a head and page size.
-template <int FMT, int NU, typename F>
+template <int FMT, int NU, int kDim, typename F>
 void WithMove(int chunks, F&& f) {
-  if (chunks <= 4) return f(Kv8EvictMoveKernel<FMT, NU, 1>);
-  if (chunks <= 8) return f(Kv8EvictMoveKernel<FMT, NU, 2>);
-  return f(Kv8EvictMoveKernel<FMT, NU, 4>);
+  if (chunks <= 4) return f(Kv8EvictMoveKernel<FMT, NU, kDim, 1>);
+  if (chunks <= 8) return f(Kv8EvictMoveKernel<FMT, NU, kDim, 2>);
+  return f(Kv8EvictMoveKernel<FMT, NU, kDim, 4>);
+}
+template <int FMT, typename F>
+void WithMove(const Kv8View& c, F&& f) {
+  if (c.dim == 64) return WithMove<FMT, 1, 64>(c.chunks, f);
+  if (c.dim < 64) return WithMove<FMT, 1, 0>(c.chunks, f);
+  if (c.dim == 128) return WithMove<FMT, 2, 128>(c.chunks, f);
+  if (c.dim < 128) return WithMove<FMT, 2, 0>(c.chunks, f);
+  return WithMove<FMT, 4, 0>(c.chunks, f);
 }
 template <typename F>
 void WithMove(const Kv8View& c, F&& f) {
-  const bool int8 = c.format == DSD_KV8_INT8;
-  if (c.dim <= 64) {
-    return int8 ? WithMove<DSD_KV8_INT8, 1>(c.chunks, f) : WithMove<DSD_KV8_E4M3, 1>(c.chunks, f);
-  }
-  if (c.dim <= 128) {
-    return int8 ? WithMove<DSD_KV8_INT8, 2>(c.chunks, f) : WithMove<DSD_KV8_E4M3, 2>(c.chunks, f);
-  }
-  return int8 ? WithMove<DSD_KV8_INT8, 4>(c.chunks, f) : WithMove<DSD_KV8_E4M3, 4>(c.chunks, f);
+  c.format == DSD_KV8_INT8 ? WithMove<DSD_KV8_INT8>(c, f) : WithMove<DSD_KV8_E4M3>(c, f);
 }
 
 }  // namespace
