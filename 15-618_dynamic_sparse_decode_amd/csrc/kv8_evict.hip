@@ -314,37 +314,37 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
 
 // ---- the move ---------------------------------------------------------------------
 
-// Where a kept token lies.
-struct Source {
-  int page;  // < 0: none
-  int off;
-  float key_scale;
-  float value_scale;
-};
-
 typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t I16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ unsigned Max16(unsigned x, unsigned y) {
   return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(U16x2, x),
                                                                 __builtin_bit_cast(U16x2, y)));
 }
 
-// The magnitudes of four codes, which order as their bytes do (0 for NaN).
+// The magnitudes of bytes 0 and 2 (odd: 1 and 3) of four codes, which order as the numbers
+// do (an e4m3 NaN's, 127, above all of them).
 template <int FMT>
-__device__ __forceinline__ unsigned Sizes4(unsigned w) {
+__device__ __forceinline__ unsigned Sizes2(unsigned w, bool odd) {
   if constexpr (FMT == DSD_KV8_INT8) {
-    const unsigned sign = (w >> 7) & 0x01010101u;
-    return (w ^ (sign * 0xffu)) + sign;
+    const unsigned high = odd ? w & 0xff00ff00u : (w << 8) & 0xff00ff00u;
+    const I16x2 x = __builtin_bit_cast(I16x2, high) >> 1;  // (-128 has a magnitude too)
+    const I16x2 zero = {0, 0};
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(x, zero - x));
   } else {
-    return (w & 0x7f7f7f7fu) & ~((NanBytes(w) >> 7) * 0xffu);
+    return (odd ? w >> 8 : w) & 0x007f007fu;
   }
 }
 template <int FMT>
 __device__ __forceinline__ double NumberOf(unsigned size) {
   if constexpr (FMT == DSD_KV8_INT8) {
-    return static_cast<double>(size);
+    return static_cast<double>(size >> 7);
   } else {
     return static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(size), 0));
   }
+}
+// The codes' magnitudes with 0 in place of NaN.
+__device__ __forceinline__ unsigned WithoutNan(unsigned w) {
+  return w & ~((NanBytes(w) >> 7) * 0xffu);
 }
 
 // The least scale whose largest code reaches `most`.
@@ -417,24 +417,35 @@ __device__ __forceinline__ unsigned Quick4(unsigned w, const float (&ratio)[4], 
   }
 }
 
+__device__ __forceinline__ float ReadLane(float x, int lane) {
+  return __uint_as_float(static_cast<unsigned>(
+      __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(x)), lane)));
+}
+
 // Grid (key heads * new pages, batch): one new page of one key head.  Waves 2 i have the
 // keys, 2 i + 1 the values of chunks i, i + kWaves / 2, ... of 16 tokens (U of them) in
 // registers, as codes: keys lane l unit l + 64 j (16 dims) of the chunk's [16][dim],
-// values lane l dims l + 64 j, all 16 tokens.  NU = ceil(dim / 64); kDim: head_dim where it
-// is 64 * NU, else 0.
+// values lane l dims l + 64 j, all 16 tokens; of the chunk's token l % 16 it has the place
+// and scale.  NU = ceil(dim / 64); kDim: head_dim where it is 64 * NU, else 0.
 template <int FMT, int NU, int kDim, int U>
 __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(16) uint8_t tile[];  // the new keys (for their mean)
   __shared__ double wave_most[8];
   __shared__ float key_scale;
   const Kv8View& c = a.c;
   const int D = kDim > 0 ? kDim : c.dim, units = D / 16, ps = c.page;
   const int head = blockIdx.x % c.heads, index = blockIdx.x / c.heads, r = blockIdx.y;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int waves = blockDim.x / kWave;
+  const bool is_key = (wave & 1) == 0;
+  auto chunk_of = [&](int u) { return wave / 2 + waves / 2 * u; };
   // (loads that do not wait for each other)
   const int* kept = a.kept + (static_cast<int64_t>(r) * c.heads + head) * a.keep + index * ps;
-  int place = 0;
-  if (static_cast<int>(threadIdx.x) < ps && index * ps + static_cast<int>(threadIdx.x) < a.keep) {
-    place = kept[threadIdx.x];
+  int place[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = 16 * chunk_of(u) + (lane & 15);
+    place[u] = i < ps && index * ps + i < a.keep ? kept[i] : -1;
   }
   Kv8Request q;
   const bool listed = Kv8ReadList(a.b, r, &q);
@@ -445,137 +456,140 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
     return;
   }
-  Source* source = reinterpret_cast<Source*>(smem);
-  uint8_t* tile = smem + sizeof(Source) * ps;  // the new keys (for their mean)
+  if (threadIdx.x == 0 && head == 0) c.token_counts[page] = count;
   const int64_t to = static_cast<int64_t>(page) * c.heads + head;
   const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
-  for (int i = threadIdx.x; i < ps; i += blockDim.x) {
-    if (i >= static_cast<int>(blockDim.x) && i < count) place = kept[i];
-    Source s = {-1, 0, 0.0f, 0.0f};
-    float weight = 0.0f;
-    if (i < count) {
-      const int slot = c.chunks == 1 ? place >> 4 : static_cast<int>(__umulhi(place >> 4, inverse));
-      s.off = place - slot * ps;
-      s.page = a.b.page_ids[q.list + slot];
-      const int64_t at = static_cast<int64_t>(s.page) * c.heads + head;
-      s.key_scale = c.key_scales[at];
-      s.value_scale = c.value_scales[at];
-      weight = a.weights[at * ps + s.off];
-    }
-    source[i] = s;
-    a.weights[to * ps + i] = weight;
-  }
-  if (threadIdx.x == 0 && head == 0) c.token_counts[page] = count;
-  __syncthreads();
-
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int waves = blockDim.x / kWave;
-  const bool is_key = (wave & 1) == 0;
   const int page_bytes = ps * D;
   unsigned w[U][NU][4];
+  float had[U];  // of the lane's token
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int chunk = wave / 2 + waves / 2 * u;
+    const int chunk = chunk_of(u);
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[u][j][i] = 0u;
     }
+    had[u] = 0.0f;
     if (chunk >= c.chunks) continue;
-    if (is_key) {
+    const int here = count - 16 * chunk;  // tokens of the chunk
+    const bool mine = (lane & 15) < here;
+    const int slot = c.chunks == 1 ? place[u] >> 4 : static_cast<int>(__umulhi(place[u] >> 4, inverse));
+    const int off = place[u] - slot * ps;
+    const int from = mine ? a.b.page_ids[q.list + slot] : 0;
+    const int64_t old = static_cast<int64_t>(from) * c.heads + head;
+    const int64_t begin =
+        !mine ? 0 : old * page_bytes + (is_key ? off * D : (off >> 4) * (16 * D) + (off & 15));
+    const int low = static_cast<int>(begin), high = static_cast<int>(begin >> 32);
+    if (here <= 0) {
+      // (a chunk behind the last token: zeros)
+    } else if (is_key) {
 #pragma unroll
       for (int j = 0; j < NU; ++j) {
-        const int i = lane + kWave * j;
-        if (kDim > 0 || i < D) {
-          const int token = i / units;
-          const Source s = source[16 * chunk + token];
-          if (s.page >= 0) {
-            const uint4 x = *reinterpret_cast<const uint4*>(
-                c.keys + (static_cast<int64_t>(s.page) * c.heads + head) * page_bytes + s.off * D +
-                16 * (i - token * units));
-            w[u][j][0] = x.x;
-            w[u][j][1] = x.y;
-            w[u][j][2] = x.z;
-            w[u][j][3] = x.w;
-          }
+        const int i = min(lane + kWave * j, D - 1), token = i / units;
+        const uint64_t at =
+            static_cast<uint64_t>(static_cast<unsigned>(__shfl(high, token, kWave))) << 32 |
+            static_cast<unsigned>(__shfl(low, token, kWave));
+        if (token < here && (kDim > 0 || lane + kWave * j < D)) {
+          const uint4 x = *reinterpret_cast<const uint4*>(c.keys + at + 16 * (i - token * units));
+          w[u][j][0] = x.x;
+          w[u][j][1] = x.y;
+          w[u][j][2] = x.z;
+          w[u][j][3] = x.w;
         }
       }
     } else {
+      // (all on their way at once: no branch between them, a token beyond the last is the
+      // last one's and masked)
+      unsigned code[16][NU];
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        const Source s = source[16 * chunk + t];
-        if (s.page >= 0) {
-          const uint8_t* p = c.values +
-                             (static_cast<int64_t>(s.page) * c.heads + head) * page_bytes +
-                             (s.off >> 4) * (16 * D) + (s.off & 15);
+        const int token = min(t, here - 1);
+        const uint64_t at =
+            static_cast<uint64_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, token))) << 32 |
+            static_cast<unsigned>(__builtin_amdgcn_readlane(low, token));
+        const uint8_t* p = c.values + at;
 #pragma unroll
-          for (int j = 0; j < NU; ++j) {
-            const int d = lane + kWave * j;
-            if (kDim > 0 || d < D) {
-              w[u][j][t >> 2] |= static_cast<unsigned>(p[d * 16]) << (8 * (t & 3));
-            }
-          }
+        for (int j = 0; j < NU; ++j) code[t][j] = p[min(lane + kWave * j, D - 1) * 16];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int have = min(max(here - 4 * k, 0), 4);
+        const unsigned mask = have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1u;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+          w[u][j][k] = (code[4 * k][j] | code[4 * k + 1][j] << 8 | code[4 * k + 2][j] << 16 |
+                        code[4 * k + 3][j] << 24) & mask;
         }
       }
+    }
+    if (mine) had[u] = (is_key ? c.key_scales : c.value_scales)[old];
+    if (is_key && lane < 16) {
+      a.weights[to * ps + 16 * chunk + lane] = mine ? a.weights[old * ps + off] : 0.0f;
     }
   }
   // The largest number: of a token's codes by their bytes, then of the tokens'.
   double most = 0.0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int chunk = wave / 2 + waves / 2 * u;
-    if (chunk >= c.chunks) continue;
-    if (is_key) {
+    if (chunk_of(u) >= c.chunks) continue;
+    auto by_tokens = [&](bool nan) {
+      double got = 0.0;
+      auto codes = [&](int j, int k) { return nan ? WithoutNan(w[u][j][k]) : w[u][j][k]; };
+      if (is_key) {
 #pragma unroll
-      for (int j = 0; j < NU; ++j) {
-        const int i = lane + kWave * j;
-        if (kDim > 0 || i < D) {
+        for (int j = 0; j < NU; ++j) {
           unsigned top = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const unsigned x = Sizes4<FMT>(w[u][j][k]);
-            top = Max16(top, Max16(x & 0x00ff00ffu, (x >> 8) & 0x00ff00ffu));
+            const unsigned x = codes(j, k);
+            top = Max16(top, Max16(Sizes2<FMT>(x, false), Sizes2<FMT>(x, true)));
           }
           top = max(top & 0xffffu, top >> 16);
-          most = fmax(most, NumberOf<FMT>(top) *
-                                static_cast<double>(source[16 * chunk + i / units].key_scale));
+          const int token = min(lane + kWave * j, D - 1) / units;
+          got = fmax(got, NumberOf<FMT>(top) * static_cast<double>(__shfl(had[u], token, kWave)));
+          if (FMT == DSD_KV8_E4M3 && top == 127u) got = INFINITY;
         }
-      }
-    } else {
-      // tokens 4 k + {0, 2} and 4 k + {1, 3}; then half of them from each lane's partner,
-      // until a lane has two tokens' of its 8 lanes, of which the wave has 8 groups
-      unsigned top[8];
+      } else {
+        // tokens 4 k + {0, 2} and 4 k + {1, 3}; then half of them from each lane's partner,
+        // until a lane has two tokens' of its 8 lanes, of which the wave has 8 groups
+        unsigned top[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        unsigned even = 0, odd = 0;
+        for (int k = 0; k < 4; ++k) {
+          top[2 * k] = top[2 * k + 1] = 0;
 #pragma unroll
-        for (int j = 0; j < NU; ++j) {
-          const unsigned x = Sizes4<FMT>(w[u][j][k]);
-          even = Max16(even, x & 0x00ff00ffu);
-          odd = Max16(odd, (x >> 8) & 0x00ff00ffu);
+          for (int j = 0; j < NU; ++j) {
+            const unsigned x = codes(j, k);
+            top[2 * k] = Max16(top[2 * k], Sizes2<FMT>(x, false));
+            top[2 * k + 1] = Max16(top[2 * k + 1], Sizes2<FMT>(x, true));
+          }
         }
-        top[2 * k] = even;
-        top[2 * k + 1] = odd;
-      }
 #pragma unroll
-      for (int half = 4; half >= 1; half >>= 1) {
-        const bool high = (lane & half) != 0;  // keeps the upper half
+        for (int half = 4; half >= 1; half >>= 1) {
+          const bool upper = (lane & half) != 0;  // keeps the upper half
 #pragma unroll
-        for (int k = 0; k < half; ++k) {
-          const unsigned give = high ? top[k] : top[k + half];
-          const unsigned keep = high ? top[k + half] : top[k];
-          top[k] = Max16(keep, static_cast<unsigned>(__shfl_xor(static_cast<int>(give), half, kWave)));
+          for (int k = 0; k < half; ++k) {
+            const unsigned give = upper ? top[k] : top[k + half];
+            const unsigned keep = upper ? top[k + half] : top[k];
+            top[k] = Max16(keep, static_cast<unsigned>(__shfl_xor(static_cast<int>(give), half, kWave)));
+          }
         }
-      }
 #pragma unroll
-      for (int o = 8; o < kWave; o <<= 1) {
-        top[0] = Max16(top[0], static_cast<unsigned>(__shfl_xor(static_cast<int>(top[0]), o, kWave)));
+        for (int o = 8; o < kWave; o <<= 1) {
+          top[0] = Max16(top[0], static_cast<unsigned>(__shfl_xor(static_cast<int>(top[0]), o, kWave)));
+        }
+        // top[0]: index lane & 7 of the eight
+        const int token = 4 * ((lane & 7) >> 1) + (lane & 1);
+        const unsigned t0 = top[0] & 0xffffu, t1 = top[0] >> 16;
+        got = fmax(NumberOf<FMT>(t0) * static_cast<double>(__shfl(had[u], token, kWave)),
+                   NumberOf<FMT>(t1) * static_cast<double>(__shfl(had[u], token + 2, kWave)));
+        if (FMT == DSD_KV8_E4M3 && (t0 == 127u || t1 == 127u)) got = INFINITY;
       }
-      // top[0]: index lane & 7 of the eight
-      const int token = 16 * chunk + 4 * ((lane & 7) >> 1) + (lane & 1);
-      most = fmax(most, NumberOf<FMT>(top[0] & 0xffffu) * static_cast<double>(source[token].value_scale));
-      most = fmax(most, NumberOf<FMT>(top[0] >> 16) * static_cast<double>(source[token + 2].value_scale));
-    }
+      return got;
+    };
+    double got = by_tokens(false);
+    if (FMT == DSD_KV8_E4M3 && __ballot(got == INFINITY) != 0) got = by_tokens(true);  // seldom
+    most = fmax(most, got);
   }
   most = WaveMost(most);
   if (lane == 0) wave_most[wave] = most;
@@ -590,50 +604,40 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   // Brought to it.
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int chunk = wave / 2 + waves / 2 * u;
+    const int chunk = chunk_of(u);
     if (chunk >= c.chunks) continue;
-    // lane t: of token t % 16
-    const Source mine = source[16 * chunk + (lane & 15)];
     bool fast;
-    const float ratio = RatioOf<FMT>(is_key ? mine.key_scale : mine.value_scale, scale, &fast);
+    const float ratio = RatioOf<FMT>(had[u], scale, &fast);
     const bool all_fast = __ballot(!fast) == 0;
-    const bool same = __ballot(mine.page >= 0 && ratio != 1.0f) == 0 && all_fast;
+    const bool same =
+        all_fast && __ballot((lane & 15) < count - 16 * chunk && ratio != 1.0f) == 0;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int i = lane + kWave * j;
-      if (kDim == 0 && i >= D) continue;
       if (!same) {
-        const int token = is_key ? i / units : 0;
+        // of the token that the lane's keys are of
+        const int token = min(i, D - 1) / units;
+        const float key_ratio = is_key ? __shfl(ratio, token, kWave) : 0.0f;
+        const float key_had = is_key ? __shfl(had[u], token, kWave) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float by[4];
           bool sure = false;
           unsigned x = 0;
           if (all_fast) {
-            if (is_key) {
-              const float mine_by = __shfl(ratio, token, kWave);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) by[e] = mine_by;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                by[e] = __uint_as_float(static_cast<unsigned>(__builtin_amdgcn_readlane(
-                    static_cast<int>(__float_as_uint(ratio)), 4 * k + e)));
-              }
-            }
+            for (int e = 0; e < 4; ++e) by[e] = is_key ? key_ratio : ReadLane(ratio, 4 * k + e);
             x = Quick4<FMT>(w[u][j][k], by, &sure);
           }
           if (!sure) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              by[e] = is_key ? source[16 * chunk + token].key_scale
-                             : source[16 * chunk + 4 * k + e].value_scale;
-            }
+            for (int e = 0; e < 4; ++e) by[e] = is_key ? key_had : ReadLane(had[u], 4 * k + e);
             x = Slow4<FMT>(w[u][j][k], by, scale);
           }
           w[u][j][k] = x;
         }
       }
+      if (kDim == 0 && i >= D) continue;
       const uint4 out = make_uint4(w[u][j][0], w[u][j][1], w[u][j][2], w[u][j][3]);
       const int64_t at = to * page_bytes + chunk * 16 * D + 16 * i;
       *reinterpret_cast<uint4*>((is_key ? c.keys : c.values) + at) = out;
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
 }
 
 size_t MoveLdsBytes(const Kv8View& c) {
-  return sizeof(Source) * c.page + static_cast<size_t>(c.page) * c.dim;
+  return c.summaries != nullptr ? static_cast<size_t>(c.page) * c.dim : 0;
 }
 
 // Calls f with the kernel of a head and page size.
