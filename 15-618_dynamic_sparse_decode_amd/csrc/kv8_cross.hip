@@ -9,12 +9,29 @@
 namespace dsdk {
 namespace {
 
+// The request whose list is the i-th longest, so that long ones are not begun last (up to
+// 64 requests, a lane each; more are taken as they come).  All lanes of a wave.
+__device__ __forceinline__ int ByLength(const dsd_kv8_batch& b, int i) {
+  if (b.batch == 1 || b.batch > kWave) return i;
+  const int lane = threadIdx.x & (kWave - 1);
+  Kv8Request q;
+  int pages = -1;
+  if (lane < b.batch) pages = Kv8ReadList(b, lane, &q) ? q.pages : 0;
+  int before = 0;
+  for (int k = 0; k < b.batch; ++k) {
+    const int other = __builtin_amdgcn_readlane(pages, k);
+    before += other > pages || (other == pages && k < lane) ? 1 : 0;
+  }
+  return __ffsll(__ballot(lane < b.batch && before == i)) - 1;
+}
+
 // Grid (key heads * blocks of 128 rows, batch, pieces).
 template <typename T, int FMT, int NU, int kDim>
 __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void
 Kv8CrossKernel(Kv8AttendArgs a, Plan plan) {
   extern __shared__ __align__(16) _Float16 smem[];
-  PromptBlock<T, FMT, NU, kDim, false, false>(a, plan, blockIdx.x, blockIdx.y, blockIdx.z, smem);
+  PromptBlock<T, FMT, NU, kDim, false, false>(a, plan, blockIdx.x, ByLength(a.b, blockIdx.y),
+                                              blockIdx.z, smem);
 }
 
 // Calls f with the kernel of a head size.
