@@ -9,6 +9,9 @@
 namespace dsdk {
 namespace {
 
+constexpr int kWideWaves = 8;
+constexpr int kWideRows = 32 * kWideWaves;
+
 // The request whose list is the i-th longest, so that long ones are not begun last (up to
 // 64 requests, a lane each; more are taken as they come).  All lanes of a wave.
 __device__ __forceinline__ int ByLength(const dsd_kv8_batch& b, int i) {
@@ -25,32 +28,54 @@ __device__ __forceinline__ int ByLength(const dsd_kv8_batch& b, int i) {
   return __ffsll(__ballot(lane < b.batch && before == i)) - 1;
 }
 
-// Grid (key heads * blocks of 128 rows, batch, pieces).
-template <typename T, int FMT, int NU, int kDim>
-__global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void
-Kv8CrossKernel(Kv8AttendArgs a, Plan plan) {
-  extern __shared__ __align__(16) _Float16 smem[];
-  PromptBlock<T, FMT, NU, kDim, false, false>(a, plan, blockIdx.x, ByLength(a.b, blockIdx.y),
-                                              blockIdx.z, smem);
+// Eight waves to a workgroup where a request has more than 128 rows: the halves of a group
+// of 64 tokens then go to LDS, whose writes are a quarter of its reads' rate (31 bytes a
+// cycle measured), once for 256 rows.  4096 tokens over 8192: 543 us, four waves 604; 1024
+// over 8192: 240 and 217 (a workgroup a CU either way), 512: 237 and 135.  16-bit rows of
+// heads of up to 128 (others' registers hold one workgroup of four waves a CU).
+template <typename T>
+bool Wide(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+  const int group = q_heads / c.heads;
+  const int64_t rows = static_cast<int64_t>(b.max_tokens) * group;
+  const int64_t blocks = (rows + kWideRows - 1) / kWideRows * c.heads * b.batch;
+  return sizeof(T) == 2 && c.dim <= 128 && rows > kRows && blocks >= 256;
 }
 
-// Calls f with the kernel of a head size.
+// Grid (key heads * blocks of 32 W rows, batch, pieces).
+template <typename T, int FMT, int NU, int kDim, int W>
+__global__ __launch_bounds__(W* kWave, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void
+Kv8CrossKernel(Kv8AttendArgs a, Plan plan) {
+  extern __shared__ __align__(16) _Float16 smem[];
+  PromptBlock<T, FMT, NU, kDim, false, false, W>(a, plan, blockIdx.x, ByLength(a.b, blockIdx.y),
+                                                 blockIdx.z, smem);
+}
+
+// Calls f with the kernel of a head size, and its threads.
 template <typename T, int FMT, typename F>
-void WithKernel(int dim, F&& f) {
-  if (dim == 64) return f(Kv8CrossKernel<T, FMT, 1, 64>);
-  if (dim < 64) return f(Kv8CrossKernel<T, FMT, 1, 0>);
-  if (dim == 128) return f(Kv8CrossKernel<T, FMT, 2, 128>);
-  if (dim < 128) return f(Kv8CrossKernel<T, FMT, 2, 0>);
-  return f(Kv8CrossKernel<T, FMT, 4, 0>);
+void WithKernel(int dim, bool wide, F&& f) {
+  if constexpr (sizeof(T) == 2) {
+    if (wide) {
+      if (dim == 64) return f(Kv8CrossKernel<T, FMT, 1, 64, kWideWaves>, kWideWaves * kWave);
+      if (dim < 64) return f(Kv8CrossKernel<T, FMT, 1, 0, kWideWaves>, kWideWaves * kWave);
+      if (dim == 128) return f(Kv8CrossKernel<T, FMT, 2, 128, kWideWaves>, kWideWaves * kWave);
+      return f(Kv8CrossKernel<T, FMT, 2, 0, kWideWaves>, kWideWaves * kWave);
+    }
+  }
+  if (dim == 64) return f(Kv8CrossKernel<T, FMT, 1, 64, kPromptWaves>, kThreads);
+  if (dim < 64) return f(Kv8CrossKernel<T, FMT, 1, 0, kPromptWaves>, kThreads);
+  if (dim == 128) return f(Kv8CrossKernel<T, FMT, 2, 128, kPromptWaves>, kThreads);
+  if (dim < 128) return f(Kv8CrossKernel<T, FMT, 2, 0, kPromptWaves>, kThreads);
+  return f(Kv8CrossKernel<T, FMT, 4, 0, kPromptWaves>, kThreads);
 }
 
 template <typename T, int FMT>
 void Launch(const Kv8AttendArgs& a, hipStream_t stream) {
-  Plan p = PromptPlan(a.c, a.b, a.q_heads);
+  const bool wide = Wide<T>(a.c, a.b, a.q_heads);
+  Plan p = PromptPlan(a.c, a.b, a.q_heads, wide ? kWideRows : kRows);
   PlaceParts(&p, a);
   const dim3 grid(a.c.heads * p.blocks, a.b.batch, p.pieces);
-  WithKernel<T, FMT>(a.c.dim, [&](auto kernel) {
-    kernel<<<grid, kThreads, PromptLdsBytes(a.c.dim), stream>>>(a, p);
+  WithKernel<T, FMT>(a.c.dim, wide, [&](auto kernel, int threads) {
+    kernel<<<grid, threads, PromptLdsBytes(a.c.dim), stream>>>(a, p);
   });
   DSD_HIP_CHECK(hipGetLastError());
   Merge<T>(a, p, stream);
@@ -64,12 +89,15 @@ void LaunchType(const Kv8AttendArgs& a, hipStream_t stream) {
 
 template <typename T, int FMT>
 void PreloadDim(const Kv8View& c) {
-  WithKernel<T, FMT>(c.dim, [&](auto kernel) {
-    PreloadKernel(kernel);
-    DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(PromptLdsBytes(c.dim))));
-  });
+  for (const bool wide : {false, true}) {
+    if (wide && c.dim > 128) continue;
+    WithKernel<T, FMT>(c.dim, wide, [&](auto kernel, int) {
+      PreloadKernel(kernel);
+      DSD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(PromptLdsBytes(c.dim))));
+    });
+  }
 }
 
 template <typename T>

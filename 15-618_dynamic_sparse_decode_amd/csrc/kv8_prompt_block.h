@@ -13,7 +13,7 @@ typedef float F32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPromptWaves = 4;
 constexpr int kThreads = kPromptWaves * kWave;
-constexpr int kRows = 32 * kPromptWaves;
+constexpr int kRows = 32 * kPromptWaves;  // of a workgroup of so many waves
 constexpr int kGroup = 64;             // tokens
 // The running maxima follow a row's once it is 2^4 ahead of them (following it at
 // once, 64 products an update, cost 6%): weights reach 2^(11 + 4).
@@ -52,7 +52,7 @@ inline size_t PromptLdsBytes(int dim) {
          2 * 4 * sizeof(ChunkInfo) + sizeof(int) * dim;
 }
 
-// One piece of request r's list for a block of 128 rows (unit: key heads * blocks, the
+// One piece of request r's list for a block of 32 W rows (unit: key heads * blocks, the
 // key head fastest, the last rows first).  kCausal: a row sees its request's tokens up
 // to its own; else all of the list's, each page's count of them.  kJoin: a later
 // launch joins the piece with others.  Wave w
@@ -60,10 +60,14 @@ inline size_t PromptLdsBytes(int dim) {
 // row n.  Logits come out transposed, S^T = K Q^T in two tiles of 32 tokens
 // dealt so that lane (n, h) holds all 16 tokens of chunk 2 t + h for row n, and
 // go into O^T = V^T P^T as they stand.
-template <typename T, int FMT, int NU, int kDim, bool kCausal, bool kJoin>
+template <typename T, int FMT, int NU, int kDim, bool kCausal, bool kJoin, int W = kPromptWaves>
 __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& plan, int unit,
                                             int r, int piece, _Float16* smem) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>;
+  constexpr int kBlockThreads = W * kWave, kBlockRows = 32 * W;
+  // 16-byte units of a group's keys (values) that a thread turns
+  constexpr int NJ = NU * kThreads > kBlockThreads ? NU * kThreads / kBlockThreads : 1;
+  constexpr bool kAllUnits = kDim > 0 && 4 * kDim == NJ * kBlockThreads;
   constexpr int KS = 4 * NU, NT = 2 * NU;
   constexpr int kMfma = 0x008, kDsRead = 0x100;  // (the scheduler's groups)
   constexpr int kAhead = 4;
@@ -72,10 +76,10 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int n = lane & 31, h = lane >> 5;
   const int head = unit % c.heads;
-  const int first = (plan.blocks - 1 - unit / c.heads) * kRows;
+  const int first = (plan.blocks - 1 - unit / c.heads) * kBlockRows;
   const int group = plan.group;
   Span s;
-  if (!FindSpan(a, group, r, first, kRows, &s)) return;
+  if (!FindSpan(a, group, r, first, kBlockRows, &s)) return;
   const int pieces = Pieces(plan, s);
   const bool parts = kJoin || pieces > 1;
   if (piece >= pieces) return;
@@ -90,7 +94,7 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
 
   if (!kCausal && s.chunks == 0) {  // no token: zeros
     const int quads = D / 4;
-    for (int i = threadIdx.x; i < kRows * quads; i += kThreads) {
+    for (int i = threadIdx.x; i < kBlockRows * quads; i += kBlockThreads) {
       const int row = first + i / quads, d = 4 * (i % quads);
       if (row >= s.rows) break;
       const int token = row / group;
@@ -122,7 +126,7 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
     slot0 = 4 * g0 / c.chunks;
     slots = (min(4 * stage_end, s.chunks) - 1) / c.chunks + 1 - slot0;
     bool mine = false;
-    for (int i = threadIdx.x; i < slots; i += kThreads) {
+    for (int i = threadIdx.x; i < slots; i += kBlockThreads) {
       info[i] = ReadPage(a, s, head, slot0 + i);
       mine = mine || (kCausal ? info[i].tokens == 0 : info[i].tokens < c.page);
     }
@@ -138,14 +142,14 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
   };
 
   // A group's codes on their way to LDS: a chunk's keys and its values are dim
-  // units of 16 bytes each, at the same offset of both arrays, and thread i has
-  // units i + 256 j of the group's four chunks.
-  uint4 kw[NU], vw[NU];
+  // units of 16 bytes each, at the same offset of both arrays, and thread i has every
+  // kBlockThreads-th unit of the group's four chunks.
+  uint4 kw[NJ], vw[NJ];
   auto fetch = [&](int grp) {
 #pragma unroll
-    for (int j = 0; j < NU; ++j) {
-      const int i = threadIdx.x + kThreads * j;
-      if (kDim > 0 || i < 4 * D) {
+    for (int j = 0; j < NJ; ++j) {
+      const int i = threadIdx.x + kBlockThreads * j;
+      if (kAllUnits || i < 4 * D) {
         const int k = i / D;
         int sub;
         const int page = place(4 * grp + k, &sub).page;
@@ -167,9 +171,9 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
     }
     const bool tail = bad || (kCausal && (grp + 1) * kGroup > s.q.past + s.q.n);
 #pragma unroll
-    for (int j = 0; j < NU; ++j) {
-      const int i = threadIdx.x + kThreads * j;
-      if (kDim > 0 || i < 4 * D) {
+    for (int j = 0; j < NJ; ++j) {
+      const int i = threadIdx.x + kBlockThreads * j;
+      if (kAllUnits || i < 4 * D) {
         // as keys: 16 dims of token t; as values: 16 tokens of dim d
         const int t = i / units, u = i - t * units;
         const int k = i / D, d = i - k * D;
@@ -219,7 +223,7 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
   const int q_head = head * group + (there ? row - token * group : 0);
   F16x8 q[KS][NQ];
   float to_logit;  // what a product with codes lacks but the page's scale; >= 0
-  for (int i = threadIdx.x; i < D; i += kThreads) nan_from[i] = 0x7fffffff;
+  for (int i = threadIdx.x; i < D; i += kBlockThreads) nan_from[i] = 0x7fffffff;
   const bool bad_here = stage(begin);
   {
     const T* qp = static_cast<const T*>(a.q) + (s.q.row0 + token) * a.q_stride +
@@ -476,14 +480,14 @@ __device__ __forceinline__ void PromptBlock(const Kv8AttendArgs& a, const Plan& 
 }
 
 constexpr int kPromptTarget = 512;  // workgroups the chip runs at once
-inline Plan PromptPlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads) {
+inline Plan PromptPlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, int block = kRows) {
   Plan p;
   p.group = q_heads / c.heads;
   p.rows = static_cast<int64_t>(b.max_tokens) * p.group;
-  p.block = kRows;
-  p.blocks = static_cast<int>((p.rows + kRows - 1) / kRows);
+  p.block = block;
+  p.blocks = static_cast<int>((p.rows + block - 1) / block);
   const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
-  const int64_t most = kPromptTarget / std::max<int64_t>(units, 1);
+  const int64_t most = kPromptTarget * kRows / block / std::max<int64_t>(units, 1);
   // A group takes a workgroup about 1.5 us; pieces cost the second launch, 5 us,
   // and a write and a read of their sums at about 3 TB/s.
   const int64_t groups = ListGroups(c, b);

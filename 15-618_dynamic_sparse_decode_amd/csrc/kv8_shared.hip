@@ -43,12 +43,22 @@ __global__ __launch_bounds__(kAttendWaves* kWave, NU <= 2 ? 2 : 1) void Kv8Share
   AttendBlock<T, FMT, NU, kDim, kAttendWaves, true>(a, p, at.unit, at.list, at.piece, lds);
 }
 
-// Prefixes of many rows.  Grid (key heads * blocks of 128 rows, groups, pieces).
+// The same for prefixes of many rows, 128 a workgroup: their workgroups are bound by the
+// matrix and vector units, the own lists' by HBM, so one launch runs them side by side.
 template <typename T, int FMT, int NU, int kDim>
 __global__ __launch_bounds__(kThreads, NU <= 2 && sizeof(T) == 2 ? 2 : 1) void
-Kv8SharedRowsKernel(Kv8AttendArgs a, Plan plan) {
-  extern __shared__ __align__(16) _Float16 smem[];
-  PromptBlock<T, FMT, NU, kDim, false, true>(a, plan, blockIdx.x, blockIdx.y, blockIdx.z, smem);
+Kv8SharedRowsKernel(SharedArgs s) {
+  extern __shared__ __align__(16) float lds[];
+  const int i = blockIdx.x;
+  if (i < s.pre_items) {
+    const Item at = ItemOf(i, s.pre.c.heads * s.pre_plan.blocks, s.pre.b.batch);
+    PromptBlock<T, FMT, NU, kDim, false, true>(s.pre, s.pre_plan, at.unit, at.list, at.piece,
+                                               reinterpret_cast<_Float16*>(lds));
+  } else {
+    const Item at = ItemOf(i - s.pre_items, s.own.c.heads * s.own_plan.blocks, s.own.b.batch);
+    AttendBlock<T, FMT, NU, kDim, kAttendWaves, true>(s.own, s.own_plan, at.unit, at.list, at.piece,
+                                                      lds);
+  }
 }
 
 // The group of request r, -1: none (two: reported).  All lanes of a wave.
@@ -187,6 +197,8 @@ constexpr int64_t kMostItems = 0x800000;
 
 size_t SlotBytes(const Kv8View& c) { return sizeof(float) * c.dim + sizeof(PieceStats); }
 
+size_t RowsLdsBytes(int dim) { return std::max(PromptLdsBytes(dim), AttendLdsBytes(dim)); }
+
 // ---- launches -----------------------------------------------------------------------
 
 #define DSD_WITH_DIM(KERNEL)                            \
@@ -211,18 +223,17 @@ template <typename T, int FMT>
 void Launch(SharedPlan m, hipStream_t stream) {
   SharedArgs& s = m.s;
   const int dim = s.own.c.dim;
-  s.pre_items = m.many ? 0 : static_cast<int>(Items(s.pre.c, s.pre_plan, s.pre.b));
-  const int own_items = static_cast<int>(Items(s.own.c, s.own_plan, s.own.b));
+  s.pre_items = static_cast<int>(Items(s.pre.c, s.pre_plan, s.pre.b));
+  const int items = s.pre_items + static_cast<int>(Items(s.own.c, s.own_plan, s.own.b));
   if (m.many) {
-    const dim3 grid(s.own.c.heads * s.pre_plan.blocks, s.pre.b.batch, s.pre_plan.pieces);
     WithSharedRows<T, FMT>(dim, [&](auto kernel) {
-      kernel<<<grid, kThreads, PromptLdsBytes(dim), stream>>>(s.pre, s.pre_plan);
+      kernel<<<items, kThreads, RowsLdsBytes(dim), stream>>>(s);
     });
-    DSD_HIP_CHECK(hipGetLastError());
+  } else {
+    WithShared<T, FMT>(dim, [&](auto kernel) {
+      kernel<<<items, kAttendWaves * kWave, AttendLdsBytes(dim), stream>>>(s);
+    });
   }
-  WithShared<T, FMT>(dim, [&](auto kernel) {
-    kernel<<<s.pre_items + own_items, kAttendWaves * kWave, AttendLdsBytes(dim), stream>>>(s);
-  });
   DSD_HIP_CHECK(hipGetLastError());
   Kv8JoinKernel<T><<<dim3(s.own.q_heads, s.own.b.batch), 256, 0, stream>>>(s);
   DSD_HIP_CHECK(hipGetLastError());
@@ -243,7 +254,7 @@ void PreloadDim(const Kv8View& c) {
                                       static_cast<int>(lds)));
   };
   WithShared<T, FMT>(c.dim, [&](auto kernel) { load(kernel, AttendLdsBytes(c.dim)); });
-  WithSharedRows<T, FMT>(c.dim, [&](auto kernel) { load(kernel, PromptLdsBytes(c.dim)); });
+  WithSharedRows<T, FMT>(c.dim, [&](auto kernel) { load(kernel, RowsLdsBytes(c.dim)); });
 }
 
 template <typename T>
