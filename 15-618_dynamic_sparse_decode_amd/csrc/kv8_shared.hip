@@ -77,20 +77,33 @@ __device__ __forceinline__ int GroupOf(const Kv8AttendArgs& pre, int r) {
   return claims == 1 ? group : -1;
 }
 
-// A row's pieces joined, a workgroup a row.  Grid (query heads, batch).
+// A row's pieces joined, a workgroup a row.  Grid (query heads, batch).  All of the row's
+// slots are asked for before it is known which of them have pieces.
 template <typename T>
 __global__ __launch_bounds__(256) void Kv8JoinKernel(SharedArgs s) {
   __shared__ float factor[kMostPieces];
   __shared__ Power last;
   __shared__ int counts[2];
   __shared__ F32x4 part_sum[256];
-  const Kv8View& c = s.own.c;
-  const int D = c.dim, quads = D / 4;
+  const int D = s.own.c.dim, quads = D / 4;
   const int r = blockIdx.y, q_head = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t slot0 = (static_cast<int64_t>(r) * c.heads * s.own_plan.group + q_head) *
-                        s.own_plan.stride;
+  const int stride = s.own_plan.stride, base = s.own_plan.base;
+  const int64_t slot0 =
+      (static_cast<int64_t>(r) * s.own.c.heads * s.own_plan.group + q_head) * stride;
+  const int shares = 256 / quads;  // threads per quad
+  const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
+  const float* part = s.own_plan.part + slot0 * D + d;
+  constexpr int kAhead = 4;
+  F32x4 x[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int z = share + i * shares;
+    if (share < shares && z < stride) x[i] = *reinterpret_cast<const F32x4*>(part + z * D);
+  }
   if (threadIdx.x < kWave) {
+    PieceStats st = {-INFINITY, -1.0f, 0.0f};
+    if (lane < stride) st = s.own_plan.stats[slot0 + lane];
     Span span;
     int n_pre = 0, n_own = 0;
     const int group = GroupOf(s.pre, r);
@@ -98,28 +111,28 @@ __global__ __launch_bounds__(256) void Kv8JoinKernel(SharedArgs s) {
       n_pre = Pieces(s.pre_plan, span);
     }
     if (FindSpan(s.own, s.own_plan.group, r, 0, 1, &span)) n_own = Pieces(s.own_plan, span);
-    PieceStats st = {-INFINITY, -1.0f, 0.0f};
-    if (lane < n_pre + n_own) {
-      st = s.own_plan.stats[slot0 + (lane < n_pre ? lane : s.own_plan.base + lane - n_pre)];
-    }
+    const bool has = lane < n_pre || (lane >= base && lane < base + n_own);
+    if (!has) st = {-INFINITY, -1.0f, 0.0f};
     Power to_out;
     factor[lane] = JoinFactor<kWave>(st, !(st.l < 0.0f), &to_out);
     if (lane == 0) {
       last = to_out;
       counts[0] = n_pre;
-      counts[1] = n_own;
+      counts[1] = base + n_own;
     }
   }
   __syncthreads();
-  const int n_pre = counts[0], n = n_pre + counts[1];
-  const int shares = 256 / quads;  // threads per quad
-  const int share = threadIdx.x / quads, d = 4 * (threadIdx.x - share * quads);
+  const int n_pre = counts[0], end = counts[1];
   F32x4 o = {0, 0, 0, 0};
   if (share < shares) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int z = share + i * shares;
+      if (z < n_pre || (z >= base && z < end)) o += x[i] * factor[z];
+    }
 #pragma unroll 4
-    for (int z = share; z < n; z += shares) {
-      const int64_t slot = slot0 + (z < n_pre ? z : s.own_plan.base + z - n_pre);
-      o += *reinterpret_cast<const F32x4*>(s.own_plan.part + slot * D + d) * factor[z];
+    for (int z = share + kAhead * shares; z < end; z += shares) {
+      if (z < n_pre || z >= base) o += *reinterpret_cast<const F32x4*>(part + z * D) * factor[z];
     }
   }
   part_sum[threadIdx.x] = o;
@@ -177,13 +190,21 @@ SharedPlan MakePlan(const Kv8AttendArgs& own, const dsd_kv8_prefix& prefix) {
   auto cut = [&](Plan* p, int64_t groups, int64_t length, int64_t at_most) {
     CutLists(p, groups, std::min((groups + length - 1) / length, at_most), 1);
   };
-  // (Rows in blocks of 128 run in a launch of their own.)
-  const int64_t pre = pre_units * pre_groups, all = own_units * own_groups + (m.many ? 0 : pre);
+  const int64_t pre = pre_units * pre_groups, own_all = own_units * own_groups;
+  const int64_t all = own_all + (m.many ? 0 : pre);
   const int64_t length = std::max<int64_t>((all + kAttendTarget - 1) / kAttendTarget, kAttendWaves);
   cut(&s.own_plan, own_groups, length, most / 2);
-  cut(&s.pre_plan, pre_groups,
-      m.many ? std::max<int64_t>((pre + kPromptTarget - 1) / kPromptTarget, 1) : length,
-      most - s.own_plan.pieces);
+  int64_t pre_length = length;
+  if (m.many) {
+    // Blocks of 128 rows: one workgroup a CU beside the own lists' (a group of 64 tokens
+    // 2.3 us) or two that the own lists' follow (2.45 us, which at 3.8 TB/s take what is
+    // left).  64 requests behind 32768 tokens, own lists of 200-2000: 82 and 93 us.
+    const double step = static_cast<double>(pre) / kPromptTarget;
+    const double own_us = static_cast<double>(own_all) * 128 * c.dim / 3.8e6;
+    const int64_t target = own_us > (2 * 2.3 - 2.45) * step ? kPromptTarget / 2 : kPromptTarget;
+    pre_length = std::max<int64_t>((pre + target - 1) / target, 1);
+  }
+  cut(&s.pre_plan, pre_groups, pre_length, most - s.own_plan.pieces);
   s.pre_plan.stride = s.own_plan.stride = s.pre_plan.pieces + s.own_plan.pieces;
   s.own_plan.base = s.pre_plan.pieces;
   return m;
