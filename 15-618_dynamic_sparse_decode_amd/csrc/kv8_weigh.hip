@@ -23,9 +23,11 @@ __global__ __launch_bounds__(kAttendWaves* kWave, NU <= 2 ? 2 : 1) void Kv8Atten
 }
 
 // Grid (shares of a list, key heads, batch): a wave has kBlocks blocks of 64 tokens at a
-// time on their way, lane l their place l.
+// time on their way, lane l their place l; the first ones' logits and pages are asked for
+// before the rows' sums are formed.
 constexpr int kRowTile = 64;
 constexpr int kBlocks = 4;
+constexpr int kFirstRows = 4;
 __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, const float* logits,
                                                       float* weights) {
   __shared__ float row_base[kRowTile], row_inv[kRowTile];
@@ -38,10 +40,31 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
   const int first = static_cast<int>(blockIdx.x) * 4 * kBlocks;
   if (first >= blocks) return;
   const int pieces = Pieces(p, s);
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
   const float* from = logits + LogitBlock(a, p, head, r, s.q.list, 0) +
                       ((lane >> 2 & 3) * 4 + (lane >> 4)) * p.group * 4 + (lane & 3);
+  const int block_floats = 64 * p.group;
   for (int row0 = 0; row0 < p.group; row0 += kRowTile) {
     const int rows = min(kRowTile, p.group - row0);
+    float y[kFirstRows][kBlocks];
+    int page[kBlocks], off[kBlocks];
+    auto logit = [&](int b0, int k, int i) {  // (of a block behind the last: the last one's)
+      return from[static_cast<int64_t>(min(b0 + k, blocks - 1)) * block_floats +
+                  4 * (row0 + min(i, rows - 1))];
+    };
+    auto fetch = [&](int b0) {
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int at = min((b0 + k) * 64 + lane, s.q.pages * c.page - 1);
+        const int slot = c.chunks == 1 ? at >> 4 : static_cast<int>(__umulhi(at >> 4, inverse));
+        off[k] = at - slot * c.page;
+        page[k] = a.b.page_ids[s.q.list + slot];
+#pragma unroll
+        for (int i = 0; i < kFirstRows; ++i) y[i][k] = logit(b0, k, i);
+      }
+    };
+    int b0 = first + wave * kBlocks;
+    fetch(min(b0, blocks - 1));
     __syncthreads();
     for (int i = wave; i < rows; i += 4) {
       PieceStats st = {-INFINITY, -1.0f, 0.0f};
@@ -60,25 +83,35 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
       }
     }
     __syncthreads();
-    for (int b0 = first + wave * kBlocks; b0 < blocks; b0 += gridDim.x * 4 * kBlocks) {
+    for (; b0 < blocks; b0 += gridDim.x * 4 * kBlocks) {
+      if (b0 != first + wave * kBlocks) fetch(b0);
+      int count[kBlocks];
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        count[k] = InPool(page[k], c.capacity) ? c.token_counts[page[k]] : 0;
+      }
       float w[kBlocks] = {};
-      const float* x = from + (static_cast<int64_t>(b0) * 64 * p.group + row0 * 4);
-#pragma unroll 4
-      for (int i = 0; i < rows; ++i) {
-        const float base = row_base[i], inv = row_inv[i];
+#pragma unroll
+      for (int i = 0; i < kFirstRows; ++i) {
+        if (i >= rows) break;
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
-          const float y = b0 + k < blocks ? x[k * 64 * p.group + 4 * i] : 0.0f;
-          w[k] = fmaf(Exp2(y - base), inv, w[k]);
+          w[k] = fmaf(Exp2(y[i][k] - row_base[i]), row_inv[i], w[k]);
+        }
+      }
+#pragma unroll 4
+      for (int i = kFirstRows; i < rows; ++i) {
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+          w[k] = fmaf(Exp2(logit(b0, k, i) - row_base[i]), row_inv[i], w[k]);
         }
       }
 #pragma unroll
       for (int k = 0; k < kBlocks; ++k) {
-        const int at = (b0 + k) * 64 + lane, slot = at / c.page, off = at - slot * c.page;
-        if (slot >= s.q.pages) continue;
-        const int page = a.b.page_ids[s.q.list + slot];
-        if (!InPool(page, c.capacity) || off >= c.token_counts[page]) continue;
-        unsafeAtomicAdd(weights + (static_cast<int64_t>(page) * c.heads + head) * c.page + off, w[k]);
+        if ((b0 + k) * 64 + lane < s.q.pages * c.page && off[k] < count[k]) {
+          unsafeAtomicAdd(weights + (static_cast<int64_t>(page[k]) * c.heads + head) * c.page + off[k],
+                          w[k]);
+        }
       }
     }
   }
