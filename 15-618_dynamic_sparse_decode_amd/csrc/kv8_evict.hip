@@ -221,9 +221,9 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
 
   // The count-th best place: of those whose digits so far are its own the next digit is
   // counted, until few are left, which rank themselves.
-  unsigned key = kGone;
+  unsigned key = f.count > 0 ? kGone : kAlways;  // (all are kept, or none)
   int last = -1;  // of the places with its key the last that is kept
-  if (f.count < f.held) {
+  if (f.count > 0 && f.count < f.held) {
     int left = f.count;
     unsigned key_known = 0, key_mask = 0;  // the digits so far, and which bits they are
     unsigned place_known = 0, place_mask = 0;

@@ -829,7 +829,7 @@ int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* bat
  * the lower place first among equals (NaN counts as larger than all numbers); first +
  * recent <= keep.  A list of no more is kept whole.  The lists are those of the requests
  * alone that shall be cut; a list's pages stay as they are (others may share them).
- * The kept tokens go, in their order, to new pages, which the lists must not name:
+ * The kept tokens go, in their order, to new pages, each given once and named by no list:
  * request r's are new_page_ids[r * new_stride ..], device memory, as many as its kept
  * tokens fill (new_stride at least ceil(keep / page_size)); entries behind those are not
  * read.  A new page's scale is the least that the largest of its kept numbers (code *

@@ -182,6 +182,27 @@ def test_evict(gpu, case, style, fmt):
             assert torch.equal(was.view(torch.uint8), now.view(torch.uint8))
 
 
+@pytest.mark.parametrize("held", [0, 1, 16, 500, 9000, 40000])
+def test_evict_keeps_nothing_or_one(gpu, held):
+    """A budget of no token empties every list, one of a token keeps one, whatever the
+    lists' lengths; neither writes more than it says."""
+    import torch
+    pages = -(-held // 16)
+    rng = np.random.default_rng(held)
+    pair = Pair(gpu, 1, 16, 16, pages + 2)
+    pair.fill(1)
+    if held % 16:
+        pair.set_counts(pages - 1, held % 16)
+    lists, new = [list(range(pages)), []], [[pages], [pages + 1]]
+    for keep, recent in ((0, 0), (1, 0), (1, 1)):
+        weights = some_weights(rng, pair.model, "spread")
+        given, before = weights.clone(), snapshot(pair)
+        counts, kept = evict(pair, Batch(gpu, lists), keep, 0, recent, weights, device(new))
+        want = model_evict(pair, lists, keep, 0, recent, given, new)
+        check_evict(pair, lists, new, (weights, counts, kept), want, before)
+        assert counts.tolist() == [min(held, keep), 0]
+
+
 @pytest.mark.parametrize("fmt", [kv8.E4M3, kv8.INT8])
 def test_evict_any_list(gpu, fmt):
     """Half-full and empty pages in the middle of a list, pages that two lists share; the
