@@ -4,6 +4,12 @@
 //
 // A list's pages may hold fewer tokens than they have places, any of them: a group of
 // 64 tokens is masked where one of its chunks is not full, which the wave votes on.
+//
+// What bounds it: a group's turning into halves and its exponentials (vector units), LDS,
+// and the products (matrix units), in turn.  bf16, 32 query heads on 8 of 128: 4096
+// queries over 8192 tokens 546 us, 1007 TFLOP/s (a large bf16 matrix product reaches 1356
+// here); 16 requests of 1 to 300 queries over 200 to 3000 tokens, int8, 130 us, where the
+// longest lists' 47 groups in turn end the launch.
 #include "kv8_prompt_block.h"
 
 namespace dsdk {
