@@ -87,7 +87,53 @@ struct Search {
 // kPacked: all pages but the last are full, so place i is token i.
 template <int kHeld, bool kPacked>
 __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search& f,
-                                             SelectLds& lds);
+                                             const float* weights, SelectLds& lds);
+
+// kBatch tiles are read at a time, without a branch between them (beyond the list: its
+// last place again), so that their loads are on their way together.
+constexpr int kBatch = 8;
+struct Places {
+  int page[kBatch], off[kBatch];
+};
+__device__ __forceinline__ Places ReadPlaces(const Kv8EvictArgs& a, int list, int places, int base,
+                                             int j0) {
+  const Kv8View& c = a.c;
+  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
+  Places x;
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) {
+    const int at = min(base + (j0 + k) * kWave, places - 1);
+    const int slot = c.chunks == 1 ? at >> 4 : static_cast<int>(__umulhi(at >> 4, inverse));
+    x.off[k] = at - slot * c.page;
+    x.page[k] = a.b.page_ids[list + slot];
+  }
+  return x;
+}
+__device__ __forceinline__ float ReadWeight(const Kv8EvictArgs& a, int head, int page, int off) {
+  const int64_t at = InPool(page, a.c.capacity) ? page : 0;
+  return a.weights[(at * a.c.heads + head) * a.c.page + off];
+}
+// Of all a wave's tiles, the next batch's pages beside a batch's weights.
+template <int kHeld>
+__device__ __forceinline__ void ReadWeights(const Kv8EvictArgs& a, int list, int head, int places,
+                                            int tiles, float* weights) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int base = wave * tiles * kWave + lane;
+  Places x = ReadPlaces(a, list, places, base, 0);
+#pragma unroll
+  for (int j0 = 0; j0 < kHeld; j0 += kBatch) {
+    if (j0 >= tiles) break;
+    const Places y = x;
+    if (j0 + kBatch < kHeld) x = ReadPlaces(a, list, places, base, j0 + kBatch);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) weights[j0 + k] = ReadWeight(a, head, y.page[k], y.off[k]);
+  }
+}
+// The tokens of a list's last page.
+__device__ __forceinline__ int LastCount(const Kv8EvictArgs& a, const Kv8Request& q) {
+  const int page = a.b.page_ids[q.list + q.pages - 1];
+  return InPool(page, a.c.capacity) ? min(max(a.c.token_counts[page], 0), a.c.page) : 0;
+}
 
 // Grid (key heads, batch).  kHeld: tiles of 64 places that a wave holds in registers; of
 // longer lists the weights are read again for each pass.
@@ -104,6 +150,11 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
     }
     return;
   }
+  for (int i = threadIdx.x; i < kBins; i += kSelectThreads) lds.bins[i] = 0;
+  const int places = q.pages * c.page;
+  const int tiles = ((places + kWave - 1) / kWave + kSelectWaves - 1) / kSelectWaves;
+  float weights[kHeld];  // (on their way beside the pages' counts)
+  if (places > 0 && tiles <= kHeld) ReadWeights<kHeld>(a, q.list, head, places, tiles, weights);
   // Tokens before each thread's pages, and where the first and the last ones lie.
   auto count_of = [&](int slot) {
     const int page = a.b.page_ids[q.list + slot];
@@ -126,86 +177,74 @@ __global__ __launch_bounds__(kSelectThreads) void Kv8EvictSelectKernel(Kv8EvictA
     lds.first_end = 0;
     lds.recent_begin = 0x7fffffff;
   }
+  const int behind = q.pages > 0 ? LastCount(a, q) : 0;
   const bool packed = __syncthreads_and(full) != 0;
-  int held;
-  int rank = BlockBefore(mine, lds.wave_sums, &held);
-  const bool all = held <= a.keep;
-  if (!all && packed) {
-    if (threadIdx.x == 0) {
-      lds.first_end = a.first;
-      if (a.recent > 0) lds.recent_begin = held - a.recent;
+  int held = packed ? max(q.pages - 1, 0) * c.page + behind : 0;
+  int first_end = 0, recent_begin = 0x7fffffff;
+  if (packed) {
+    if (held > a.keep) {
+      first_end = a.first;
+      if (a.recent > 0) recent_begin = held - a.recent;
     }
-  } else if (!all) {
-    const int from = held - a.recent;  // the rank of the first of the last
+  } else {
+    int rank = BlockBefore(mine, lds.wave_sums, &held);
+    const bool all = held <= a.keep;
+    const int from = all ? held : held - a.recent;  // the rank of the first of the last
     for (int s = s0; s < s1; ++s) {
       const int n = count_of(s);
-      if (rank < a.first && a.first <= rank + n) lds.first_end = s * c.page + a.first - rank;
+      if (!all && rank < a.first && a.first <= rank + n) lds.first_end = s * c.page + a.first - rank;
       if (rank <= from && from < rank + n) lds.recent_begin = s * c.page + from - rank;
       rank += n;
     }
+    __syncthreads();
+    first_end = lds.first_end;
+    recent_begin = lds.recent_begin;
   }
-  __syncthreads();
   const int count = min(held, a.keep);
   if (threadIdx.x == 0 && head == 0) {
     a.kept_tokens[r] = count;
     a.new_counts[r] = (count + c.page - 1) / c.page;
   }
-
-  const int places = q.pages * c.page;
-  const int tiles = ((places + kWave - 1) / kWave + kSelectWaves - 1) / kSelectWaves;
-  const Search f = {q, head, r, places, tiles, lds.first_end, lds.recent_begin, count, held};
+  const Search f = {q, head, r, places, tiles, first_end, recent_begin, count, held};
   if (tiles <= kHeld) {
-    packed ? SelectPlaces<kHeld, true>(a, f, lds) : SelectPlaces<kHeld, false>(a, f, lds);
+    packed ? SelectPlaces<kHeld, true>(a, f, weights, lds)
+           : SelectPlaces<kHeld, false>(a, f, weights, lds);
   } else {
-    packed ? SelectPlaces<0, true>(a, f, lds) : SelectPlaces<0, false>(a, f, lds);
+    packed ? SelectPlaces<0, true>(a, f, weights, lds) : SelectPlaces<0, false>(a, f, weights, lds);
   }
 }
 
 // Wave w has the w-th `tiles` tiles of 64 places, lane l place l of each.
 template <int kHeld, bool kPacked>
 __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search& f,
-                                             SelectLds& lds) {
+                                             const float* weights, SelectLds& lds) {
   const Kv8View& c = a.c;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int tiles = f.tiles;
   const int base = wave * tiles * kWave + lane;
 
-  // kBatch tiles are read at a time, without a branch between them (beyond the list: its
-  // last place again), so that their loads are on their way together.
-  constexpr int kBatch = 8;
-  const unsigned inverse = 0xffffffffu / static_cast<unsigned>(c.chunks) + 1u;
-  auto read = [&](int j0, unsigned* p) {
-    int page[kBatch], off[kBatch];
-    float w[kBatch];
+  auto key_of = [&](int j, float w, bool counted) {
+    const int at = base + j * kWave;
+    const bool there = j < tiles && (kPacked ? at < f.held : at < f.places && counted);
+    return !there ? kGone : (at < f.first_end || at >= f.recent_begin ? kAlways : KeyOf(w));
+  };
+  // (the pages' counts where not all are full)
+  auto counts = [&](const Places& x, bool* counted) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int at = min(base + (j0 + k) * kWave, f.places - 1);
-      const int slot = c.chunks == 1 ? at >> 4 : static_cast<int>(__umulhi(at >> 4, inverse));
-      off[k] = at - slot * c.page;
-      page[k] = a.b.page_ids[f.q.list + slot];
-    }
-    int count[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const bool ok = InPool(page[k], c.capacity);
-      const int64_t at = ok ? page[k] : 0;
-      w[k] = a.weights[(at * c.heads + f.head) * c.page + off[k]];
-      if constexpr (!kPacked) count[k] = ok ? c.token_counts[at] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int at = base + (j0 + k) * kWave;
-      const bool there = kPacked ? at < f.held : at < f.places && off[k] < count[k];
-      p[k] = !there || j0 + k >= tiles
-                 ? kGone
-                 : (at < f.first_end || at >= f.recent_begin ? kAlways : KeyOf(w[k]));
+      const bool ok = InPool(x.page[k], c.capacity);
+      counted[k] = x.off[k] < (ok ? c.token_counts[x.page[k]] : 0);
     }
   };
   unsigned keys[kHeld > 0 ? kHeld : 1];
   if constexpr (kHeld > 0) {
 #pragma unroll
     for (int j0 = 0; j0 < kHeld; j0 += kBatch) {
-      if (j0 < tiles) read(j0, keys + j0);
+      if (j0 >= tiles) break;
+      bool counted[kBatch] = {};
+      if constexpr (!kPacked) counts(ReadPlaces(a, f.q.list, f.places, base, j0), counted);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) keys[j0 + k] = key_of(j0 + k, weights[j0 + k], counted[k]);
     }
   }
   // with(j, key) for the wave's tiles in order.
@@ -217,46 +256,39 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
       }
     } else {
       for (int j0 = 0; j0 < tiles; j0 += kBatch) {
-        unsigned p[kBatch];
-        read(j0, p);
+        const Places x = ReadPlaces(a, f.q.list, f.places, base, j0);
+        float w[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) with(j0 + k, p[k]);
+        for (int k = 0; k < kBatch; ++k) w[k] = ReadWeight(a, f.head, x.page[k], x.off[k]);
+        bool counted[kBatch] = {};
+        if constexpr (!kPacked) counts(x, counted);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) with(j0 + k, key_of(j0 + k, w[k], counted[k]));
       }
     }
   };
 
   // The count-th best place: of those whose digits so far are its own the next digit is
-  // counted, until few are left, which rank themselves.
+  // counted, until few are left.
   unsigned key = f.count > 0 ? kGone : kAlways;  // (all are kept, or none)
   int last = -1;  // of the places with its key the last that is kept
   if (f.count > 0 && f.count < f.held) {
     int left = f.count;
-    unsigned key_known = 0, key_mask = 0;  // the digits so far, and which bits they are
-    unsigned place_known = 0, place_mask = 0;
-    auto matches = [&](unsigned p, unsigned turned) {
-      return p != kGone && (p & key_mask) == key_known && (turned & place_mask) == place_known;
-    };
+    unsigned known = 0, place_known = 0;  // the key's digits so far, then the turned place's
+    int few = 0;
     auto turned_place = [&](int j) { return 0x7fffffffu - static_cast<unsigned>(base + j * kWave); };
-#pragma unroll 1
-    for (int step = 0;; ++step) {
-      // bits 21.., 10.., 0.. of the key (11, 11, 10 of them), then 20.., 9.., 0.. of the
-      // place turned (11, 11, 9)
-      const bool by_key = step < 3;
-      const int shift = by_key ? max(21 - 11 * step, 0) : max(20 - 11 * (step - 3), 0);
-      const int width = step == 2 ? 10 : (step == 5 ? 9 : kDigit);
-      for (int i = threadIdx.x; i < kBins; i += kSelectThreads) lds.bins[i] = 0;
+    // One digit: with(j, key, &bin) says which are counted.
+    auto digit = [&](auto&& with) {
       if (threadIdx.x == 0) lds.few = 0;
-      __syncthreads();
       each([&](int j, unsigned p) {
-        const unsigned turned = turned_place(j);
-        if (matches(p, turned)) {
-          atomicAdd(&lds.bins[((by_key ? p : turned) >> shift) & ((1u << width) - 1u)], 1);
-        }
+        unsigned bin;
+        if (with(j, p, &bin)) atomicAdd(&lds.bins[bin], 1);
       });
       __syncthreads();
-      // thread t: bins kBins - 1 - 2 t and the one below it
+      // thread t: bins kBins - 1 - 2 t and the one below it, cleared for the next digit
       const int b0 = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
       const int n0 = lds.bins[b0], n1 = lds.bins[b0 - 1];
+      lds.bins[b0] = lds.bins[b0 - 1] = 0;
       int sum;
       const int above = BlockBefore(n0 + n1, lds.wave_sums, &sum);
       if (above < left && left <= above + n0 + n1) {
@@ -267,13 +299,13 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
       }
       __syncthreads();
       left -= lds.found_above;
-      (by_key ? key_known : place_known) |= lds.found_digit << shift;
-      (by_key ? key_mask : place_mask) |= ((1u << width) - 1u) << shift;
-      const int few = lds.found_count;
-      if (few > kFew) continue;  // (places differ: the last step leaves one)
+      few = lds.found_count;
+      return lds.found_digit;
+    };
+    // Those that are left rank themselves.
+    auto finish = [&](auto&& with) {
       each([&](int j, unsigned p) {
-        const unsigned turned = turned_place(j);
-        if (matches(p, turned)) lds.list[atomicAdd(&lds.few, 1)] = make_uint2(p, turned);
+        if (with(j, p)) lds.list[atomicAdd(&lds.few, 1)] = make_uint2(p, turned_place(j));
       });
       __syncthreads();
       if (static_cast<int>(threadIdx.x) < few) {
@@ -292,7 +324,43 @@ __device__ __forceinline__ void SelectPlaces(const Kv8EvictArgs& a, const Search
       __syncthreads();
       key = lds.found_digit;
       last = lds.found_above;
-      break;
+    };
+    // Bits 21.., 10.., 0.. of the key (11, 11, 10 of them; kGone alone has a first digit of 0).
+    known = digit([&](int, unsigned p, unsigned* bin) {
+      *bin = p >> 21;
+      return p != kGone;
+    });
+    int shift = 21;
+#pragma unroll 1
+    while (few > kFew && shift > 0) {
+      const int next = max(shift - kDigit, 0);
+      const unsigned found = digit([&](int, unsigned p, unsigned* bin) {
+        *bin = (p >> next) & ((1u << (shift - next)) - 1u);
+        return p >> shift == known;
+      });
+      known = known << (shift - next) | found;
+      shift = next;
+    }
+    if (few <= kFew) {
+      finish([&](int, unsigned p) { return p >> shift == known; });
+    } else {
+      // many of one key: bits 20.., 9.., 0.. of the turned place (11, 11, 9); places differ,
+      // so the last digit leaves one
+      shift = 31;
+#pragma unroll 1
+      while (few > kFew) {
+        const int next = max(shift - kDigit, 0);
+        const unsigned found = digit([&](int j, unsigned p, unsigned* bin) {
+          const unsigned turned = turned_place(j);
+          *bin = (turned >> next) & ((1u << (shift - next)) - 1u);
+          return p == known && turned >> shift == place_known;
+        });
+        place_known = place_known << (shift - next) | found;
+        shift = next;
+      }
+      finish([&](int j, unsigned p) {
+        return p == known && turned_place(j) >> shift == place_known;
+      });
     }
   }
 
