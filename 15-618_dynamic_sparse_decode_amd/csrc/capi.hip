@@ -3198,8 +3198,7 @@ void RequireQueryRows(const dsd_kv8_batch* b, int q_heads) {
 void RequireSizes(const dsd_kv8* cache, const dsd_kv8_batch* batch, int q_heads, const size_t* bytes) {
   Require(cache != nullptr && batch != nullptr && bytes != nullptr,
           "cache, batch and bytes must be non-null");
-  Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0 &&
-              batch->total_pages >= 0,
+  Require(batch->batch >= 0 && batch->max_tokens >= 0 && batch->max_pages >= 0,
           "sizes must be non-negative");
   RequireHeads(cache, q_heads);
   RequireQueryRows(batch, q_heads);
@@ -3541,6 +3540,7 @@ int dsd_kv8_weigh_workspace_bytes(const dsd_kv8* cache, const dsd_kv8_batch* bat
                                   int num_q_heads, size_t* bytes) {
   return Guard([&] {
     RequireSizes(cache, batch, num_q_heads, bytes);
+    Require(batch->total_pages >= 0, "sizes must be non-negative");
     *bytes = num_q_heads > 0 ? dsdk::Kv8WeighWorkspaceBytes(cache->view, *batch, num_q_heads) : 0;
   });
 }

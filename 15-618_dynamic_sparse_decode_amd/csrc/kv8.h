@@ -1,5 +1,6 @@
-// kv8.h -- the 8-bit paged cache (dsd_kv8_*): launch interface of
-// kv8_append.hip, kv8_attend.hip, kv8_prompt.hip and kv8_cross.hip.
+// kv8.h -- the 8-bit paged cache (dsd_kv8_*): launch interface of kv8_append.hip,
+// kv8_attend.hip, kv8_prompt.hip, kv8_cross.hip, kv8_shared.hip, kv8_weigh.hip and
+// kv8_evict.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>

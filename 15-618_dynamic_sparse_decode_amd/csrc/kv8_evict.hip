@@ -12,7 +12,7 @@
 // rounded once to it.
 //
 // What bounds it: the selection is a chain (weights, counts, a digit, counts again) in one
-// workgroup a list and key head: 13 us for one list of 4300 tokens, 45 for 32 of 32768 (8
+// workgroup a list and key head: 10.5 us for one list of 4300 tokens, 45 for 32 of 32768 (8
 // key heads; 36 MB of weights).  The move is bound by HBM: kept tokens lie apart and a
 // value's load is 16 tokens of one dim, so 32 lists cut to 4096 touch 0.84 GB for 0.27 GB
 // that are kept and write 0.27, 285 us.
