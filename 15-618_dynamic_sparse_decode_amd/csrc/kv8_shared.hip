@@ -220,7 +220,7 @@ SharedPlan MakePlan(const Kv8AttendArgs& own, const dsd_kv8_prefix& prefix) {
 int64_t Items(const Kv8View& c, const Plan& p, const dsd_kv8_batch& b) {
   return static_cast<int64_t>(c.heads) * p.blocks * b.batch * p.pieces;
 }
-constexpr int64_t kMostItems = 0x800000;
+constexpr int64_t kMostItems = 0xffffff;
 
 size_t SlotBytes(const Kv8View& c) { return sizeof(float) * c.dim + sizeof(PieceStats); }
 
@@ -294,8 +294,7 @@ void PreloadType(const Kv8View& c) {
 
 bool Kv8SharedFits(const Kv8AttendArgs& a, const dsd_kv8_prefix& prefix) {
   const SharedPlan m = MakePlan(a, prefix);
-  return Items(a.c, m.s.pre_plan, m.s.pre.b) <= kMostItems &&
-         Items(a.c, m.s.own_plan, a.b) <= kMostItems;
+  return Items(a.c, m.s.pre_plan, m.s.pre.b) + Items(a.c, m.s.own_plan, a.b) <= kMostItems;
 }
 
 size_t Kv8SharedBytes(const Kv8View& c, const dsd_kv8_batch& b, const dsd_kv8_prefix& prefix,
