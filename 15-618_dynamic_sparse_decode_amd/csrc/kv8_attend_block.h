@@ -132,7 +132,7 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
   // here and there among the reads costs HBM a fifth of its rate, bursts of them a
   // twentieth (16 bytes read a byte written, alone: 459 us for 2 GiB and 413 of 341
   // without writes; 355 where the reads leave the caches alone besides).
-  const int tile_rows = min(p.group - first, 16);
+  const int tile_rows = kWeigh ? min(p.group - first, 16) : 16;
   const int most_held = kSlotFloats / (64 * tile_rows);
   float* kept = lds + (sizeof(PageInfo) * kStage / sizeof(float)) + wave * kSlotFloats;
   int held = 0;
