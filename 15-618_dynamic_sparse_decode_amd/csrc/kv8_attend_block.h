@@ -31,7 +31,9 @@ constexpr int kSlotFloats = 4096;
 // four][4 chunks of 16][rows of the key head][4], so that a wave's store of one of its
 // four tiles is 64 bytes and more a chunk side by side, whole lines (rows of a head's
 // tokens each in a line of its own took 497 us in place of the figure in kv8_weigh.hip).
-// A list's first block is a whole one of its own.
+// A list's first block is a whole one of its own.  Lists that begin no earlier than those
+// before them end have blocks that no other writes; one behind a fall of page_offsets may
+// name entries of an earlier one and keeps no logits (LaterList).
 __host__ __device__ inline int64_t LogitBlocks(const Kv8AttendArgs& a) {
   return static_cast<int64_t>(a.b.total_pages) * a.c.page / 64 + a.b.batch + 1;
 }
@@ -39,6 +41,17 @@ __device__ __forceinline__ int64_t LogitBlock(const Kv8AttendArgs& a, const Plan
                                               int list, int block) {
   const int64_t first = static_cast<int64_t>(list) * a.c.page / 64 + r;
   return (head * LogitBlocks(a) + first + block) * 64 * p.group;
+}
+// Not 0 in some lane of the wave: page_offsets falls before request r's entry.
+__device__ __forceinline__ int LaterList(const dsd_kv8_batch& b, int r) {
+  if (b.list_stride > 0 || r == 0) return 0;
+  const int lane = threadIdx.x & (kWave - 1), i = min(lane, r - 1);
+  int fell = b.page_offsets[i + 1] < b.page_offsets[i] ? 1 : 0;
+#pragma unroll 8
+  for (int j = kWave + lane; j < r; j += kWave) {
+    fell |= b.page_offsets[j + 1] < b.page_offsets[j] ? 1 : 0;
+  }
+  return fell;
 }
 
 // One piece of request r's list for one tile of 16 rows (unit: key heads * row tiles,
@@ -51,11 +64,13 @@ __device__ __forceinline__ int64_t LogitBlock(const Kv8AttendArgs& a, const Plan
 // is free), whose first operand, 16 tokens of one dim, is one load of the
 // values' layout.  No number crosses lanes but for the maxima.
 // kJoin: a later launch joins the piece with others.  kWeigh: logits (times log2 e) go
-// to `logits` as well, and the rows' sums to p.stats.
+// to `logits` as well, unless a lane's `later` says that the list has no place there,
+// and the rows' sums to p.stats.
 // kDim: head_dim where it is 64 * NU (no bounds tests), else 0.
 template <typename T, int FMT, int NU, int kDim, int W, bool kJoin, bool kWeigh = false>
 __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& p, int unit, int r,
-                                            int piece, float* lds, float* logits = nullptr) {
+                                            int piece, float* lds, float* logits = nullptr,
+                                            int later = 0) {
   constexpr int NQ = kQueryTerms<T>, NP = kWeightTerms<T>, NT = 4 * NU;
   // The loads of a wave's last group are issued too (its own once more): a wait for the
   // values then counts the next keys and the stores, whichever path led there, and does
@@ -138,7 +153,8 @@ __device__ __forceinline__ void AttendBlock(const Kv8AttendArgs& a, const Plan& 
   int held = 0;
   auto flush = [&](int last) {  // blocks last, last - W, ...
     const int quads = 16 * tile_rows;
-    for (int i = 0; i < held; ++i) {
+    const int some = __ballot(later != 0) == 0 ? held : 0;
+    for (int i = 0; i < some; ++i) {
       float* to = logits + LogitBlock(a, p, head, r, s.q.list, last - (held - 1 - i) * W) + first * 4;
       const float* from = kept + i * 64 * tile_rows;
       for (int e = lane; e < quads; e += kWave) {

@@ -8,6 +8,8 @@
 // attention writes them to the workspace and a second launch turns them into weights.
 // Sums over a group's heads are float32, in order; a token's own sum takes one atomic
 // addition (a page that several requests list gets all of theirs, in any order).
+// Logits lie by their list's place in page_ids.  Where page_offsets falls, a list behind
+// may name entries of one before: its logits are formed a second time instead.
 //
 // What bounds it: HBM.  32 requests of 32768 tokens, 32 query heads on 8 of 128, bf16:
 // attention 460 us for 2.15 GB of codes and 134 MB of logits, where reads alone reach
@@ -23,14 +25,87 @@ template <typename T, int FMT, int NU, int kDim>
 __global__ __launch_bounds__(kAttendWaves* kWave, NU <= 2 ? 2 : 1) void Kv8AttendLogitsKernel(
     Kv8AttendArgs a, Plan p, float* logits) {
   extern __shared__ __align__(16) float lds[];
-  AttendBlock<T, FMT, NU, kDim, kAttendWaves, false, true>(a, p, blockIdx.x, blockIdx.y, blockIdx.z,
-                                                           lds, logits);
+  AttendBlock<T, FMT, NU, kDim, kAttendWaves, false, true>(
+      a, p, blockIdx.x, blockIdx.y, blockIdx.z, lds, logits, LaterList(a.b, blockIdx.y));
 }
 
-// Grid (shares of a list, key heads, batch): a wave has kBlocks blocks of 64 tokens at a
-// time on their way, lane l their place l; the first ones' logits and pages are asked for
-// before the rows' sums are formed.
+// A logit (times log2 e) from the query and the codes, in 64 bits: of lists that the
+// attention kept none of.  Element i of the queries, byte c of the codes.
+__device__ __forceinline__ double QueryNumber(const Kv8AttendArgs& a, int64_t i) {
+  switch (a.type) {
+    case DSD_TYPE_F32: return static_cast<double>(static_cast<const float*>(a.q)[i]);
+    case DSD_TYPE_BF16: return static_cast<double>(static_cast<float>(static_cast<const __bf16*>(a.q)[i]));
+    default: return static_cast<double>(static_cast<float>(static_cast<const _Float16*>(a.q)[i]));
+  }
+}
+__device__ __forceinline__ float LogitOf(const Kv8AttendArgs& a, int64_t query, int64_t key, float scale) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int d = 0; d < a.c.dim; ++d) {
+    const uint8_t c = a.c.keys[key + d];
+    const double k = a.c.format == DSD_KV8_INT8
+                         ? static_cast<double>(static_cast<int8_t>(c))
+                         : static_cast<double>(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c), 0));
+    sum = fma(QueryNumber(a, query + d), k, sum);
+  }
+  return static_cast<float>(sum * static_cast<double>(scale) * (static_cast<double>(a.scale) * kLog2e));
+}
+
 constexpr int kRowTile = 64;
+
+// Maxima and reciprocal sums of rows [row0, row0 + rows) of a key head.
+__device__ __forceinline__ void RowSums(const Kv8AttendArgs& a, const Plan& p, int r, int head, int row0,
+                                        int rows, int pieces, float* row_base, float* row_inv) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  for (int i = wave; i < rows; i += 4) {
+    PieceStats st = {-INFINITY, -1.0f, 0.0f};
+    if (lane < pieces) st = p.stats[PartSlot(p, a.c.heads, r, head, row0 + i) + lane];
+    const bool some = !(st.l < 0.0f);
+    float peak = some ? st.m : -INFINITY;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
+    const float base = peak == -INFINITY ? 0.0f : peak;
+    float sum = some ? st.l * Exp2(st.m - base) : 0.0f;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+    if (lane == 0) {
+      row_base[i] = base;
+      row_inv[i] = 1.0f / sum;
+    }
+  }
+}
+
+// All of a list's weights by one workgroup of 256, the logits formed again.
+__device__ __forceinline__ void WeighAgain(const Kv8AttendArgs& a, const Plan& p, const Span& s, int r,
+                                           int head, float* row_base, float* row_inv, float* weights) {
+  const Kv8View& c = a.c;
+  for (int row0 = 0; row0 < p.group; row0 += kRowTile) {
+    const int rows = min(kRowTile, p.group - row0);
+    __syncthreads();
+    RowSums(a, p, r, head, row0, rows, Pieces(p, s), row_base, row_inv);
+    __syncthreads();
+#pragma unroll 1
+    for (int slot = 0; slot < s.q.pages; ++slot) {
+      const int page = a.b.page_ids[s.q.list + slot];
+      const int count = InPool(page, c.capacity) ? min(c.token_counts[page], c.page) : 0;
+      const int64_t pair = static_cast<int64_t>(page) * c.heads + head;
+      for (int at = threadIdx.x; at < count; at += 256) {
+        float w = 0.0f;
+#pragma unroll 1
+        for (int i = 0; i < rows; ++i) {
+          const int64_t query = r * a.q_stride + static_cast<int64_t>(head * p.group + row0 + i) * c.dim;
+          const float x = LogitOf(a, query, (pair * c.page + at) * c.dim, c.key_scales[pair]);
+          w = fmaf(Exp2(x - row_base[i]), row_inv[i], w);
+        }
+        unsafeAtomicAdd(weights + pair * c.page + at, w);
+      }
+    }
+  }
+}
+
+// Grid (shares of a list and one more, key heads, batch): a wave has kBlocks blocks of 64
+// tokens at a time on their way, lane l their place l; the first ones' logits and pages are
+// asked for before the rows' sums are formed.  The last share has the lists without logits.
 constexpr int kBlocks = 4;
 constexpr int kFirstRows = 4;
 __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, const float* logits,
@@ -38,8 +113,14 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
   __shared__ float row_base[kRowTile], row_inv[kRowTile];
   const Kv8View& c = a.c;
   const int r = blockIdx.z, head = blockIdx.y;
+  const int shares = static_cast<int>(gridDim.x) - 1;
+  const int later = LaterList(a.b, r);
   Span s;
   if (!FindSpan(a, p.group, r, 0, p.group, &s)) return;
+  if (static_cast<int>(blockIdx.x) == shares) {
+    if (__ballot(later != 0) != 0) WeighAgain(a, p, s, r, head, row_base, row_inv, weights);
+    return;
+  }
   const int blocks = (s.chunks + 3) / 4;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int first = static_cast<int>(blockIdx.x) * 4 * kBlocks;
@@ -71,24 +152,10 @@ __global__ __launch_bounds__(256) void Kv8WeighKernel(Kv8AttendArgs a, Plan p, c
     int b0 = first + wave * kBlocks;
     fetch(min(b0, blocks - 1));
     __syncthreads();
-    for (int i = wave; i < rows; i += 4) {
-      PieceStats st = {-INFINITY, -1.0f, 0.0f};
-      if (lane < pieces) st = p.stats[PartSlot(p, c.heads, r, head, row0 + i) + lane];
-      const bool some = !(st.l < 0.0f);
-      float peak = some ? st.m : -INFINITY;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) peak = fmaxf(peak, __shfl_xor(peak, o, kWave));
-      const float base = peak == -INFINITY ? 0.0f : peak;
-      float sum = some ? st.l * Exp2(st.m - base) : 0.0f;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-      if (lane == 0) {
-        row_base[i] = base;
-        row_inv[i] = 1.0f / sum;
-      }
-    }
+    RowSums(a, p, r, head, row0, rows, pieces, row_base, row_inv);
     __syncthreads();
-    for (; b0 < blocks; b0 += gridDim.x * 4 * kBlocks) {
+    if (__ballot(later != 0) != 0) return;
+    for (; b0 < blocks; b0 += shares * 4 * kBlocks) {
       if (b0 != first + wave * kBlocks) fetch(b0);
       int count[kBlocks];
 #pragma unroll
@@ -162,7 +229,7 @@ void Launch(const Kv8AttendArgs& a, float* weights, hipStream_t stream) {
   DSD_HIP_CHECK(hipGetLastError());
   Merge<T>(a, p, stream);
   const int64_t shares = (ListGroups(a.c, a.b) + 4 * kBlocks - 1) / (4 * kBlocks);
-  const dim3 over(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(shares, 1), 65536)),
+  const dim3 over(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(shares, 1), 65536)) + 1,
                   a.c.heads, a.b.batch);
   Kv8WeighKernel<<<over, 256, 0, stream>>>(a, p, logits, weights);
   DSD_HIP_CHECK(hipGetLastError());

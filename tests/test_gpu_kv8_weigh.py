@@ -260,3 +260,61 @@ def test_weigh_replayed_and_on_streams(gpu):
         assert torch.equal(o, outs[i])
         add, may = model_weights(pair, lists, "bf16", inputs[i])
         check_weights(torch.zeros_like(w), w, add, may)
+
+
+@pytest.mark.parametrize("fmt", [kv8.E4M3, kv8.INT8])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 16), (70, 1, 64, 48), (4, 2, 256, 64)])
+def test_weigh_beside_malformed_offsets(gpu, heads, kv, dim, page, kind, fmt):
+    """page_offsets that fall: the request they fall in is reported and has no token, all
+    others get their outputs and add their weights, though their lists overlap.  The logits
+    of one behind a fall are formed from the codes in 64 bits and rounded once, which
+    model_weights' bound holds."""
+    import torch
+    rng = np.random.default_rng(dim)
+    pair = Pair(gpu, kv, dim, page, 126, fmt)
+    pair.fill(dim + fmt)
+    for at, count in ((3, 5), (40, 0), (70, 1), (90, page - 1)):
+        pair.set_counts(at, count)
+    ids = rng.permutation(126)[:120].tolist()
+    ids[65] = 500  # (a page outside the cache)
+    for offsets in ([0, 100, 60, 120], [60, 120, 0, 50, 40, 120], [0, 500, 30, 80], [3, 3, 1, 120],
+                    [0] + [7 * i for i in range(1, 9)] + [119, 63, 70, 80, 120, 120]):
+        lists = [ids[a:b] if 0 <= a <= b <= 120 else [] for a, b in zip(offsets, offsets[1:])]
+        lists = [[p for p in l if p != 500] for l in lists]
+        batch = Batch(gpu, [ids] + [[]] * (len(lists) - 1))
+        batch.keep["page_offsets"].copy_(device(offsets))
+        q = rows(rng, kind, len(lists), heads, dim)
+        add, may = model_weights(pair, lists, kind, q)
+        before = sums(pair, rng)
+        weights, out = before.clone(), torch.full_like(q, 9.0)
+        fail = torch.zeros(1, dtype=torch.int64, device="cuda")
+        weigh(pair, batch, kind, q, out, weights, fail=fail)
+        assert int(fail) & 0xffffffff in (2, 3), offsets
+        check_attention(pair, Batch(gpu, lists), kind, q, out)
+        check_weights(before, weights, add, may)
+
+
+def test_weigh_many_requests_beside_a_malformed_one(gpu):
+    """More requests than a workgroup has threads, an entry far before the last too large
+    and one near it too small."""
+    import torch
+    rng = np.random.default_rng(77)
+    pair = Pair(gpu, 1, 64, 16, 700)
+    pair.fill(1)
+    ids = rng.permutation(700)[:600].tolist()
+    for wrong in ({5: 300}, {299: 0}, {2: 9000, 290: 100}):
+        offsets = [2 * i for i in range(301)]
+        for at, x in wrong.items():
+            offsets[at] = x
+        lists = [ids[a:b] if 0 <= a <= b <= 600 else [] for a, b in zip(offsets, offsets[1:])]
+        batch = Batch(gpu, [ids] + [[]] * 299)
+        batch.keep["page_offsets"].copy_(device(offsets))
+        q = rows(rng, "bf16", 300, 4, 64)
+        before = sums(pair, rng)
+        weights, out = before.clone(), torch.full_like(q, 9.0)
+        fail = torch.zeros(1, dtype=torch.int64, device="cuda")
+        weigh(pair, batch, "bf16", q, out, weights, fail=fail)
+        assert int(fail) & 0xffffffff == 2, wrong
+        check_attention(pair, Batch(gpu, lists), "bf16", q, out)
+        check_weights(before, weights, *model_weights(pair, lists, "bf16", q))
