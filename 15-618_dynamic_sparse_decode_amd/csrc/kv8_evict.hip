@@ -513,7 +513,7 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   const int waves = blockDim.x / kWave;
   const bool is_key = (wave & 1) == 0;
   auto chunk_of = [&](int u) { return wave / 2 + waves / 2 * u; };
-  // (loads that do not wait for each other)
+  // (on their way beside the list's; rows behind the last kept token are in the array too)
   const int* kept = a.kept + (static_cast<int64_t>(r) * c.heads + head) * a.keep + index * ps;
   int place[U];
 #pragma unroll
@@ -523,9 +523,10 @@ __global__ __launch_bounds__(512) void Kv8EvictMoveKernel(Kv8EvictArgs a) {
   }
   Kv8Request q;
   const bool listed = Kv8ReadList(a.b, r, &q);
-  const int page = a.new_ids[static_cast<int64_t>(r) * a.new_stride + index];
   const int count = min(a.kept_tokens[r] - index * ps, ps);
   if (count <= 0 || !listed) return;
+  // (the caller's array may end behind the last page that is filled)
+  const int page = a.new_ids[static_cast<int64_t>(r) * a.new_stride + index];
   if (!InPool(page, c.capacity)) {
     if (threadIdx.x == 0) ReportFailure(a.fail, kFailPageId);
     return;

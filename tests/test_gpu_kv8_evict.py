@@ -389,3 +389,24 @@ def test_serving_with_a_budget(gpu):
         torch.cuda.synchronize()
         want = model_evict(pair, mine.lists, 20, 1, 2, given, spare)
         check_evict(pair, mine.lists, spare, (weights, new_counts, kept), want, before)
+
+
+def test_evict_new_pages_behind_the_filled_ones(gpu):
+    """Entries of new_page_ids behind a list's filled pages may hold anything, and the
+    array may end behind the last list's."""
+    import torch
+    rng = np.random.default_rng(5)
+    pair = Pair(gpu, 2, 64, 16, 40)
+    pair.fill(6)
+    pair.set_counts(9, 3)
+    pair.set_counts(12, 15)
+    lists = [list(range(0, 5)), list(range(5, 10)), [10], [], [11, 12]]
+    new = [[20, 21, 22, 23], [24, 25, 26, 27], [28, -1, 1 << 30, -7], [99, 99, 99, 99], [29, 30, 77, -5]]
+    weights = some_weights(rng, pair.model, "spread")
+    given, before = weights.clone(), snapshot(pair)
+    fail = torch.zeros(1, dtype=torch.int64, device="cuda")
+    counts, kept = evict(pair, Batch(gpu, lists), 50, 1, 2, weights, device(new), fail=fail)
+    assert int(fail) == 0
+    want = model_evict(pair, lists, 50, 1, 2, given, new)
+    check_evict(pair, lists, new, (weights, counts, kept), want, before)
+    assert counts.tolist() == [4, 4, 1, 0, 2]
