@@ -7,9 +7,13 @@
 //
 // What bounds it: a group's turning into halves and its exponentials (vector units), LDS,
 // and the products (matrix units), in turn.  bf16, 32 query heads on 8 of 128: 4096
-// queries over 8192 tokens 546 us, 1007 TFLOP/s (a large bf16 matrix product reaches 1356
-// here); 16 requests of 1 to 300 queries over 200 to 3000 tokens, int8, 130 us, where the
-// longest lists' 47 groups in turn end the launch.
+// queries over 8192 tokens 546 us, 1007 TFLOP/s (557 on another card; a large bf16 matrix
+// product reaches 1356 here), f16 rows, whose weights take two terms, 725, float32 ones,
+// whose queries do too, 1255; 16 requests of 1 to 300 queries over 200 to 3000 tokens, int8,
+// 131 us a call (139 under a profiler), where the longest lists' 47 groups in turn end the
+// launch.  Heads of 144 to 256 spill: a wave has 32 rows of all dims in registers, 103 to
+// 173 of them in scratch, and 4096 over 8192 of 16 heads on 8 of 256 takes 2713 us, 203
+// TFLOP/s.
 #include "kv8_prompt_block.h"
 
 namespace dsdk {

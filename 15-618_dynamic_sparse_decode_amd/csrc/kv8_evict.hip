@@ -12,10 +12,12 @@
 // rounded once to it.
 //
 // What bounds it: the selection is a chain (weights, counts, a digit, counts again) in one
-// workgroup a list and key head: 10.5 us for one list of 4300 tokens, 45 for 32 of 32768 (8
-// key heads; 36 MB of weights).  The move is bound by HBM: kept tokens lie apart and a
-// value's load is 16 tokens of one dim, so 32 lists cut to 4096 touch 0.84 GB for 0.27 GB
-// that are kept and write 0.27, 285 us.
+// workgroup a list and key head: 10.5 us for one list of 4300 tokens, 44 for 32 of 32768 (8
+// key heads; 33.5 MB of weights).  The form that holds 32 tiles a wave spills 15 registers
+// of a lane (1024 threads have 128 each).  A longer list's ids and weights are read again in
+// each pass: a whole call that keeps 4096 of 32768 takes 49 us, of 33000 81, of 60000 119.
+// The move is bound by HBM: kept tokens lie apart and a value's load is 16 tokens of one
+// dim, so 32 lists cut to 4096 touch 0.84 GB for 0.27 GB that are kept and write 0.27, 280 us.
 #include "kv8_codes.h"
 
 #include <algorithm>

@@ -488,7 +488,8 @@ inline Plan PromptPlan(const Kv8View& c, const dsd_kv8_batch& b, int q_heads, in
   p.blocks = static_cast<int>((p.rows + block - 1) / block);
   const int64_t units = static_cast<int64_t>(c.heads) * p.blocks * b.batch;
   const int64_t most = kPromptTarget * kRows / block / std::max<int64_t>(units, 1);
-  // A group takes a workgroup about 1.5 us; pieces cost the second launch, 5 us,
+  // A group takes a workgroup about 1.5 us (a causal one of bf16 heads of 128, for all
+  // forms alike: others' take longer); pieces cost the second launch, 5 us,
   // and a write and a read of their sums at about 3 TB/s.
   const int64_t groups = ListGroups(c, b);
   const double rows = static_cast<double>(b.batch) * c.heads * static_cast<double>(p.rows);

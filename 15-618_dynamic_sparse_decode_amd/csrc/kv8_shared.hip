@@ -9,9 +9,11 @@
 //
 // What bounds it: for few rows a prefix HBM, for many the matrix and vector units.  bf16,
 // 32 query heads on 8 of 128: 8 requests behind 2000 tokens 10 us and 4.5 for the joining;
-// 64 behind 32768, own lists of 200 to 2000, 82 and 10 (36 us of bytes, 26 of products, and
+// 64 behind 32768, own lists of 200 to 2000, 81 and 10 (36 us of bytes, 26 of products, and
 // as much again of turning codes into halves, twice for 256 rows); float32, 32 / 32 heads,
-// 16 requests in 4 groups behind 4096 to 16384, 109 and 5.3, 5.4 TB/s.
+// 16 requests in 4 groups behind 4096 to 16384, 111 and 5.5, 5.3 TB/s.  Heads of 144
+// to 256 of many rows spill as kv8_cross.hip's do: the 64 behind 32768 of 16 heads on 8 of
+// 256 take 360 us a call.
 #include "kv8_attend_block.h"
 #include "kv8_prompt_block.h"
 
@@ -204,7 +206,9 @@ SharedPlan MakePlan(const Kv8AttendArgs& own, const dsd_kv8_prefix& prefix) {
   if (m.many) {
     // Blocks of 128 rows: one workgroup a CU beside the own lists' (a group of 64 tokens
     // 2.3 us) or two that the own lists' follow (2.45 us, which at 3.8 TB/s take what is
-    // left).  64 requests behind 32768 tokens, own lists of 200-2000: 82 and 93 us.
+    // left).  64 requests behind 32768 tokens, own lists of 200-2000: 82 and 93 us.  (Measured
+    // at bf16 heads of 128; other types' and sizes' groups take longer, which shifts where the
+    // two meet, not the results.)
     const double step = static_cast<double>(pre) / kPromptTarget;
     const double own_us = static_cast<double>(own_all) * 128 * c.dim / 3.8e6;
     const int64_t target = own_us > (2 * 2.3 - 2.45) * step ? kPromptTarget / 2 : kPromptTarget;

@@ -14,7 +14,7 @@
 // What bounds it: HBM.  32 requests of 32768 tokens, 32 query heads on 8 of 128, bf16:
 // attention 460 us for 2.15 GB of codes and 134 MB of logits, where reads alone reach
 // 6.3 TB/s and sixteen parts read to one written 5.0 to 5.35 (430 to 456 us); the weights
-// 55 us for 134 MB of logits read and 67 MB read and written; the whole call 539 us.
+// 60 us for 134 MB of logits read and 67 MB read and written; the whole call 538 us.
 #include "kv8_attend_block.h"
 
 namespace dsdk {
